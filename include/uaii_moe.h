@@ -417,6 +417,75 @@ UAII_MOE_API int uaii_moe_profile_enable(uaii_moe_backend* b, int enable);
 UAII_MOE_API int uaii_moe_profile_read(uaii_moe_backend* b, double* phase_ms, uint64_t* phase_calls,
                                        uint64_t* kernel_launches);
 
+/* ---- Serving operators around the decoder.  No reference counterpart: the reference keeps one f32 cache per
+ * session on the host (include/uaii/runtime/kv_cache.hpp:16-190) and attends to it one sequence at a time.  Every
+ * pointer is device memory of the backend's device; work is queued on the backend's stream and the calls return
+ * without waiting.  A position or length outside the cache, which only the device can see, is skipped (a length is
+ * clamped) and reported as UAII_MOE_INVALID_ARGUMENT by the next uaii_moe_synchronize. */
+
+/* Formats of a KV cache next to UAII_MOE_F16: one byte per value and one f32 scale per row, a row being the
+ * head_dim values x of one (sequence, kv head, position) of K or of V.  With a = max|x|:
+ *   UAII_MOE_KV_I8    scale = a / 127, byte = 128 + rint(x * (127 / a)), value = (byte - 128) * scale
+ *   UAII_MOE_KV_E4M3  scale = a / 448, byte = e4m3(x * (448 / a)),       value = e4m3^-1(byte) * scale
+ * (a / 127 and 127 / a each rounded to f32.)  A row with a < 2^-100 is kept as zeros; one with an infinity or a NaN
+ * gets a NaN scale. */
+#define UAII_MOE_KV_I8 32
+#define UAII_MOE_KV_E4M3 33
+
+/* One layer's cache, owned by the caller: k, v [batch, n_kv_heads, max_seq, head_dim] f16 or bytes, dense, 16-byte
+ * aligned; k_scale, v_scale f32 [batch, n_kv_heads, max_seq] (NULL for f16).  head_dim 64 or 128. */
+typedef struct uaii_moe_kv_cache {
+  int32_t fmt;
+  int32_t head_dim;
+  int64_t batch;
+  int64_t n_kv_heads;
+  int64_t max_seq;
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+} uaii_moe_kv_cache;
+
+/* Quantise K and V as they are written: token t < n_new[i] of sequence i (every t < n_tokens when n_new is NULL)
+ * goes to position pos[i] + t.  k and v are views [batch, n_tokens, n_kv_heads, head_dim] of f32 or f16 `dtype`
+ * (UAII_MOE_DTYPE_*) with a dense last dimension and the same element strides, for instance parts of one fused q/k/v
+ * projection. */
+UAII_MOE_API int uaii_moe_kv_append(uaii_moe_backend* b, const uaii_moe_kv_cache* cache, const void* k, const void* v,
+                                    int dtype, int64_t n_tokens, int64_t stride_batch, int64_t stride_token,
+                                    int64_t stride_head, const int32_t* pos, const int32_t* n_new);
+
+/* Positions [pos0, pos0 + n) of every sequence and head as values: k_out, v_out [batch, n_kv_heads, n, head_dim] of
+ * f32 or f16, dense, 16-byte aligned. */
+UAII_MOE_API int uaii_moe_kv_read(uaii_moe_backend* b, const uaii_moe_kv_cache* cache, int64_t pos0, int64_t n,
+                                  void* k_out, void* v_out, int dtype);
+
+/* Attention of n_tokens new tokens of each sequence over a prefix that all sequences share, read once for the whole
+ * batch, and each sequence's own positions.  The new tokens' K and V are the last n_tokens of the own_len[i] cached
+ * positions (append them first): token t of sequence i sees prefix positions [0, prefix_len) and own positions
+ * [0, own_len[i] - n_tokens + t], and gets zeros where it sees none.  prefix: a cache of batch 1, or NULL with
+ * prefix_len 0; same format, head_dim and n_kv_heads as `own`.  q: view [batch, n_tokens, n_heads, head_dim] of f32
+ * or f16 with a dense last dimension; n_heads a multiple of n_kv_heads, query head h reading kv head
+ * h / (n_heads / n_kv_heads).  scale 0 means 1 / sqrt(head_dim).  out [batch, n_tokens, n_heads, head_dim] of q's
+ * type, dense, 16-byte aligned. */
+UAII_MOE_API int uaii_moe_prefix_attention(uaii_moe_backend* b, const uaii_moe_kv_cache* prefix, int64_t prefix_len,
+                                           const uaii_moe_kv_cache* own, const int32_t* own_len, const void* q,
+                                           int dtype, int64_t n_heads, int64_t n_tokens, int64_t stride_batch,
+                                           int64_t stride_token, int64_t stride_head, float scale, void* out);
+
+/* One token per row of logits [batch, vocab] (f32 or f16, rows `ld` elements apart) from one uniform number u in
+ * [0, 1) per row.  With m = max(logits) and e_i = exp((l_i - m) / temperature), tokens are ranked by logit, the lower
+ * index first among equals.  Kept are the first top_k (0: all), of those the shortest leading part whose mass reaches
+ * top_p of theirs (1: all), and of those the tokens with e_i >= min_p (0: all); the first is always kept.  Masses are
+ * whole numbers w_i = rint(e_i * 2^31), so the result depends on no order of summation.  tokens[i] is the first kept
+ * index whose running mass over the kept indices, in index order, exceeds floor(u * mass(kept)); probs[i] =
+ * w / mass(kept) and kept[i] = the number of kept tokens (either may be NULL).  A temperature that is not above 0
+ * takes the first largest logit.  NaN logits count as -inf; a row without any other gives token -1, probability 0 and
+ * kept 0.  temperature, top_k, top_p, min_p, u: one per row.  Extends the reference's sampler
+ * (libs/uaii-runtime/src/sampling.cpp:22-128), which draws its own numbers and sorts on the host. */
+UAII_MOE_API int uaii_moe_sample(uaii_moe_backend* b, const void* logits, int dtype, int64_t batch, int64_t vocab,
+                                 int64_t ld, const float* temperature, const int32_t* top_k, const float* top_p,
+                                 const float* min_p, const float* u, int32_t* tokens, float* probs, int32_t* kept);
+
 /* ---- Batched greedy decode of a GGUF MoE transformer on the device.  Replaces the
  * reference's decode loop, Session::generate (libs/uaii-runtime/src/session.cpp:910-1046),
  * over the seq-1 transformer graph its GGUF loader builds

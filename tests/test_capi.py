@@ -84,3 +84,27 @@ def test_backend_create_reports_errors_without_crashing(um):
 def test_null_backend_is_invalid_argument(um):
     assert um.lib.uaii_moe_synchronize(None) == 1
     assert b"null backend" in um.lib.uaii_moe_last_error()
+
+
+def test_serving_entries_refuse_a_null_backend(um):
+    c = um.KVCache()
+    for st in (um.lib.uaii_moe_kv_append(None, ctypes.byref(c), None, None, 1, 1, 0, 0, 0, None, None),
+               um.lib.uaii_moe_kv_read(None, ctypes.byref(c), 0, 1, None, None, 1),
+               um.lib.uaii_moe_prefix_attention(None, None, 0, ctypes.byref(c), None, None, 1, 1, 1, 0, 0, 0, 0.0, None),
+               um.lib.uaii_moe_sample(None, None, 1, 1, 1, 1, None, None, None, None, None, None, None, None)):
+        assert st == um.INVALID_ARGUMENT and b"null backend" in um.lib.uaii_moe_last_error()
+
+
+def test_kv_cache_checks_types_and_shapes(um):
+    import torch
+    k, s = torch.zeros((1, 2, 8, 64), dtype=torch.uint8), torch.zeros((1, 2, 8))
+    c = um.kv_cache(um.KV_I8, k, k, s, s)
+    assert (c.fmt, c.head_dim, c.batch, c.n_kv_heads, c.max_seq) == (um.KV_I8, 64, 1, 2, 8)
+    with pytest.raises(TypeError):
+        um.kv_cache(um.KV_I8, k.float(), k, s, s)
+    with pytest.raises(ValueError):
+        um.kv_cache(um.KV_I8, k, k[:, :, :4], s, s)
+    with pytest.raises(ValueError):
+        um.kv_cache(um.KV_E4M3, k.transpose(1, 2), k.transpose(1, 2), s, s)
+    with pytest.raises(TypeError):
+        um.kv_cache(um.F16, k, k)

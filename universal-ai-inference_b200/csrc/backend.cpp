@@ -179,6 +179,10 @@ Error MoeCudaBackend::sync_and_check() {
   if (code != 0) {
     (void)cudaMemset(dev_err_, 0, sizeof(int));
     if (tail_.cnt) (void)cudaMemset(tail_.cnt, 0, sizeof(int) * (kTailMaxUnits + 16));  // a kernel may have stopped mid-tile
+    if (code == kErrKvPosition)
+      return Error::make(ErrorCode::InvalidArgument, "kv_append: a position lies outside the cache");
+    if (code == kErrKvLength)
+      return Error::make(ErrorCode::InvalidArgument, "prefix_attention: a sequence length lies outside its cache");
     return Error::make(ErrorCode::Internal,
                        "tensor-core expert kernel gave up waiting (code " + std::to_string(code) + ")");
   }

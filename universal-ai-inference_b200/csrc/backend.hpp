@@ -19,8 +19,10 @@
 #include <vector>
 
 #include "kernels.hpp"
+#include "serve_kernels.hpp"
 
 struct uaii_moe_layer;
+struct uaii_moe_kv_cache;
 
 namespace uaii_b200 {
 
@@ -139,6 +141,15 @@ class MoeCudaBackend {
                    bool y_f16 = false);
   Error ep_combine(const void* y_back, const int32_t* row_of, int64_t T, int world, int64_t D, float* y,
                    bool y_back_f16 = false);
+  // Serving operators (serve.cpp; device pointers only).  See include/uaii_moe.h.
+  Error kv_append(const KvCache& c, const void* k, const void* v, bool half, int64_t T, const RowView& s,
+                  const int32_t* pos, const int32_t* n_new);
+  Error kv_read(const KvCache& c, int64_t pos0, int64_t n, void* k_out, void* v_out, bool half);
+  Error prefix_attention(PrefixAttnArgs a);
+  Error sample(const void* logits, bool half, int64_t B, int64_t V, int64_t ld, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tokens,
+               float* probs, int32_t* kept);
+
   // Runs the bounded-wait self-test kernel and returns the status the host observes.
   Error selftest_wait_timeout(int64_t budget_cycles);
 
@@ -284,6 +295,8 @@ bool is_device_ptr(const void* p) noexcept;
 // The C ABI layer description (include/uaii_moe.h) as LayerArgs; false if a
 // required expert weight pointer is null.
 bool layer_args_from_c(const struct uaii_moe_layer* l, LayerArgs* out);
+// The C ABI's cache description, checked (`op` opens the messages).
+Error kv_cache_from_c(const char* op, const struct uaii_moe_kv_cache* s, KvCache* out);
 // Record `e` as this thread's last error (uaii_moe_last_error) and return its status code.
 int report_status(const Error& e);
 Error cuda_status(cudaError_t st, const char* what);

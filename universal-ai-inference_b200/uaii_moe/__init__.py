@@ -27,6 +27,9 @@ BLOCK = {F32: (1, 4), F16: (1, 2), Q4_0: (32, 18), Q4_1: (32, 20), Q5_0: (32, 22
          Q8_0: (32, 34), Q2_K: (256, 84), Q3_K: (256, 110), Q4_K: (256, 144), Q5_K: (256, 176),
          Q6_K: (256, 210)}
 
+# formats of a KV cache next to F16: one byte per value, one f32 scale per row
+KV_I8, KV_E4M3 = 32, 33
+
 OK = 0
 INVALID_ARGUMENT, NOT_FOUND, NOT_IMPLEMENTED, INTERNAL = 1, 2, 7, 8
 STATUS_NAMES = {0: "Ok", 1: "InvalidArgument", 2: "NotFound", 3: "IoError", 4: "ConfigError",
@@ -60,6 +63,12 @@ class Layer(ctypes.Structure):
                 ("gate_shexp", c_void_p), ("gate_shexp_fmt", c_int32), ("up_shexp", c_void_p),
                 ("up_shexp_fmt", c_int32), ("down_shexp", c_void_p), ("down_shexp_fmt", c_int32),
                 ("gate_inp_shexp", c_void_p)]
+
+
+class KVCache(ctypes.Structure):
+    """One layer's KV cache (uaii_moe_kv_cache); make one with kv_cache()."""
+    _fields_ = [("fmt", c_int32), ("head_dim", c_int32), ("batch", c_int64), ("n_kv_heads", c_int64),
+                ("max_seq", c_int64), ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p)]
 
 
 def _load():
@@ -124,6 +133,13 @@ def _load():
         "uaii_moe_packed_nbytes": (c_uint64, [c_int, c_int64]),
         "uaii_moe_quantize_rows": (c_int, [c_int, c_void_p, c_int64, c_int64, c_void_p]),
         "uaii_moe_fill_normal": (c_int, [c_void_p, c_int64, c_uint64, c_uint64, c_float, c_float]),
+        "uaii_moe_kv_append": (c_int, [c_void_p, POINTER(KVCache), c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
+                                       c_int64, c_void_p, c_void_p]),
+        "uaii_moe_kv_read": (c_int, [c_void_p, POINTER(KVCache), c_int64, c_int64, c_void_p, c_void_p, c_int]),
+        "uaii_moe_prefix_attention": (c_int, [c_void_p, POINTER(KVCache), c_int64, POINTER(KVCache), c_void_p, c_void_p,
+                                              c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p]),
+        "uaii_moe_sample": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
         "uaii_moe_decoder_create": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                             POINTER(c_void_p)]),
         "uaii_moe_decoder_destroy": (None, [c_void_p]),
@@ -158,7 +174,8 @@ EXPORTED = ("uaii_moe_abi_version", "uaii_moe_last_error", "uaii_moe_backend_cre
             "uaii_moe_selftest_wait_timeout", "uaii_moe_profile_enable",
             "uaii_moe_profile_read",
             "uaii_moe_packed_nbytes", "uaii_moe_quantize_rows",
-            "uaii_moe_fill_normal", "uaii_moe_decoder_create", "uaii_moe_decoder_destroy",
+            "uaii_moe_fill_normal", "uaii_moe_kv_append", "uaii_moe_kv_read", "uaii_moe_prefix_attention",
+            "uaii_moe_sample", "uaii_moe_decoder_create", "uaii_moe_decoder_destroy",
             "uaii_moe_decoder_set_kv", "uaii_moe_decoder_fill_kv", "uaii_moe_decoder_step",
             "uaii_moe_decoder_generate", "uaii_moe_decoder_position", "uaii_moe_fill_normal_device",
             "uaii_moe_quantize_rows_device")
@@ -184,6 +201,52 @@ def ptr(a) -> int | None:
             raise ValueError("tensor must be contiguous")
         return a.data_ptr()
     raise TypeError(f"cannot take the address of {type(a)}")
+
+
+def _dtype_code(t) -> int:
+    """UAII_MOE_DTYPE_* of a torch tensor's element type (f32 or f16)."""
+    name = str(t.dtype)
+    if name == "torch.float32":
+        return DTYPE_F32
+    if name == "torch.float16":
+        return DTYPE_F16
+    raise TypeError(f"expected float32 or float16, got {name}")
+
+
+def _rows(t, *shape):
+    """Element strides (batch, token, head) of a [batch, token, head, head_dim] view with a dense last dimension."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"expected shape {shape}, got {tuple(t.shape)}")
+    sb, st, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError("the last dimension must be dense")
+    return sb, st, sh
+
+
+def _whole(t, what, *shape):
+    """Address of a dense int32 / f32 vector or matrix of a known shape."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
+    return ptr(t)
+
+
+def _typed(t, what, dtype, *shape):
+    if str(t.dtype) != dtype:
+        raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
+    return _whole(t, what, *shape)
+
+
+def kv_cache(fmt: int, k, v, k_scale=None, v_scale=None) -> KVCache:
+    """A KV cache over CUDA tensors k, v [batch, n_kv_heads, max_seq, head_dim] (float16 for F16, uint8 for KV_I8 and
+    KV_E4M3) and, for the 8-bit formats, float32 scales [batch, n_kv_heads, max_seq].  Keeps the tensors alive."""
+    want = "torch.float16" if fmt == F16 else "torch.uint8"
+    b, h, s, d = k.shape
+    c = KVCache(fmt, d, b, h, s, _typed(k, "k", want, b, h, s, d), _typed(v, "v", want, b, h, s, d))
+    if fmt != F16:
+        c.k_scale = _typed(k_scale, "k_scale", "torch.float32", b, h, s)
+        c.v_scale = _typed(v_scale, "v_scale", "torch.float32", b, h, s)
+    c._keep = (k, v, k_scale, v_scale)
+    return c
 
 
 def packed_nbytes(fmt: int, n: int) -> int:
@@ -333,6 +396,53 @@ class Backend:
     def ep_combine_f16(self, y_back, row_of, T: int, world: int, d_model: int, y):
         """As ep_combine with f16 returned rows (added in f32, rank order)."""
         _check(lib.uaii_moe_ep_combine_f16(self._h, ptr(y_back), ptr(row_of), T, world, d_model, ptr(y)))
+
+    # ---- serving operators (CUDA tensors; see include/uaii_moe.h)
+    def kv_append(self, cache: KVCache, k, v, pos, n_new=None):
+        """Write k, v [batch, tokens, n_kv_heads, head_dim] (f32 or f16, any strides with a dense last dimension, the
+        same for both) at positions pos[i] + t, for t < n_new[i] (int32) where given."""
+        b, t = k.shape[0], k.shape[1]
+        sb, st, sh = _rows(k, cache.batch, t, cache.n_kv_heads, cache.head_dim)
+        if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+            raise ValueError("k and v must have the same shape, strides and type")
+        _check(lib.uaii_moe_kv_append(self._h, byref(cache), k.data_ptr(), v.data_ptr(), _dtype_code(k), t, sb, st, sh,
+                                      _typed(pos, "pos", "torch.int32", b),
+                                      None if n_new is None else _typed(n_new, "n_new", "torch.int32", b)))
+
+    def kv_read(self, cache: KVCache, pos0: int, n: int, k_out, v_out):
+        """Positions [pos0, pos0 + n) into k_out, v_out [batch, n_kv_heads, n, head_dim] (f32 or f16)."""
+        shape = (cache.batch, cache.n_kv_heads, n, cache.head_dim)
+        if v_out.dtype != k_out.dtype:
+            raise ValueError("k_out and v_out must have the same type")
+        _check(lib.uaii_moe_kv_read(self._h, byref(cache), pos0, n, _whole(k_out, "k_out", *shape),
+                                    _whole(v_out, "v_out", *shape), _dtype_code(k_out)))
+
+    def prefix_attention(self, q, own: KVCache, own_len, out, prefix: KVCache | None = None, prefix_len: int = 0,
+                         scale: float = 0.0):
+        """out = attention of q [batch, tokens, n_heads, head_dim] over the shared prefix [0, prefix_len) and each
+        sequence's own cached positions, of which its new tokens are the last; out has q's shape and type."""
+        b, t, h, d = q.shape
+        sb, st, sh = _rows(q, own.batch, t, h, own.head_dim)
+        if out.dtype != q.dtype:
+            raise ValueError("out must have q's type")
+        _check(lib.uaii_moe_prefix_attention(self._h, None if prefix is None else byref(prefix), prefix_len, byref(own),
+                                             _typed(own_len, "own_len", "torch.int32", b), q.data_ptr(),
+                                             _dtype_code(q), h, t, sb, st, sh, scale, _whole(out, "out", b, t, h, d)))
+
+    def sample(self, logits, temperature, top_k, top_p, min_p, u, tokens, probs=None, kept=None):
+        """tokens[i] (int32) sampled from logits[i] (f32 or f16, dense rows) with per-row settings and the uniform
+        number u[i]; probs (f32) and kept (int32) receive the token's probability and the size of the kept set."""
+        b, v = logits.shape
+        if logits.stride(1) != 1 and v > 1:
+            raise ValueError("a row of logits must be dense")
+        f, i = "torch.float32", "torch.int32"
+        _check(lib.uaii_moe_sample(self._h, logits.data_ptr(), _dtype_code(logits), b, v,
+                                   logits.stride(0) if b > 1 else v,
+                                   _typed(temperature, "temperature", f, b), _typed(top_k, "top_k", i, b),
+                                   _typed(top_p, "top_p", f, b), _typed(min_p, "min_p", f, b), _typed(u, "u", f, b),
+                                   _typed(tokens, "tokens", i, b),
+                                   None if probs is None else _typed(probs, "probs", f, b),
+                                   None if kept is None else _typed(kept, "kept", i, b)))
 
     def ep_combine(self, y_back, row_of, T: int, world: int, d_model: int, y):
         _check(lib.uaii_moe_ep_combine(self._h, ptr(y_back), ptr(row_of), T, world, d_model, ptr(y)))
