@@ -183,6 +183,8 @@ Error MoeCudaBackend::sync_and_check() {
       return Error::make(ErrorCode::InvalidArgument, "kv_append: a position lies outside the cache");
     if (code == kErrKvLength)
       return Error::make(ErrorCode::InvalidArgument, "prefix_attention: a sequence length lies outside its cache");
+    if (code == kErrKvCopy)
+      return Error::make(ErrorCode::Internal, "prefix_attention: a copy of cached positions did not complete");
     return Error::make(ErrorCode::Internal,
                        "tensor-core expert kernel gave up waiting (code " + std::to_string(code) + ")");
   }

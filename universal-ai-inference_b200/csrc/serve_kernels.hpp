@@ -18,6 +18,7 @@ enum KvFormat { kKvF16 = 1, kKvI8 = 32, kKvE4M3 = 33 };
 // Codes in the backend's device error word for arguments that only the device can see.
 constexpr int kErrKvPosition = 32;  // kv_append: a position outside the cache
 constexpr int kErrKvLength = 33;    // attention: a length outside the cache
+constexpr int kErrKvCopy = 34;      // attention: a copy of cached positions did not complete in time
 
 // k, v [batch, n_kv_heads, max_seq, head_dim] (f16 or bytes), scales [batch, n_kv_heads, max_seq] or null.
 struct KvCache {
