@@ -89,8 +89,8 @@ struct Plan {
   int rt;                  // rows of an item
   int unit;                // keys of a unit
   int prefix_nrt, own_nrt; // items per kv head (0: none)
-  int64_t prefix_units;    // units of a prefix item
-  int64_t prefix_items;
+  int prefix_units;        // units of a prefix item
+  int prefix_items;
   int grid;                // CTAs (0: the kernel has no work)
   float* part;             // partial sums [slot][rt][hd]
   float* ml;               // (maximum, denominator) of each partial row
@@ -168,7 +168,7 @@ struct Rows {
   float m[MT][kPer], l[MT][kPer];
   float f[MT][kPer];         // score factor: scale * log2(e), and the power of two taken out of a folded row of q
   int lim[MT][kPer];         // positions the row sees
-  uint32_t vexp;             // exponent bits of the largest V scale so far (8-bit formats)
+  float vtop;                // a power of two above every V scale so far (8-bit formats)
 
   // Leading part and rest.  Where an f16 cache holds an infinity, the rest is 0 * inf.
   static __device__ __forceinline__ float join(float lead, float rest) {
@@ -189,7 +189,7 @@ struct Rows {
         l[t][r] = 0.f;
       }
     }
-    vexp = 27u << 23;  // 2^-100
+    vtop = 0x1p-100f;
   }
 
   // Keys [key, key + 8 NT) of the tile at k_base / v_base, which starts at position pos0 and of
@@ -238,9 +238,8 @@ struct Rows {
     }
     // columns 2 tq, 2 tq + 1 of each eight keys: K scales, and V scales as fractions of a power of two
     float kf[NT][2], vf[NT][2];
-    float vshrink = 1.f;
     if constexpr (F != kKvF16) {
-      uint32_t e = 0;
+      float most = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float2 x = *reinterpret_cast<const float2*>(ks + key + 8 * n + 2 * tq);
@@ -250,89 +249,99 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (masked && key + 8 * n + 2 * tq + i >= left) vf[n][i] = 0.f;  // nothing is stored there
-          const uint32_t b = __float_as_uint(vf[n][i]) & 0x7f800000u;
-          e = max(e, b >= 254u << 23 ? 0u : b);  // a NaN scale shows in its products, not here
+          most = fmaxf(most, vf[n][i]);                                    // (a NaN shows in its products, not here)
         }
       }
-      e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-      e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-      if (e > vexp) {  // (the same in every lane)
-        vshrink = __uint_as_float(max(0, (int)(0x3f800000u + vexp) - (int)e));
-        vexp = e;
-      }
-      const float inv = __uint_as_float(0x7f000000u - vexp);  // its reciprocal
+      if (__any_sync(0xffffffffu, most >= vtop)) raise_v(most);
+      const float inv = __uint_as_float(0x7f800000u - __float_as_uint(vtop));  // 2 / vtop
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         vf[n][0] *= inv;
         vf[n][1] *= inv;
       }
     }
-    bool grew = vshrink != 1.f;
-    float mn[MT][kPer];
+    // exponents against the reference; a lane checks its own, the row's maximum is only made when one is too large
+    bool grew = false;
+    float x[MT][kPer][NT][2];
+    auto exponents = [&]() {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+          const float off = kLift - (m[t][r] == -INFINITY ? 0.f : m[t][r]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              x[t][r][n][i] = fmaf(s[t][n][2 * r + i], F == kKvF16 ? f[t][r] : kf[n][i] * f[t][r], off);
+        }
+    };
+    auto seen = [&](int t, int r, int n, int i) { return !masked || pos0 + key + 8 * n + 2 * tq + i < lim[t][r]; };
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if constexpr (FOLD) s[t][n][i] = join(s[t][n][i], s[t][n][2 + i]);
+    exponents();
+    float mx[MT][kPer];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
-        float mx = -INFINITY;
+        mx[t][r] = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& x = s[t][n][2 * r + i];
-            if constexpr (FOLD) x = join(x, s[t][n][2 + i]);
-            if constexpr (F != kKvF16) x *= kf[n][i];
-            if (!masked || pos0 + key + 8 * n + 2 * tq + i < lim[t][r]) mx = fmaxf(mx, x * f[t][r]);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mn[t][r] = mx;
-        grew |= mx > m[t][r] + kSlack;
+          for (int i = 0; i < 2; ++i)
+            if (seen(t, r, n, i)) mx[t][r] = fmaxf(mx[t][r], x[t][r][n][i]);
+        grew |= mx[t][r] > (m[t][r] == -INFINITY ? -INFINITY : kLift + kSlack);
       }
     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < kPer; ++r) {
+          float y = mx[t][r];
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+          y += (m[t][r] == -INFINITY ? 0.f : m[t][r]) - kLift;
           // whole numbers, so that neither the factors nor the differences to them round
-          const float to = fmaxf(m[t][r], ceilf(mn[t][r]));
-          const float c = to > m[t][r] ? ex2(m[t][r] - to) : 1.f, co = c * vshrink;
+          const float to = fmaxf(m[t][r], ceilf(y));
+          const float c = to > m[t][r] ? ex2(m[t][r] - to) : 1.f;
           m[t][r] = to;
           l[t][r] *= c;
 #pragma unroll
           for (int n = 0; n < HD / 8; ++n) {
-            o[t][n][2 * r] *= co;
-            o[t][n][2 * r + 1] *= co;
+            o[t][n][2 * r] *= c;
+            o[t][n][2 * r + 1] *= c;
             if constexpr (FOLD) {
-              o[t][n][2] *= co;
-              o[t][n][3] *= co;
+              o[t][n][2] *= c;
+              o[t][n][3] *= c;
             }
           }
         }
+      exponents();
     }
     float low = 0.f;  // the smallest exponent
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int r = 0; r < kPer; ++r) {
-        const float off = kLift - (m[t][r] == -INFINITY ? 0.f : m[t][r]);
+      for (int r = 0; r < kPer; ++r)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& x = s[t][n][2 * r + i];
-            const bool seen = !masked || pos0 + key + 8 * n + 2 * tq + i < lim[t][r];
-            x = fmaf(x, f[t][r], off);
-            if (seen) {
-              l[t][r] += ex2(x);
-              if constexpr (kFar) low = fminf(low, x);
-            }
-          }
-      }
+          for (int i = 0; i < 2; ++i)
+            if (kFar && seen(t, r, n, i)) low = fminf(low, x[t][r][n][i]);
     const bool far = kFar && __any_sync(0xffffffffu, low < kNear);
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
       uint32_t p[MT][4];
-      weigh<masked>(s, vf, n, key, pos0, far ? kNear : -INFINITY, INFINITY, 0.f, p);
+      weigh(x, vf, n, seen, [&](int t, int r, float y, float e) {
+        l[t][r] += e;
+        return far && y < kNear ? 0.f : e;
+      }, p);
       products(v_base, key + 8 * n, [&](int c, int t, uint32_t b0, uint32_t b1) { mma16816(o[t][c], p[t], b0, b1); });
     }
     if constexpr (kFar) {
@@ -343,7 +352,7 @@ struct Rows {
 #pragma unroll
           for (int n = 0; n < NT; n += 2) {
             uint32_t p[MT][4];
-            weigh<masked>(s, vf, n, key, pos0, top - 20.f, top, up, p);
+            weigh(x, vf, n, seen, [&](int, int, float y, float) { return y >= top - 20.f && y < top ? ex2(y + up) : 0.f; }, p);
             if (__any_sync(0xffffffffu, (p[0][0] | p[0][2]) != 0))
               products(v_base, key + 8 * n, [&](int c, int t, uint32_t b0, uint32_t b1) {
                 float x[4] = {};
@@ -357,11 +366,28 @@ struct Rows {
     }
   }
 
-  // Weights of 16 keys as an operand: those with an exponent in [from, to), raised by `up`.
-  template <bool masked, int NT>
-  __device__ __forceinline__ void weigh(const float (&s)[MT][NT][4], const float (&vf)[NT][2], int n, int key, int pos0,
-                                        float from, float to, float up, uint32_t (&p)[MT][4]) {
-    const int tq = threadIdx.x & 3;
+  // A V scale of vtop or more: the next power of two above the largest, and the sums so far brought to it.
+  static __device__ __noinline__ float next_vtop(float vtop, float most) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const uint32_t e = min((__float_as_uint(most) & 0x7f800000u) + (1u << 23), 252u << 23);
+    return fmaxf(vtop, __uint_as_float(e));
+  }
+  __device__ __forceinline__ void raise_v(float most) {
+    const float to = next_vtop(vtop, most), c = vtop / to;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[t][n][i] *= c;
+    vtop = to;
+  }
+
+  // Weights of 16 keys as an operand; take(t, r, exponent, 2^exponent) gives a seen position's weight before V's scale.
+  template <int NT, typename S, typename W>
+  __device__ __forceinline__ void weigh(const float (&x)[MT][kPer][NT][2], const float (&vf)[NT][2], int n, S&& seen,
+                                        W&& take, uint32_t (&p)[MT][4]) {
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -371,17 +397,18 @@ struct Rows {
           float w[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float x = s[t][n + h][2 * r + i];
-            const bool seen = !masked || pos0 + key + 8 * (n + h) + 2 * tq + i < lim[t][r];
-            w[i] = ex2(x + up);
-            if constexpr (F != kKvF16) w[i] *= vf[n + h][i];
-            if (!seen || x < from || x >= to) w[i] = 0.f;  // (a NaN stays)
+            const float y = x[t][r][n + h][i];
+            w[i] = 0.f;
+            if (seen(t, r, n + h, i)) {
+              w[i] = take(t, r, y, ex2(y));
+              if constexpr (F != kKvF16) w[i] *= vf[n + h][i];
+            }
           }
           const __half2 lead = __floats2half2_rn(w[0], w[1]);
           p[t][2 * h + r] = half2_bits(lead);
           if constexpr (FOLD) {
-            const float2 x = __half22float2(lead);
-            p[t][2 * h + 1] = half2_bits(__floats2half2_rn(w[0] - x.x, w[1] - x.y));
+            const float2 z = __half22float2(lead);
+            p[t][2 * h + 1] = half2_bits(__floats2half2_rn(w[0] - z.x, w[1] - z.y));
           }
         }
   }
@@ -418,7 +445,7 @@ struct Rows {
 
   // The row sums with V's power of two put back; l summed over the lanes of a row.
   __device__ __forceinline__ void finish() {
-    const float up = F == kKvF16 ? 1.f : __uint_as_float(vexp);
+    const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
@@ -464,16 +491,27 @@ struct Piece {
   int fewest;        // positions that every row sees
 };
 
+// The first unit of CTA c: the first total % grid CTAs take one unit more than the others.
+__device__ __forceinline__ int share_start(int c, int total, int grid) {
+  const int each = total / grid;
+  return c * each + min(c, total - each * grid);
+}
+// The CTA that holds unit u < total.
+__device__ __forceinline__ int share_of(int u, int total, int grid) {
+  const int each = total / grid, more = total - each * grid, split = more * (each + 1);
+  return u < split ? u / (each + 1) : more + (u - split) / each;
+}
+
 struct Walk {
-  int64_t u, end;
+  int u, end;
   int b = 0;
   __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
-    const int64_t prefix = p.prefix_items * p.prefix_units, per = a.own.heads * p.own_nrt;
-    const int64_t total = prefix + (per ? cum[a.B] * per : 0);
-    u = total * blockIdx.x / gridDim.x;
-    end = total * (blockIdx.x + 1) / gridDim.x;
+    const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
+    const int total = prefix + (per ? cum[a.B] * per : 0);
+    u = share_start(blockIdx.x, total, gridDim.x);
+    end = share_start(blockIdx.x + 1, total, gridDim.x);
     if (end > prefix) {  // the last sequence whose units start at or before the first own unit
-      const int64_t first = max(u - prefix, int64_t(0));
+      const int first = max(u - prefix, 0);
       int lo = 0, hi = (int)a.B - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -485,16 +523,15 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(Piece& x, const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
     if (u >= end) return false;
-    const int64_t prefix = p.prefix_items * p.prefix_units;
-    int64_t in, units;
+    const int prefix = p.prefix_items * p.prefix_units;
+    int in, units;
     if (u >= prefix) {
-      const int64_t per = a.own.heads * p.own_nrt, v = u - prefix;
+      const int per = (int)a.own.heads * p.own_nrt, v = u - prefix;
       while (cum[b + 1] * per <= v) ++b;
       units = cum[b + 1] - cum[b];
-      const int64_t rest = v - cum[b] * per;
-      const int j = (int)(rest / units);
+      const int rest = v - cum[b] * per, j = rest / units;
       in = rest - j * units;
-      x.slot = p.prefix_items + b * per + j;
+      x.slot = p.prefix_items + (int64_t)b * per + j;
       x.own = 1;
       x.kvh = j / p.own_nrt;
       x.rt = j % p.own_nrt;
@@ -507,7 +544,7 @@ struct Walk {
     } else {
       units = p.prefix_units;
       x.slot = u / units;
-      in = u - x.slot * units;
+      in = u - (int)x.slot * units;
       x.own = 0;
       x.kvh = (int)x.slot / p.prefix_nrt;
       x.rt = (int)x.slot % p.prefix_nrt;
@@ -515,9 +552,9 @@ struct Walk {
       x.z = x.kvh;
       x.limit = x.fewest = (int)a.prefix_len;
     }
-    const int64_t n = min(units - in, end - u);
-    x.t0 = (int)in;
-    x.t1 = (int)(in + n);
+    const int n = min(units - in, end - u);
+    x.t0 = in;
+    x.t1 = in + n;
     x.slot += blockIdx.x;
     u += n;
     return true;
@@ -797,6 +834,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     umma::fence_proxy_async_smem();  // the stages take copies again
     __syncthreads();
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&sh.abort) grace();
 }
 
@@ -966,6 +1004,7 @@ __global__ void __launch_bounds__(32 * (kWarps + 1), kWideCtas)
   __syncthreads();
   if (t >= 32 * kWarps) produce<F, HD>(a, p, maps, cum, smem, ctl);
   else consume<F, HD, kFold, Q>(a, p, cum, smem, ctl);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&ctl.abort) grace();
 }
 
@@ -1006,30 +1045,28 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
   if (row >= a.B * a.T * a.H) return;
   const int64_t h = row % a.H, bt = row / a.H, b = bt / a.T, t = bt % a.T;
   const int64_t kvh = h / po.G, g = h % po.G;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the pieces are there from here on
   float mx = -INFINITY, l = 0.f, o[N] = {};
 #pragma unroll 1
   for (int own = px.prefix_items ? 0 : 1; own < 2; ++own) {
     const Plan& p = own ? po : px;
-    const int64_t rho = own ? t * p.G + g : (b * a.T + t) * p.G + g;
-    const int64_t j = rho / p.rt, in = rho % p.rt;
-    const int64_t per = a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
-    const int64_t total = prefix + (per ? cum[a.B] * per : 0);
-    int64_t item, u0, units;
+    const int rho = (int)(own ? t * p.G + g : bt * p.G + g), j = rho / p.rt, in = rho - j * p.rt;
+    const int per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
+    const int total = prefix + (per ? cum[a.B] * per : 0);
+    int64_t item;
+    int u0, units;
     if (own) {
       units = cum[b + 1] - cum[b];
       item = p.prefix_items + b * per + kvh * p.own_nrt + j;
-      u0 = prefix + cum[b] * per + (kvh * p.own_nrt + j) * units;
+      u0 = prefix + cum[b] * per + ((int)kvh * p.own_nrt + j) * units;
     } else {
       units = p.prefix_units;
       item = kvh * p.prefix_nrt + j;
-      u0 = item * units;
+      u0 = (int)item * units;
     }
     if (units == 0) continue;
-    // CTA c holds units [total c / grid, total (c + 1) / grid)
-    int64_t c = u0 * p.grid / total;
-    while (total * (c + 1) / p.grid <= u0) ++c;
-    for (; c < p.grid && total * c / p.grid < u0 + units; ++c) {
-      if (total * c / p.grid == total * (c + 1) / p.grid) continue;  // an idle CTA
+    const int first = share_of(u0, total, p.grid), last = share_of(u0 + units - 1, total, p.grid);
+    for (int c = first; c <= last; ++c) {
       const int64_t r = (item + c) * p.rt + in;
       const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * r);
       const float* src = p.part + r * HD + N * lane;
@@ -1086,6 +1123,7 @@ struct Layout {
   Plan narrow, wide;
   bool prefix_wide = false, own_wide = false;
   size_t bytes = 0;
+  int64_t most = 0;  // units of either kernel, at most
   const Plan& of_prefix() const { return prefix_wide ? wide : narrow; }
   const Plan& of_own() const { return own_wide ? wide : narrow; }
 };
@@ -1107,10 +1145,11 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     p.unit = w ? kTile : kWarps * narrow_keys(a);
     p.own_nrt = own ? (own_rows + p.rt - 1) / p.rt : 0;
     p.prefix_nrt = prefix ? (prefix_rows + p.rt - 1) / p.rt : 0;
-    p.prefix_units = prefix ? (a.prefix_len + p.unit - 1) / p.unit : 0;
-    p.prefix_items = a.own.heads * p.prefix_nrt;
+    p.prefix_units = prefix ? (int)((a.prefix_len + p.unit - 1) / p.unit) : 0;
+    p.prefix_items = (int)a.own.heads * p.prefix_nrt;
     const int64_t own_items = a.B * a.own.heads * p.own_nrt;
-    const int64_t most = p.prefix_items * p.prefix_units + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
+    const int64_t most = (int64_t)p.prefix_items * p.prefix_units + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
+    l.most = most > l.most ? most : l.most;
     const int full = kSms * (w ? kWideCtas : kNarrowCtas);
     p.grid = (int)(most < full ? most : full);
     if (p.grid == 0) continue;
@@ -1157,10 +1196,18 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
                                        : run(narrow_attn_kernel<F, HD, true, __half>, smem, threads, a, p, maps, given, cum, st);
     if (e != cudaSuccess) return e;
   }
-  const unsigned blocks = (unsigned)((a.B * a.T * a.H + 3) / 4);
-  if (a.half) join_kernel<HD, __half><<<blocks, 128, 0, st>>>(a, l.of_prefix(), l.of_own(), cum);
-  else join_kernel<HD, float><<<blocks, 128, 0, st>>>(a, l.of_prefix(), l.of_own(), cum);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((a.B * a.T * a.H + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const int32_t* sums = cum;
+  return a.half ? cudaLaunchKernelEx(&cfg, join_kernel<HD, __half>, a, l.of_prefix(), l.of_own(), sums)
+                : cudaLaunchKernelEx(&cfg, join_kernel<HD, float>, a, l.of_prefix(), l.of_own(), sums);
 }
 
 template <int F>
@@ -1174,6 +1221,7 @@ size_t prefix_attn_ws(const PrefixAttnArgs& a) { return lay_out(a, nullptr).byte
 
 cudaError_t launch_prefix_attn(const PrefixAttnArgs& a, void* ws, int* launches, cudaStream_t st) {
   const Layout l = lay_out(a, static_cast<char*>(ws));
+  if (l.most >= (int64_t(1) << 30)) return cudaErrorInvalidValue;  // (a cache of 2^36 positions)
   int32_t* cum = static_cast<int32_t*>(ws);
   const int32_t* given = nullptr;
   *launches = 1 + (l.wide.grid > 0) + (l.narrow.grid > 0);
