@@ -108,7 +108,7 @@ __device__ __forceinline__ int own_length(const PrefixAttnArgs& a, int64_t b, bo
 // ---------------------------------------------------------------- operands
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(  // not volatile: independent products may be interleaved
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -503,9 +503,9 @@ __device__ __forceinline__ int share_of(int u, int total, int grid) {
 }
 
 struct Walk {
-  int u, end;
-  int b = 0;
-  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
+  int u, end, b;
+  Walk() = default;
+  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) : b(0) {
     const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
     const int total = prefix + (per ? cum[a.B] * per : 0);
     u = share_start(blockIdx.x, total, gridDim.x);
@@ -654,28 +654,21 @@ __device__ __forceinline__ void zero_v(uint8_t* v, int from, int to, int thread,
 
 // ---------------------------------------------------------------- narrow
 
+// What a warp copies next: position `key` of piece x, up to `end`.  Kept in shared memory: it is used once a tile.
+struct Ahead {
+  Walk w;
+  Piece x;
+  int key, end;
+};
+
 template <int F, int HD>
 struct NarrowShared {
   uint64_t full[kWarps][Narrow<F, HD>::kStages];
+  Ahead ahead[kWarps];
   int abort;
   int where[kWarps];
   float ml[kWarps][16][2];
   int32_t cum[kMaxScan + 1];
-};
-
-// The warp's tiles of kKeys positions: tiles warp, warp + 4, ... of every unit run of every piece.
-struct Steps {
-  Walk w;
-  Piece x;
-  int key, end;      // next position and the end of the warp's share of the piece
-  __device__ __forceinline__ bool next(int keys, int warp, const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
-    while (key >= end) {
-      if (!w.next(x, p, a, cum)) return false;
-      key = x.t0 * p.unit + warp * keys;
-      end = min(x.t1 * p.unit, x.limit);
-    }
-    return true;
-  }
 };
 
 template <int F, int HD, bool FOLD, typename Q>
@@ -699,19 +692,36 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
   __syncthreads();
   uint8_t* tiles = smem + warp * N::kStages * N::kStage;
   float* scales = reinterpret_cast<float*>(smem + kWarps * N::kStages * N::kStage + warp * N::kScales);
-  Steps ahead{Walk(p, a, cum), {}, 0, 0};
+  Ahead& ahead = sh.ahead[warp];
+  if (lane == 0) {
+    ahead.w = Walk(p, a, cum);
+    ahead.key = ahead.end = 0;
+  }
+  __syncwarp();
   int issued = 0, done = 0;     // tiles copied and used by this warp: stage = count mod kStages
   // Copy the warp's next tile.  The stage is the one whose tile was used last, so at least one stage is free whenever
   // no tile is being worked on: the join at the end of a piece uses it.
   auto copy = [&]() {
-    if (!ahead.next(KEYS, warp, p, a, cum)) return;
+    if (ahead.key >= ahead.end) {
+      __syncwarp();
+      if (lane == 0)  // tiles warp, warp + 4, ... of every piece
+        while (ahead.key >= ahead.end && ahead.w.next(ahead.x, p, a, cum)) {
+          ahead.key = ahead.x.t0 * N::kUnit + warp * KEYS;
+          ahead.end = min(ahead.x.t1 * N::kUnit, ahead.x.limit);
+        }
+      __syncwarp();
+      if (ahead.key >= ahead.end) return;
+    }
     const int s = issued % N::kStages, z = ahead.x.z, pos = ahead.key;
-    const KvCache& c = ahead.x.own ? a.own : a.prefix;
+    const bool own = ahead.x.own != 0;
+    const KvCache& c = own ? a.own : a.prefix;
+    __syncwarp();
     uint64_t* bar = &sh.full[warp][s];
     const uint32_t dst = umma::smem_u32(tiles + s * N::kStage);
     if (lane == 0) {
       umma::mbar_arrive_expect_tx(bar, 2 * Tl::kBytes);
-      const CUtensorMap *mk = ahead.x.own ? &maps.ok : &maps.pk, *mv = ahead.x.own ? &maps.ov : &maps.pv;
+      ahead.key = pos + kWarps * KEYS;
+      const CUtensorMap *mk = own ? &maps.ok : &maps.pk, *mv = own ? &maps.ov : &maps.pv;
 #pragma unroll
       for (int b = 0; b < Tl::kBoxes; ++b) {
         tma_load_3d(dst + b * Tl::kBoxBytes, mk, bar, b * (Tl::kPart / Tl::kEsz), pos, z);
@@ -727,8 +737,8 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
       asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * KEYS), "l"(c.v_scale + at), "r"(bytes) : "memory");
       asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
     }
-    ahead.key += kWarps * KEYS;
     ++issued;
+    __syncwarp();
   };
   for (int i = 0; i < N::kStages - 1; ++i) copy();
 
