@@ -1,0 +1,264 @@
+// attn_common.cuh -- what the attention kernels (attn_narrow.cuh, attn_wide.cuh) share: stored tiles and their bytes
+// as f16 operands, items and pieces, and the CTAs' shares of the work.  The mathematics is in prefix_attn.cu.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "serve_kernels.hpp"
+#include "umma.cuh"
+
+namespace uaii_b200 {
+namespace attn {
+
+constexpr int kSms = 148;
+constexpr int kTile = 64;        // wide: keys of a tile
+constexpr int kWarps = 4;        // narrow: warps of a CTA
+constexpr int kNarrowCtas = 3;   // narrow: CTAs per SM (wide: one)
+constexpr int kMaxScan = 1024;   // sequences whose tile counts a CTA sums itself
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities are 2^(s - m + 8) (in sums and denominators alike), and m follows the running maximum only when that
+// rises by more than 6: the sums are then seldom rescaled, weights stay below 2^14 (2^15 with V's scale, a fraction
+// below 2), and f16 keeps 11 bits of each down to 2^-22 of the largest.
+constexpr float kLift = 8.0f, kSlack = 6.0f;
+
+// A stored row, and a copied tile of KEYS rows of K or V: boxes of at most 128 bytes a row (the swizzle span).
+template <int F, int HD, int KEYS>
+struct Tile {
+  static constexpr int kEsz = F == kKvF16 ? 2 : 1;
+  static constexpr int kRow = HD * kEsz;
+  static constexpr int kPart = kRow < 128 ? kRow : 128;
+  static constexpr int kBoxes = kRow / kPart;
+  static constexpr int kBoxBytes = kPart * KEYS;
+  static constexpr int kBytes = kBoxes * kBoxBytes;
+  static constexpr int kScaleBytes = F == kKvF16 ? 0 : 2 * KEYS * 4;
+};
+
+struct Maps {
+  CUtensorMap pk, pv, ok, ov;
+};
+
+// The items of one kernel: prefix items first, then own ones (either may be missing).
+struct Plan {
+  int G;                   // query heads per kv head
+  int prefix_rows;         // B * T * G
+  int own_rows;            // T * G
+  int rt;                  // rows of an item
+  int slot_rows, subs;     // rows of a slot; parts of an item's rows in it (2: each half of the keys has its own)
+  bool split_keys;         // wide: the two row tiles hold the same rows
+  int unit;                // keys of a unit
+  int prefix_nrt, own_nrt; // items per kv head (0: none)
+  int prefix_units;        // units of a prefix item
+  int prefix_items;
+  int grid;                // CTAs (0: the kernel has no work)
+  float* part;             // partial sums [slot][slot_rows][hd]
+  float* ml;               // (maximum, denominator) of each partial row
+};
+
+__device__ __forceinline__ int own_length(const PrefixAttnArgs& a, int64_t b, bool report) {
+  int64_t n = a.own_len[b];
+  if (n < 0 || n > a.own.max_seq) {
+    if (report) atomicExch(a.err, kErrKvLength);
+    n = n < 0 ? 0 : a.own.max_seq;
+  }
+  return (int)n;
+}
+
+// ---------------------------------------------------------------- operands
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm(  // not volatile: independent products may be interleaved
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+// Two pairs of stored bytes -> two f16 pairs.  i8: a byte u behind 0x64 is the half 1024 + u, less 1152 = u - 128.
+// SEL: bytes (0, 1) and (2, 3) for K, whose pairs run along a row; (0, 2) and (1, 3) for V, whose transposed words
+// hold two dimensions of two positions.
+template <int F, bool V>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t& a, uint32_t& b) {
+  if constexpr (F == kKvI8) {
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+    const uint32_t x = __byte_perm(w, 0x64646464u, V ? 0x4240 : 0x4140);
+    const uint32_t y = __byte_perm(w, 0x64646464u, V ? 0x4341 : 0x4342);
+    a = half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&x), bias));
+    b = half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&y), bias));
+  } else {
+    const uint32_t p = V ? __byte_perm(w, 0, 0x3120) : w;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(a), "=r"(b) : "r"(p));
+  }
+}
+
+// Address of 16-byte piece c of row r of a K or V tile (boxes of kPart bytes a row, swizzled as the copy writes them).
+template <int F, int HD, int KEYS>
+__device__ __forceinline__ uint32_t piece(uint32_t base, int r, int c) {
+  using Gm = Tile<F, HD, KEYS>;
+  if constexpr (Gm::kPart == 128) return base + (c >> 3) * Gm::kBoxBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+  else return base + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+
+// ---------------------------------------------------------------- the walk over a CTA's pieces
+
+struct Piece {
+  int64_t slot;      // item + CTA
+  int own;
+  int z, kvh, rt;    // plane of the cache; kv head, row tile
+  int seq;           // own items: the sequence
+  int t0, t1;        // units of this CTA
+  int limit;         // positions that some row of the item sees
+  int fewest;        // positions that every row sees
+};
+
+// The first unit of CTA c: the first total % grid CTAs take one unit more than the others.
+__device__ __forceinline__ int share_start(int c, int total, int grid) {
+  const int each = total / grid;
+  return c * each + min(c, total - each * grid);
+}
+// The CTA that holds unit u < total.
+__device__ __forceinline__ int share_of(int u, int total, int grid) {
+  const int each = total / grid, more = total - each * grid, split = more * (each + 1);
+  return u < split ? u / (each + 1) : more + (u - split) / each;
+}
+
+struct Walk {
+  int u, end, b;
+  Walk() = default;
+  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) : b(0) {
+    const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
+    const int total = prefix + (per ? cum[a.B] * per : 0);
+    u = share_start(blockIdx.x, total, gridDim.x);
+    end = share_start(blockIdx.x + 1, total, gridDim.x);
+    if (end > prefix) {  // the last sequence whose units start at or before the first own unit
+      const int first = max(u - prefix, 0);
+      int lo = 0, hi = (int)a.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (cum[mid] * per <= first) lo = mid;
+        else hi = mid - 1;
+      }
+      b = lo;
+    }
+  }
+  __device__ __forceinline__ bool next(Piece& x, const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
+    if (u >= end) return false;
+    const int prefix = p.prefix_items * p.prefix_units;
+    int in, units;
+    if (u >= prefix) {
+      const int per = (int)a.own.heads * p.own_nrt, v = u - prefix;
+      while (cum[b + 1] * per <= v) ++b;
+      units = cum[b + 1] - cum[b];
+      const int rest = v - cum[b] * per, j = rest / units;
+      in = rest - j * units;
+      x.slot = p.prefix_items + (int64_t)b * per + j;
+      x.own = 1;
+      x.kvh = j / p.own_nrt;
+      x.rt = j % p.own_nrt;
+      x.seq = b;
+      x.z = b * (int)a.own.heads + x.kvh;
+      const int first = x.rt * p.rt / p.G, last = (min((x.rt + 1) * p.rt, p.own_rows) - 1) / p.G;  // tokens
+      const int seen = own_length(a, b, false) - (int)a.T + 1;
+      x.limit = seen + last;
+      x.fewest = seen + first;
+    } else {
+      units = p.prefix_units;
+      x.slot = u / units;
+      in = u - (int)x.slot * units;
+      x.own = 0;
+      x.kvh = (int)x.slot / p.prefix_nrt;
+      x.rt = (int)x.slot % p.prefix_nrt;
+      x.seq = 0;
+      x.z = x.kvh;
+      x.limit = x.fewest = (int)a.prefix_len;
+    }
+    const int n = min(units - in, end - u);
+    x.t0 = in;
+    x.t1 = in + n;
+    x.slot += blockIdx.x;
+    u += n;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(umma::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// After a copy that was late: time for what is in flight to land before the shared memory is reused.
+__device__ __noinline__ void grace() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 20000000LL) {}
+}
+
+// The sequences' unit counts, summed: cum[b] units of one row tile and kv head lie before sequence b.  Every CTA sums
+// up to kMaxScan sequences itself; CTA 0 leaves the sums for the joining kernel.
+__device__ const int32_t* unit_sums(const PrefixAttnArgs& a, const Plan& p, const int32_t* given, int32_t* shared,
+                                    int32_t* out) {
+  if (given || p.own_nrt == 0) return given;
+  const int t = threadIdx.x, lane = t & 31;
+  if (t < 32) {
+    int sum = 0;
+    for (int b0 = 0; b0 < (int)a.B; b0 += 32) {
+      const int b = b0 + lane;
+      int n = b < a.B ? (own_length(a, b, blockIdx.x == 0) + p.unit - 1) / p.unit : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += y;
+      }
+      if (b < a.B) {
+        shared[b + 1] = sum + n;
+        if (blockIdx.x == 0) out[b + 1] = sum + n;
+      }
+      sum += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) {
+      shared[0] = 0;
+      if (blockIdx.x == 0) out[0] = 0;
+    }
+  }
+  return shared;
+}
+
+// q row of logical row `row` of an item (null past the end) and the positions it sees.
+template <typename Q>
+__device__ __forceinline__ const Q* q_row(const PrefixAttnArgs& a, const Plan& p, const Piece& x, int row, int& lim) {
+  const int rho = x.rt * p.rt + row;
+  if (rho >= (x.own ? p.own_rows : p.prefix_rows)) {
+    lim = 0;
+    return nullptr;
+  }
+  const int64_t b = x.own ? x.seq : rho / p.own_rows;
+  const int in = x.own ? rho : rho % p.own_rows;
+  const int t = in / p.G, g = in % p.G;
+  lim = x.own ? x.fewest + t - x.rt * p.rt / p.G : x.limit;
+  return static_cast<const Q*>(a.q) + b * a.qs.batch + t * a.qs.token + ((int64_t)x.kvh * p.G + g) * a.qs.head;
+}
+
+// A power of two that brings the largest of a folded row into [1, 2): its exponent leaves through the score factor, so
+// that neither part of the split overflows or loses bits.  bits: max |q|; returns 2^-e.
+__device__ __forceinline__ float row_shrink(uint32_t bits) {
+  const uint32_t e = min(max(bits & 0x7f800000u, 64u << 23), 190u << 23);
+  return __uint_as_float(0x7f000000u - e);
+}
+
+}  // namespace attn
+}  // namespace uaii_b200

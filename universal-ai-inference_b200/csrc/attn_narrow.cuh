@@ -1,0 +1,532 @@
+// attn_narrow.cuh -- attention items of at most 8 or 16 rows on warp-level MMAs (see prefix_attn.cu).
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace uaii_b200 {
+namespace attn {
+
+// Narrow: each warp copies for itself, kKeys positions at a time, the next ones while it works.  Three CTAs of four
+// warps hold 190 KB of an SM, about half of it in flight.
+template <int F, int HD>
+struct Narrow {
+  static constexpr int kKeys = F == kKvF16 && HD == 128 ? 16 : 32;
+  using Tl = Tile<F, HD, kKeys>;
+  static constexpr int kStage = 2 * Tl::kBytes;             // 4, 8 or (f16 of 16 keys) 8 KB
+  static constexpr int kStages = 16 * 1024 / kStage;
+  static constexpr int kScales = kStages * Tl::kScaleBytes; // of one warp, after all the tiles
+  static constexpr int kSmem = kWarps * (kStages * kStage + kScales) + 1024;
+  static constexpr int kUnit = kWarps * kKeys;
+};
+
+// ---------------------------------------------------------------- one warp's running softmax
+
+template <int F, int HD, bool FOLD, int KEYS>
+struct Rows {
+  static constexpr int kPer = FOLD ? 1 : 2;  // logical rows of a lane in one MMA tile
+  static constexpr int kPieces = HD * Tile<F, HD, KEYS>::kEsz / 16;  // 16-byte pieces of a row
+  // The two parts of a weight resolve 2^-24, f16's smallest step.  Smaller weights are added in passes of their own,
+  // 20 binary orders at a time, raised to [2^-6, 2^14): only very uneven scores (22 e-foldings) need them.
+  static constexpr bool kFar = FOLD;
+  static constexpr float kNear = -24.f;
+  float o[HD / 8][4];
+  float m[kPer], l[kPer];
+  float f[kPer];         // score factor: scale * log2(e), and the power of two taken out of a folded row of q
+  int lim[kPer];         // positions the row sees
+  float vtop;                // a power of two above every V scale so far (8-bit formats)
+
+  // Leading part and rest.  Where an f16 cache holds an infinity, the rest is 0 * inf.
+  static __device__ __forceinline__ float join(float lead, float rest) {
+    if constexpr (F == kKvF16) return fabsf(lead) == INFINITY ? lead : lead + rest;
+    return lead + rest;
+  }
+
+  __device__ __forceinline__ void clear() {
+    {
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+      }
+    }
+    vtop = 0x1p-100f;
+  }
+
+  // Keys [key, key + 8 NT) of the tile at k_base / v_base, which starts at position pos0 and of
+  // which some row sees the first `left`; masked says that some row may not see all of them.  a(ks, frag) gives
+  // the query operands.
+  template <int NT, bool masked, typename A>
+  __device__ __forceinline__ void step(uint32_t k_base, uint32_t v_base, const float* ks, const float* vs, int key,
+                                       int left, int pos0, A&& a) {
+    const int lane = threadIdx.x & 31, tq = lane & 3, mi = lane >> 3, r8 = lane & 7;
+    float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+    // scores: four 16-byte pieces of eight keys at a time
+#pragma unroll
+    for (int c = 0; c < kPieces; c += 4) {
+      constexpr int kSteps = F == kKvF16 ? 2 : 4;
+      uint32_t q[kSteps][4];
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
+        a((F == kKvF16 ? c / 2 : c) + j, q[j]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        uint32_t w[4];
+        ldsm4(w, piece<F, HD, KEYS>(k_base, key + 8 * n + r8, c + mi));
+        if constexpr (F == kKvF16) {
+          {
+            mma16816(s[n], q[0], w[0], w[1]);
+            mma16816(s[n], q[1], w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t b0, b1;
+            unpack<F, false>(w[j], b0, b1);
+        mma16816(s[n], q[j], b0, b1);
+          }
+        }
+      }
+    }
+    // columns 2 tq, 2 tq + 1 of each eight keys: K scales, and V scales as fractions of a power of two
+    float kf[NT][2], vf[NT][2];
+    if constexpr (F != kKvF16) {
+      float most = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float2 x = *reinterpret_cast<const float2*>(ks + key + 8 * n + 2 * tq);
+        const float2 y = *reinterpret_cast<const float2*>(vs + key + 8 * n + 2 * tq);
+        kf[n][0] = x.x; kf[n][1] = x.y;
+        vf[n][0] = y.x; vf[n][1] = y.y;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (masked && key + 8 * n + 2 * tq + i >= left) vf[n][i] = 0.f;  // nothing is stored there
+          most = fmaxf(most, vf[n][i]);                                    // (a NaN shows in its products, not here)
+        }
+      }
+      if (__any_sync(0xffffffffu, most >= vtop)) raise_v(most);
+      const float inv = __uint_as_float(0x7f800000u - __float_as_uint(vtop));  // 2 / vtop
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        vf[n][0] *= inv;
+        vf[n][1] *= inv;
+      }
+    }
+    // exponents against the reference; a lane checks its own, the row's maximum is only made when one is too large
+    bool grew = false;
+    float x[kPer][NT][2];
+    auto exponents = [&]() {
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+          const float off = kLift - (m[r] == -INFINITY ? 0.f : m[r]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              x[r][n][i] = fmaf(s[n][2 * r + i], F == kKvF16 ? f[r] : kf[n][i] * f[r], off);
+        }
+    };
+    auto seen = [&](int r, int n, int i) { return !masked || pos0 + key + 8 * n + 2 * tq + i < lim[r]; };
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if constexpr (FOLD) s[n][i] = join(s[n][i], s[n][2 + i]);
+    exponents();
+    float mx[kPer];
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        mx[r] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (seen(r, n, i)) mx[r] = fmaxf(mx[r], x[r][n][i]);
+        grew |= mx[r] > (m[r] == -INFINITY ? -INFINITY : kLift + kSlack);
+      }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+          float y = mx[r];
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
+          y += (m[r] == -INFINITY ? 0.f : m[r]) - kLift;
+          // whole numbers, so that neither the factors nor the differences to them round
+          const float to = fmaxf(m[r], ceilf(y));
+          const float c = to > m[r] ? ex2(m[r] - to) : 1.f;
+          m[r] = to;
+          l[r] *= c;
+#pragma unroll
+          for (int n = 0; n < HD / 8; ++n) {
+            o[n][2 * r] *= c;
+            o[n][2 * r + 1] *= c;
+            if constexpr (FOLD) {
+              o[n][2] *= c;
+              o[n][3] *= c;
+            }
+          }
+        }
+      exponents();
+    }
+    float low = 0.f;  // the smallest exponent
+#pragma unroll
+      for (int r = 0; r < kPer; ++r)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (kFar && seen(r, n, i)) low = fminf(low, x[r][n][i]);
+    const bool far = kFar && __any_sync(0xffffffffu, low < kNear);
+#pragma unroll
+    for (int n = 0; n < NT; n += 2) {
+      uint32_t p[4];
+      weigh(x, vf, n, seen, [&](int r, float y, float e) {
+        l[r] += e;
+        return far && y < kNear ? 0.f : e;
+      }, p);
+      products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) { mma16816(o[c], p, b0, b1); });
+    }
+    if constexpr (kFar) {
+      if (far) {
+#pragma unroll 1
+        for (float top = kNear, up = 38.f; top > -130.f; top -= 20.f, up += 20.f) {
+          const float down = ex2(-up);
+#pragma unroll
+          for (int n = 0; n < NT; n += 2) {
+            uint32_t p[4];
+            weigh(x, vf, n, seen, [&](int, float y, float) { return y >= top - 20.f && y < top ? ex2(y + up) : 0.f; }, p);
+            if (__any_sync(0xffffffffu, (p[0] | p[2]) != 0))
+              products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) {
+                float x[4] = {};
+                mma16816(x, p, b0, b1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[c][i] = fmaf(x[i], down, o[c][i]);
+              });
+          }
+        }
+      }
+    }
+  }
+
+  // A V scale of vtop or more: the next power of two above the largest, and the sums so far brought to it.
+  static __device__ __noinline__ float next_vtop(float vtop, float most) {
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const uint32_t e = min((__float_as_uint(most) & 0x7f800000u) + (1u << 23), 252u << 23);
+    return fmaxf(vtop, __uint_as_float(e));
+  }
+  __device__ __forceinline__ void raise_v(float most) {
+    const float to = next_vtop(vtop, most), c = vtop / to;
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] *= c;
+    vtop = to;
+  }
+
+  // Weights of 16 keys as an operand; take(r, exponent, 2^exponent) gives a seen position's weight before V's scale.
+  template <int NT, typename S, typename W>
+  __device__ __forceinline__ void weigh(const float (&x)[kPer][NT][2], const float (&vf)[NT][2], int n, S&& seen,
+                                        W&& take, uint32_t (&p)[4]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float y = x[r][n + h][i];
+            w[i] = 0.f;
+            if (seen(r, n + h, i)) {
+              w[i] = take(r, y, ex2(y));
+              if constexpr (F != kKvF16) w[i] *= vf[n + h][i];
+            }
+          }
+          const __half2 lead = __floats2half2_rn(w[0], w[1]);
+          p[2 * h + r] = half2_bits(lead);
+          if constexpr (FOLD) {
+            const float2 z = __half22float2(lead);
+            p[2 * h + 1] = half2_bits(__floats2half2_rn(w[0] - z.x, w[1] - z.y));
+          }
+        }
+  }
+
+  // The V operands of 16 keys: use(c, b0, b1) for every output tile c and row tile t.
+  template <typename U>
+  __device__ __forceinline__ void products(uint32_t v_base, int key, U&& use) {
+    const int lane = threadIdx.x & 31, mi = lane >> 3, r8 = lane & 7;
+#pragma unroll
+    for (int c = 0; c < kPieces; c += 2) {
+      uint32_t w[4];
+      ldsm4t(w, piece<F, HD, KEYS>(v_base, key + 8 * (mi & 1) + r8, c + (mi >> 1)));
+      if constexpr (F == kKvF16) {
+        {
+          use(c, w[0], w[1]);
+          use(c + 1, w[2], w[3]);
+        }
+      } else {  // a piece holds 16 dimensions: its even ones are tile 2 c, its odd ones tile 2 c + 1
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t e0, e1, d0, d1;
+          unpack<F, true>(w[2 * j], e0, d0);
+          unpack<F, true>(w[2 * j + 1], e1, d1);
+          {
+            use(2 * (c + j), e0, e1);
+            use(2 * (c + j) + 1, d0, d1);
+          }
+        }
+      }
+    }
+  }
+
+  // The row sums with V's power of two put back; l summed over the lanes of a row.
+  __device__ __forceinline__ void finish() {
+    const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
+#pragma unroll
+      for (int r = 0; r < kPer; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float& x = o[n][2 * r + i];
+            if constexpr (FOLD) x = join(x, o[n][2 + i]);
+            x *= up;
+          }
+      }
+  }
+
+  // Row r to dst[HD].
+  __device__ __forceinline__ void store(float* dst, int r) const {
+    const int tq = threadIdx.x & 3;
+    if constexpr (F == kKvF16) {
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+        *reinterpret_cast<float2*>(dst + 8 * n + 2 * tq) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < HD / 8; n += 2)
+        *reinterpret_cast<float4*>(dst + 8 * n + 4 * tq) =
+            make_float4(o[n][2 * r], o[n + 1][2 * r], o[n][2 * r + 1], o[n + 1][2 * r + 1]);
+    }
+  }
+};
+
+// Rows of the last tile past the end of the cached positions hold other data: V of f16 and e4m3 may be NaN there.
+template <int F, int HD, int KEYS>
+__device__ __forceinline__ void zero_v(uint8_t* v, int from, int to, int thread, int threads) {
+  using Gm = Tile<F, HD, KEYS>;
+  constexpr int kPer = Gm::kPart / 16;
+  for (int i = thread; i < (to - from) * kPer * Gm::kBoxes; i += threads) {
+    const int box = i / ((to - from) * kPer), j = i % ((to - from) * kPer);
+    *reinterpret_cast<uint4*>(v + box * Gm::kBoxBytes + (from + j / kPer) * Gm::kPart + (j % kPer) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  umma::fence_proxy_async_smem();
+}
+
+// ---------------------------------------------------------------- narrow
+
+// What a warp copies next: position `key` of piece x, up to `end`.  Kept in shared memory: it is used once a tile.
+struct Ahead {
+  Walk w;
+  Piece x;
+  int key, end;
+};
+
+template <int F, int HD>
+struct NarrowShared {
+  uint64_t full[kWarps][Narrow<F, HD>::kStages];
+  Ahead ahead[kWarps];
+  int abort;
+  int where[kWarps];
+  float ml[kWarps][16][2];
+  int32_t cum[kMaxScan + 1];
+};
+
+template <int F, int HD, bool FOLD, typename Q>
+__global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
+    narrow_attn_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan p, const __grid_constant__ Maps maps,
+                       const int32_t* given, int32_t* cum_out) {
+  using N = Narrow<F, HD>;
+  using Tl = typename N::Tl;
+  constexpr int KEYS = N::kKeys, RT = FOLD ? 8 : 16, kPer = FOLD ? 1 : 2;
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  __shared__ NarrowShared<F, HD> sh;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, tq = lane & 3;
+  if (t == 0) {
+    for (int i = 0; i < kWarps; ++i)
+      for (int j = 0; j < N::kStages; ++j) umma::mbar_init(&sh.full[i][j], F == kKvF16 ? 1 : 33);
+    sh.abort = 0;
+    umma::fence_barrier_init();
+  }
+  const int32_t* cum = unit_sums(a, p, given, sh.cum, cum_out);
+  __syncthreads();
+  uint8_t* tiles = smem + warp * N::kStages * N::kStage;
+  float* scales = reinterpret_cast<float*>(smem + kWarps * N::kStages * N::kStage + warp * N::kScales);
+  Ahead& ahead = sh.ahead[warp];
+  if (lane == 0) {
+    ahead.w = Walk(p, a, cum);
+    ahead.key = ahead.end = 0;
+  }
+  __syncwarp();
+  int issued = 0, done = 0;     // tiles copied and used by this warp: stage = count mod kStages
+  // Copy the warp's next tile.  The stage is the one whose tile was used last, so at least one stage is free whenever
+  // no tile is being worked on: the join at the end of a piece uses it.
+  auto copy = [&]() {
+    if (ahead.key >= ahead.end) {
+      __syncwarp();
+      if (lane == 0)  // tiles warp, warp + 4, ... of every piece
+        while (ahead.key >= ahead.end && ahead.w.next(ahead.x, p, a, cum)) {
+          ahead.key = ahead.x.t0 * N::kUnit + warp * KEYS;
+          ahead.end = min(ahead.x.t1 * N::kUnit, ahead.x.limit);
+        }
+      __syncwarp();
+      if (ahead.key >= ahead.end) return;
+    }
+    const int s = issued % N::kStages, z = ahead.x.z, pos = ahead.key;
+    const bool own = ahead.x.own != 0;
+    const KvCache& c = own ? a.own : a.prefix;
+    __syncwarp();
+    uint64_t* bar = &sh.full[warp][s];
+    const uint32_t dst = umma::smem_u32(tiles + s * N::kStage);
+    if (lane == 0) {
+      umma::mbar_arrive_expect_tx(bar, 2 * Tl::kBytes);
+      ahead.key = pos + kWarps * KEYS;
+      const CUtensorMap *mk = own ? &maps.ok : &maps.pk, *mv = own ? &maps.ov : &maps.pv;
+#pragma unroll
+      for (int b = 0; b < Tl::kBoxes; ++b) {
+        tma_load_3d(dst + b * Tl::kBoxBytes, mk, bar, b * (Tl::kPart / Tl::kEsz), pos, z);
+        tma_load_3d(dst + Tl::kBytes + b * Tl::kBoxBytes, mv, bar, b * (Tl::kPart / Tl::kEsz), pos, z);
+      }
+    }
+    if constexpr (F != kKvF16) {  // row scales: 4-byte copies, zero past the end of the cache
+      const bool in = pos + lane < c.max_seq;
+      const int64_t at = (int64_t)z * c.max_seq + (in ? pos + lane : 0);
+      const uint32_t to = umma::smem_u32(scales + s * (2 * KEYS)) + 4 * lane;
+      const int bytes = in ? 4 : 0;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(c.k_scale + at), "r"(bytes) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * KEYS), "l"(c.v_scale + at), "r"(bytes) : "memory");
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
+    }
+    ++issued;
+    __syncwarp();
+  };
+  for (int i = 0; i < N::kStages - 1; ++i) copy();
+
+  Rows<F, HD, FOLD, KEYS> st;
+  const float base = a.scale * kLog2e;
+  Walk w(p, a, cum);
+  Piece x;
+  while (w.next(x, p, a, cum)) {
+    st.clear();
+    uint32_t qa[HD / 16][4];
+    const Q* src[2];
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      src[r] = q_row<Q>(a, p, x, g + 8 * r, st.lim[r]);
+      st.f[r] = base;
+    }
+    float shrink = 1.f;
+    if constexpr (FOLD && sizeof(Q) == 4) {
+      uint32_t mx = 0;
+      if (src[0])
+#pragma unroll
+        for (int d = 0; d < HD / 4; ++d) mx = max(mx, __float_as_uint((float)src[0][4 * d + tq]) & 0x7fffffffu);
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      shrink = row_shrink(mx);
+      st.f[0] = base / shrink;
+    }
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // elements 2 tq, 2 tq + 1 (+ 8): dimensions 4 tq ... of K's words in bytes
+        const int d = F == kKvF16 ? 16 * ks + 8 * h + 2 * tq : 16 * ks + 4 * tq + 2 * h;
+#pragma unroll
+        for (int r = 0; r < kPer; ++r) {
+          const float y0 = src[r] ? (float)src[r][d] * shrink : 0.f, y1 = src[r] ? (float)src[r][d + 1] * shrink : 0.f;
+          const __half2 lead = __floats2half2_rn(y0, y1);
+          qa[ks][2 * h + r] = half2_bits(lead);
+          if constexpr (FOLD) {
+            const float2 z = __half22float2(lead);
+            qa[ks][2 * h + 1] = half2_bits(__floats2half2_rn(y0 - z.x, y1 - z.y));
+          }
+        }
+      }
+    const int end = min(x.t1 * N::kUnit, x.limit);
+#pragma unroll 1
+    for (int key = x.t0 * N::kUnit + warp * KEYS; key < end; key += kWarps * KEYS) {
+      copy();
+      const int s = done % N::kStages;
+      umma::bounded_wait(&sh.full[warp][s], (done / N::kStages) & 1, &sh.abort, a.err, kErrKvCopy);
+      uint8_t* stage = tiles + s * N::kStage;
+      const uint32_t k_base = umma::smem_u32(stage);
+      const int left = x.limit - key;
+      if (F != kKvI8 && left < KEYS) {
+        zero_v<F, HD, KEYS>(stage + Tl::kBytes, left, KEYS, lane, 32);
+        __syncwarp();
+      }
+      const float* ks = scales + s * (2 * KEYS);
+      auto frag = [&](int step, uint32_t (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = qa[step][i];
+      };
+      if (key + KEYS > x.fewest) st.template step<KEYS / 8, true>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, left, key, frag);
+      else st.template step<KEYS / 8, false>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, left, key, frag);
+      __syncwarp();
+      ++done;
+    }
+    st.finish();
+    // join the four warps' keys: each leaves its rows in its free stage
+    const int free_stage = (done + N::kStages - 1) % N::kStages;
+    float* mine = reinterpret_cast<float*>(tiles + free_stage * N::kStage);
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      st.store(mine + (g + 8 * r) * HD, r);
+      if (tq == 0) {
+        sh.ml[warp][g + 8 * r][0] = st.m[r];
+        sh.ml[warp][g + 8 * r][1] = st.l[r];
+      }
+    }
+    if (lane == 0) sh.where[warp] = (int)(reinterpret_cast<uint8_t*>(mine) - smem);
+    __syncthreads();
+    float* part = p.part + x.slot * (RT * HD);
+    float* ml = p.ml + x.slot * (RT * 2);
+    for (int i = t; i < RT * HD / 4; i += 32 * kWarps) {
+      const int row = i / (HD / 4);
+      float mx = sh.ml[0][row][0];
+#pragma unroll
+      for (int k = 1; k < kWarps; ++k) mx = fmaxf(mx, sh.ml[k][row][0]);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float f = mx == -INFINITY ? 1.f : ex2(sh.ml[k][row][0] - mx);
+        const float4 y = reinterpret_cast<const float4*>(smem + sh.where[k])[i];
+        sum.x = fmaf(f, y.x, sum.x);
+        sum.y = fmaf(f, y.y, sum.y);
+        sum.z = fmaf(f, y.z, sum.z);
+        sum.w = fmaf(f, y.w, sum.w);
+        l = fmaf(f, sh.ml[k][row][1], l);
+      }
+      reinterpret_cast<float4*>(part)[i] = sum;
+      if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(ml + 2 * row) = make_float2(mx, l);
+    }
+    umma::fence_proxy_async_smem();  // the stages take copies again
+    __syncthreads();
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (*(volatile int*)&sh.abort) grace();
+}
+
+}  // namespace attn
+}  // namespace uaii_b200

@@ -1,0 +1,553 @@
+// attn_wide.cuh -- attention items of many rows on tcgen05 (see prefix_attn.cu).
+//
+// One CTA per SM works on two row tiles of 128: two softmax warpgroups alternate, so that the tensor core works on one
+// tile's products while the other's exponentials are made.
+//   rows split   the item's 256 rows are the two tiles, and every key tile serves both (f16 queries, many rows)
+//   keys split   the item's 128 rows are both, and each takes every other key tile (f32 queries, whose leading parts and
+//                rests are two operands added into one accumulator; or up to 128 rows)
+// Per key tile of 64: copied bytes -> (four warps) f16 operands in shared memory, K as [key][dim], V transposed to
+// [dim][key] -> S = Q K^T, Q from tensor memory -> (a thread per row) 2^(S - m), weights packed into the tensor memory
+// that held S -> O += P V, P from tensor memory.  Q and P in tensor memory leave shared memory's bandwidth to K and V:
+// with Q there as well, S alone would read 6 KB per 32 cycles of products.
+// Tensor memory: S and P of tile r at column 64 r, Q at 128 + 64 r, O at 256 + 128 r.
+#pragma once
+
+#include "attn_common.cuh"
+
+namespace uaii_b200 {
+namespace attn {
+
+template <int F, int HD>
+struct Wide {
+  using Tl = Tile<F, HD, kTile>;
+  static constexpr int kRaw = 2 * Tl::kBytes;                       // K, then V
+  static constexpr int kRawStages = kRaw > 16384 ? 2 : 3;
+  static constexpr int kOpK = kTile * HD * 2, kOp = 2 * kOpK;       // K as [HD / 64][64 keys][128 B], V as [HD][128 B]
+  static constexpr int kSmem = 2 * kOp + kRawStages * kRaw + 1024;
+  static constexpr int kSoft = 256, kConvert = 128, kThreads = kSoft + kConvert + 64;
+};
+
+template <int F, int HD>
+struct WideShared {
+  static constexpr int kRawStages = Wide<F, HD>::kRawStages;
+  uint64_t raw_full[kRawStages], raw_empty[kRawStages], op_full[2], op_empty[2];
+  uint64_t q_full, s_full[2], p_full[2], o_done[2];
+  uint32_t tmem;
+  int abort;
+  alignas(16) float raw_scale[kRawStages][2][kTile];
+  alignas(16) float kf[2][kTile];   // K scale * softmax scale * log2(e)
+  alignas(16) float vf[2][kTile];   // V scale * 2 / vtop: below 2
+  float vtop[2];
+  int32_t cum[kMaxScan + 1];
+};
+
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+__device__ __forceinline__ int tiles_of(const Piece& x) { return min(x.t1, (x.limit + kTile - 1) / kTile) - x.t0; }
+
+// ---------------------------------------------------------------- copies
+
+template <int F, int HD>
+__device__ void wide_copy(const PrefixAttnArgs& a, const Plan& p, const Maps& maps, const int32_t* cum, uint8_t* raw,
+                          WideShared<F, HD>& sh) {
+  using Wd = Wide<F, HD>;
+  using Tl = typename Wd::Tl;
+  const int lane = threadIdx.x & 31;
+  Walk w(p, a, cum);
+  Piece x;
+  int count = 0;
+  while (w.next(x, p, a, cum)) {
+    const KvCache& c = x.own ? a.own : a.prefix;
+    const CUtensorMap *mk = x.own ? &maps.ok : &maps.pk, *mv = x.own ? &maps.ov : &maps.pv;
+    for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
+      const int s = count % Wd::kRawStages, pos = (x.t0 + i) * kTile;
+      umma::bounded_wait(&sh.raw_empty[s], ((count / Wd::kRawStages) & 1) ^ 1, &sh.abort, a.err, kErrKvCopy);
+      if (*(volatile int*)&sh.abort) return;
+      uint64_t* bar = &sh.raw_full[s];
+      if (lane == 0) {
+        umma::mbar_arrive_expect_tx(bar, 2 * Tl::kBytes);
+        const uint32_t dst = umma::smem_u32(raw + s * Wd::kRaw);
+#pragma unroll
+        for (int b = 0; b < Tl::kBoxes; ++b) {
+          tma_load_3d(dst + b * Tl::kBoxBytes, mk, bar, b * (Tl::kPart / Tl::kEsz), pos, x.z);
+          tma_load_3d(dst + Tl::kBytes + b * Tl::kBoxBytes, mv, bar, b * (Tl::kPart / Tl::kEsz), pos, x.z);
+        }
+      }
+      if constexpr (F != kKvF16) {  // row scales: 4-byte copies, zero past the end of the cache
+#pragma unroll
+        for (int j = 0; j < 2 * kTile / 32; ++j) {
+          const int k = (j % (kTile / 32)) * 32 + lane;
+          const bool in = pos + k < c.max_seq;
+          const float* src = (j < kTile / 32 ? c.k_scale : c.v_scale) + (int64_t)x.z * c.max_seq + (in ? pos + k : 0);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(umma::smem_u32(&sh.raw_scale[s][0][0]) + (j * 32 + lane) * 4),
+                       "l"(src), "r"(in ? 4 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
+      }
+      __syncwarp();
+    }
+  }
+}
+
+// ---------------------------------------------------------------- bytes to operands
+
+template <int F, int HD>
+__device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, uint8_t* raw,
+                             WideShared<F, HD>& sh) {
+  using Wd = Wide<F, HD>;
+  using Tl = typename Wd::Tl;
+  constexpr int kPieces = Tl::kRow / 16;
+  const int lane = threadIdx.x & 31, cw = ((int)threadIdx.x - Wd::kSoft) >> 5;  // keys 16 cw .. 16 cw + 15
+  const int mi = lane >> 3, r8 = lane & 7, tq = lane & 3;
+  const float base = a.scale * kLog2e;
+  Walk w(p, a, cum);
+  Piece x;
+  int count = 0;
+  while (w.next(x, p, a, cum)) {
+    float vtop = 0x1p-100f;
+    for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
+      const int s = count % Wd::kRawStages, o = count & 1, left = x.limit - (x.t0 + i) * kTile;
+      umma::bounded_wait(&sh.raw_full[s], (count / Wd::kRawStages) & 1, &sh.abort, a.err, kErrKvCopy);
+      umma::bounded_wait(&sh.op_empty[o], ((count >> 1) & 1) ^ 1, &sh.abort, a.err, kErrKvCopy);
+      const uint32_t rk = umma::smem_u32(raw + s * Wd::kRaw), rv = rk + Tl::kBytes;
+      const uint32_t ok = umma::smem_u32(ops + o * Wd::kOp), ov = ok + Wd::kOpK;
+      // K: 16-byte chunk c of an operand row holds positions 8 c ... of the MMA's K axis; chunks of 64 dimensions apart
+      // lie 8 KB apart
+      auto k_to = [&](int row, int c) { return ok + (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4); };
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int row = 16 * cw + 8 * g + r8;
+#pragma unroll
+        for (int c = 0; c < kPieces; c += 4) {
+          uint32_t v[4];
+          ldsm4(v, piece<F, HD, kTile>(rk, row, c + mi));
+          if constexpr (F == kKvF16) {
+            stsm4(k_to(row, c + mi), v[0], v[1], v[2], v[3]);
+          } else {  // a word's four dimensions go to chunks 2 c and 2 c + 1 (operand_dim)
+            uint32_t b[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpack<F, false>(v[j], b[2 * j], b[2 * j + 1]);
+            stsm4(k_to(row, 2 * c + mi), b[0], b[1], b[2], b[3]);
+            stsm4(k_to(row, 2 * c + 4 + mi), b[4], b[5], b[6], b[7]);
+          }
+        }
+      }
+      // V transposed: 8-bit pieces hold 16 dimensions, whose even ones become rows 16 c .. 16 c + 7 and odd ones the next
+      // eight.  Nothing is stored past the item's last position: zeros, since 0 * NaN would not be 0.
+      auto v_to = [&](int row) { return ov + row * 128 + (((2 * cw + (mi & 1)) ^ (row & 7)) << 4); };
+      auto keep = [&](uint32_t pair, int key) {
+        if (key + 1 < left) return pair;
+        return key < left ? pair & 0xffffu : 0u;
+      };
+#pragma unroll
+      for (int c = 0; c < kPieces; c += 2) {
+        uint32_t v[4];
+        ldsm4t(v, piece<F, HD, kTile>(rv, 16 * cw + 8 * (mi & 1) + r8, c + (mi >> 1)));
+        const int lo = 16 * cw + 2 * tq, hi = lo + 8;
+        if constexpr (F == kKvF16) {
+          if (left < kTile) {
+            v[0] = keep(v[0], lo); v[1] = keep(v[1], hi);
+            v[2] = keep(v[2], lo); v[3] = keep(v[3], hi);
+          }
+          stsm4(v_to(8 * (c + (mi >> 1)) + r8), v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t e0, d0, e1, d1;
+            unpack<F, true>(v[2 * j], e0, d0);
+            unpack<F, true>(v[2 * j + 1], e1, d1);
+            if (F == kKvE4M3 && left < kTile) {
+              e0 = keep(e0, lo); d0 = keep(d0, lo);
+              e1 = keep(e1, hi); d1 = keep(d1, hi);
+            }
+            stsm4(v_to(16 * (c + j) + 8 * (mi >> 1) + r8), e0, e1, d0, d1);
+          }
+        }
+      }
+      if constexpr (F != kKvF16) {
+        if (cw == 0) {  // the tile's column factors
+          float kx[2], vx[2], most = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            kx[j] = sh.raw_scale[s][0][32 * j + lane];
+            vx[j] = 32 * j + lane < left ? sh.raw_scale[s][1][32 * j + lane] : 0.f;
+            most = fmaxf(most, vx[j]);  // (a NaN shows in its products, not here)
+          }
+          if (__any_sync(0xffffffffu, most >= vtop)) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            vtop = fmaxf(vtop, __uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + (1u << 23), 252u << 23)));
+          }
+          const float inv = __uint_as_float(0x7f800000u - __float_as_uint(vtop));  // 2 / vtop
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            sh.kf[o][32 * j + lane] = kx[j] * base;
+            sh.vf[o][32 * j + lane] = vx[j] * inv;
+          }
+          if (lane == 0) sh.vtop[o] = vtop;
+        }
+      }
+      umma::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        umma::mbar_arrive(&sh.raw_empty[s]);
+        umma::mbar_arrive(&sh.op_full[o]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- products
+
+template <int F, int HD, bool SPLIT_Q>
+__device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, WideShared<F, HD>& sh) {
+  using Wd = Wide<F, HD>;
+  constexpr uint32_t kIdS = umma::idesc_f16_f32(128, kTile), kIdO = umma::idesc_f16_f32(128, HD);
+  const uint32_t tm = sh.tmem;
+  Walk w(p, a, cum);
+  Piece x;
+  int count = 0, pieces = 0;
+  uint32_t p_seen[2] = {0, 0}, o_made[2] = {0, 0};
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    umma::bounded_wait(bar, parity, &sh.abort, a.err, kErrKvCopy);
+    umma::tc_fence_after();
+  };
+  auto scores = [&](int r, int stage) {  // S_r = Q K^T
+    const uint64_t k = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp));
+#pragma unroll
+    for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part) {
+      const uint32_t q = tm + 128 + (SPLIT_Q ? 64 * part : p.split_keys ? 0 : 64 * r);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)  // 32 bytes a step, 64 dimensions a swizzled block
+        umma::mma_f16_ts(tm + 64 * r, q + 8 * ks, k + (uint64_t)(((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4), kIdS, part | ks);
+    }
+    umma::mma_commit(&sh.s_full[r]);
+  };
+  auto outputs = [&](int r, int stage, bool first) {  // O_r += P V
+    wait(&sh.p_full[r], p_seen[r]++ & 1);
+    const uint64_t v = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp + Wd::kOpK));
+#pragma unroll
+    for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
+#pragma unroll
+      for (int ks = 0; ks < kTile / 16; ++ks)
+        umma::mma_f16_ts(tm + 256 + 128 * r, tm + 64 * r + 32 * part + 8 * ks, v + 2 * ks, kIdO, !first || part || ks);
+    umma::mma_commit(&sh.o_done[r]);
+    ++o_made[r];
+  };
+  while (w.next(x, p, a, cum)) {
+    const int n = tiles_of(x);
+    if (n <= 0) continue;
+    wait(&sh.q_full, pieces++ & 1);
+    for (int i = 0; i < n; ++i, ++count) {
+      const int o = count & 1;
+      wait(&sh.op_full[o], (count >> 1) & 1);
+      if (p.split_keys) {
+        const int r = i & 1;
+        if (i >= 2) wait(&sh.o_done[r], (o_made[r] - 1) & 1);  // P's place is S's
+        scores(r, o);
+        if (i >= 1) {
+          outputs(r ^ 1, o ^ 1, i < 3);
+          umma::mma_commit(&sh.op_empty[o ^ 1]);
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if (i > 0) {
+            outputs(r, o ^ 1, i == 1);
+            if (r == 1) umma::mma_commit(&sh.op_empty[o ^ 1]);
+            wait(&sh.o_done[r], (o_made[r] - 1) & 1);
+          }
+          scores(r, o);
+        }
+      }
+    }
+    const int o = (count - 1) & 1;
+    if (p.split_keys) {
+      outputs((n - 1) & 1, o, n < 3);
+    } else {
+      outputs(0, o, n == 1);
+      outputs(1, o, n == 1);
+    }
+    umma::mma_commit(&sh.op_empty[o]);
+  }
+}
+
+// ---------------------------------------------------------------- softmax
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Operand position -> dimension: K's words hold four consecutive dimensions of a byte row, which lie in two chunks of an
+// operand row.  Even positions keep their neighbour.
+template <int F>
+__device__ __forceinline__ int operand_dim(int pos) {
+  if constexpr (F == kKvF16) return pos;
+  return (pos & ~15) | ((pos & 6) << 1) | ((pos & 8) >> 2) | (pos & 1);
+}
+
+// This thread's row of q (null: zeros) into tensor memory as operand `part` (1: the rests of a split); returns the power
+// of two by which a split row was multiplied.
+template <int F, int HD, bool SPLIT_Q, typename Q>
+__device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_t taddr) {
+  float shrink = 1.f;
+  auto load16 = [&](int g, float (&v)[16]) {  // dimensions 16 g ... 16 g + 15
+    if (src == nullptr) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    } else if (vec) {
+      Q e[16];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(Q); ++i)
+        reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(src + 16 * g)[i];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = (float)e[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = (float)src[16 * g + i];
+    }
+  };
+  if constexpr (SPLIT_Q) {
+    uint32_t mx = 0;
+#pragma unroll 2
+    for (int g = 0; g < HD / 16; ++g) {
+      float v[16];
+      load16(g, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+    shrink = row_shrink(mx);
+  }
+#pragma unroll
+  for (int h = 0; h < HD / 64; ++h) {
+    uint32_t c[32];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float v[16];
+      load16(4 * h + g, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = operand_dim<F>(2 * j);
+        const float y0 = v[d] * shrink, y1 = v[d + 1] * shrink;
+        __half2 e = __floats2half2_rn(y0, y1);
+        if (SPLIT_Q && part) {
+          const float2 z = __half22float2(e);
+          e = __floats2half2_rn(y0 - z.x, y1 - z.y);
+        }
+        c[8 * g + j] = half2_bits(e);
+      }
+    }
+    umma::tmem_st32(taddr + 32 * h, c);
+  }
+  umma::tmem_st_wait();
+  return shrink;
+}
+
+template <int F, int HD, bool SPLIT_Q, typename Q>
+__device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, WideShared<F, HD>& sh) {
+  const int lane = threadIdx.x & 31, warp = (int)threadIdx.x >> 5, r = warp >> 2, row = threadIdx.x & 127;
+  const uint32_t tm = sh.tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's 32 lanes of tensor memory
+  const uint32_t ts = tm + 64 * r, to = tm + 256 + 128 * r;
+  const float base = a.scale * kLog2e;
+  Walk w(p, a, cum);
+  Piece x;
+  int count = 0;            // key tiles of the CTA
+  uint32_t mine = 0;        // key tiles of this warpgroup
+  while (w.next(x, p, a, cum)) {
+    const int n = tiles_of(x), step = p.split_keys ? 2 : 1, first = p.split_keys ? r : 0;
+    int lim;
+    const Q* src = q_row<Q>(a, p, x, p.split_keys ? row : 128 * r + row, lim);
+    float m = -INFINITY, l = 0.f, row_f = 1.f, vtop = 0x1p-100f;
+    if (n > 0) {
+      if (p.split_keys) asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's products with q are done
+      const float shrink = put_q<F, HD, SPLIT_Q, Q>(src, a.q_vec, r, tm + 128 + 64 * r);
+      if constexpr (SPLIT_Q) row_f = 1.f / shrink;
+      umma::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(&sh.q_full);
+    }
+    for (int i = first; i < n; i += step, ++mine) {
+      const int at = count + i, o = at & 1, pos0 = (x.t0 + i) * kTile;
+      umma::bounded_wait(&sh.op_full[o], (at >> 1) & 1, &sh.abort, a.err, kErrKvCopy);  // the column factors
+      umma::bounded_wait(&sh.s_full[r], mine & 1, &sh.abort, a.err, kErrKvCopy);
+      umma::tc_fence_after();
+      float s[kTile];
+      tmem_ld32(ts, reinterpret_cast<uint32_t*>(s));
+      tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(s) + 32);
+      umma::tmem_ld_wait();
+      const bool masked = pos0 + kTile > x.fewest;
+      const int seen = masked ? lim - pos0 : kTile;
+      if constexpr (F == kKvF16) {
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) s[j] *= base;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kTile; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&sh.kf[o][j]);
+          s[j] *= f.x; s[j + 1] *= f.y; s[j + 2] *= f.z; s[j + 3] *= f.w;
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < kTile; ++j)
+          if (j >= seen) s[j] = -INFINITY;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_f;
+      float shrink_o = 1.f;
+      if (F != kKvF16 && sh.vtop[o] != vtop) {
+        shrink_o = vtop / sh.vtop[o];
+        vtop = sh.vtop[o];
+      }
+      if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
+        const float t = ceilf(top), c = ex2(m - t);
+        l *= c;
+        shrink_o *= c;
+        m = t;
+      }
+      if (i != first && __any_sync(0xffffffffu, shrink_o != 1.f)) {  // S came after the last products: O is at rest
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t y[32];
+          tmem_ld32(to + 32 * c, y);
+          umma::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
+          umma::tmem_st32(to + 32 * c, y);
+        }
+      }
+      const float off = kLift - (m == -INFINITY ? 0.f : m);
+      float sum[4] = {};
+#pragma unroll
+      for (int j = 0; j < kTile; ++j) {
+        s[j] = ex2(fmaf(s[j], row_f, off));
+        sum[j & 3] += s[j];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if constexpr (F != kKvF16) {
+#pragma unroll
+        for (int j = 0; j < kTile; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&sh.vf[o][j]);
+          s[j] *= f.x; s[j + 1] *= f.y; s[j + 2] *= f.z; s[j + 3] *= f.w;
+        }
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < kTile; ++j)
+            if (j >= seen) s[j] = 0.f;  // whatever the scale there
+        }
+      }
+      uint32_t pk[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const __half2 e = __floats2half2_rn(s[2 * j], s[2 * j + 1]);
+        pk[j] = half2_bits(e);
+        if constexpr (SPLIT_Q) {
+          const float2 z = __half22float2(e);
+          s[2 * j] -= z.x;
+          s[2 * j + 1] -= z.y;
+        }
+      }
+      umma::tmem_st32(ts, pk);
+      if constexpr (SPLIT_Q) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) pk[j] = half2_bits(__floats2half2_rn(s[2 * j], s[2 * j + 1]));
+        umma::tmem_st32(ts + 32, pk);
+      }
+      umma::tmem_st_wait();
+      umma::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) umma::mbar_arrive(&sh.p_full[r]);
+    }
+    count += n > 0 ? n : 0;
+    const int64_t at = x.slot * 256 + 128 * r + row;
+    float* part = p.part + at * HD;
+    *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m, l);
+    if (n > first) {
+      umma::bounded_wait(&sh.o_done[r], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
+      umma::tc_fence_after();
+      const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t u[32];
+        tmem_ld32(to + 32 * c, u);
+        umma::tmem_ld_wait();
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(u[j]) * up;
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          // 8-bit pieces: even dimensions of 16 lie before the odd ones
+          const int e = (j & 16) + ((j & 15) >> 1);
+          reinterpret_cast<float4*>(part + 32 * c + j)[0] =
+              F == kKvF16 ? make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]) : make_float4(y[e], y[e + 8], y[e + 1], y[e + 9]);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int j = 0; j < HD; j += 4) reinterpret_cast<float4*>(part + j)[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    umma::tc_fence_before();
+  }
+}
+
+template <int F, int HD, typename Q>
+__global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
+    wide_attn_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan p, const __grid_constant__ Maps maps,
+                     const int32_t* given, int32_t* cum_out) {
+  using Wd = Wide<F, HD>;
+  constexpr bool kSplitQ = sizeof(Q) == 4;
+  extern __shared__ uint8_t dynamic[];
+  uint8_t* ops = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t(1023));
+  uint8_t* raw = ops + 2 * Wd::kOp;
+  __shared__ WideShared<F, HD> sh;
+  const int t = threadIdx.x, warp = t >> 5;
+  constexpr int kCopyWarp = (Wd::kSoft + Wd::kConvert) / 32, kProductWarp = kCopyWarp + 1;
+  if (t == 0) {
+    for (int i = 0; i < Wd::kRawStages; ++i) {
+      umma::mbar_init(&sh.raw_full[i], F == kKvF16 ? 1 : 33);
+      umma::mbar_init(&sh.raw_empty[i], Wd::kConvert / 32);
+    }
+    for (int i = 0; i < 2; ++i) {
+      umma::mbar_init(&sh.op_full[i], Wd::kConvert / 32);
+      umma::mbar_init(&sh.op_empty[i], 1);
+      umma::mbar_init(&sh.s_full[i], 1);
+      umma::mbar_init(&sh.p_full[i], 4);
+      umma::mbar_init(&sh.o_done[i], 1);
+    }
+    umma::mbar_init(&sh.q_full, 8);
+    sh.abort = 0;
+    umma::fence_barrier_init();
+  }
+  if (warp == kProductWarp) umma::tmem_alloc(&sh.tmem, 512);
+  const int32_t* cum = unit_sums(a, p, given, sh.cum, cum_out);
+  umma::tc_fence_before();
+  __syncthreads();
+  umma::tc_fence_after();
+  if (t < Wd::kSoft) wide_softmax<F, HD, kSplitQ, Q>(a, p, cum, sh);
+  else if (t < Wd::kSoft + Wd::kConvert) wide_convert<F, HD>(a, p, cum, ops, raw, sh);
+  else if (warp == kCopyWarp) wide_copy<F, HD>(a, p, maps, cum, raw, sh);
+  else if ((t & 31) == 0) wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh);
+  __syncwarp();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (*(volatile int*)&sh.abort) grace();
+  umma::tc_fence_before();
+  __syncthreads();
+  if (warp == kProductWarp) umma::tmem_dealloc(sh.tmem, 512);
+}
+
+}  // namespace attn
+}  // namespace uaii_b200

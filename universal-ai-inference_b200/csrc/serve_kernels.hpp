@@ -51,6 +51,7 @@ struct PrefixAttnArgs {
   const int32_t* own_len = nullptr;
   const void* q = nullptr;
   bool half = false;
+  bool q_vec = false;  // every row of q starts on a 16-byte boundary (set by launch_prefix_attn)
   int64_t B = 0, T = 0, H = 0;
   RowView qs;
   float scale = 0.f;
@@ -58,7 +59,7 @@ struct PrefixAttnArgs {
   int* err = nullptr;
 };
 size_t prefix_attn_ws(const PrefixAttnArgs& a);
-cudaError_t launch_prefix_attn(const PrefixAttnArgs& a, void* ws, int* launches, cudaStream_t st);
+cudaError_t launch_prefix_attn(PrefixAttnArgs a, void* ws, int* launches, cudaStream_t st);
 
 // One token per row of logits [B, V] (f16 when half, else f32; rows ld elements apart); probs and kept may be null.
 cudaError_t launch_sample(const void* logits, bool half, int64_t B, int64_t V, int64_t ld, const float* temperature,
