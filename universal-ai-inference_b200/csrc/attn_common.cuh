@@ -52,6 +52,7 @@ struct Plan {
   int prefix_units;        // units of a prefix item
   int prefix_items;
   int grid;                // CTAs (0: the kernel has no work)
+  int workers;             // shares of the work: wide CTAs or narrow warps
   float* part;             // partial sums [slot][slot_rows][hd]
   float* ml;               // (maximum, denominator) of each partial row
 };
@@ -114,37 +115,37 @@ __device__ __forceinline__ uint32_t piece(uint32_t base, int r, int c) {
   else return base + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-// ---------------------------------------------------------------- the walk over a CTA's pieces
+// ---------------------------------------------------------------- the walk over a worker's pieces
 
 struct Piece {
-  int64_t slot;      // item + CTA
+  int64_t slot;      // item + worker
   int own;
   int z, kvh, rt;    // plane of the cache; kv head, row tile
   int seq;           // own items: the sequence
-  int t0, t1;        // units of this CTA
+  int t0, t1;        // units of this worker
   int limit;         // positions that some row of the item sees
   int fewest;        // positions that every row sees
 };
 
-// The first unit of CTA c: the first total % grid CTAs take one unit more than the others.
-__device__ __forceinline__ int share_start(int c, int total, int grid) {
-  const int each = total / grid;
-  return c * each + min(c, total - each * grid);
+// The first unit of worker c: the first total % n workers take one unit more than the others.
+__device__ __forceinline__ int share_start(int c, int total, int n) {
+  const int each = total / n;
+  return c * each + min(c, total - each * n);
 }
-// The CTA that holds unit u < total.
-__device__ __forceinline__ int share_of(int u, int total, int grid) {
-  const int each = total / grid, more = total - each * grid, split = more * (each + 1);
+// The worker that holds unit u < total.
+__device__ __forceinline__ int share_of(int u, int total, int n) {
+  const int each = total / n, more = total - each * n, split = more * (each + 1);
   return u < split ? u / (each + 1) : more + (u - split) / each;
 }
 
 struct Walk {
-  int u, end, b;
+  int u, end, b, worker;
   Walk() = default;
-  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) : b(0) {
+  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum, int worker_) : b(0), worker(worker_) {
     const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
     const int total = prefix + (per ? cum[a.B] * per : 0);
-    u = share_start(blockIdx.x, total, gridDim.x);
-    end = share_start(blockIdx.x + 1, total, gridDim.x);
+    u = share_start(worker, total, p.workers);
+    end = share_start(worker + 1, total, p.workers);
     if (end > prefix) {  // the last sequence whose units start at or before the first own unit
       const int first = max(u - prefix, 0);
       int lo = 0, hi = (int)a.B - 1;
@@ -190,7 +191,7 @@ struct Walk {
     const int n = min(units - in, end - u);
     x.t0 = in;
     x.t1 = in + n;
-    x.slot += blockIdx.x;
+    x.slot += worker;
     u += n;
     return true;
   }

@@ -6,8 +6,8 @@
 namespace uaii_b200 {
 namespace attn {
 
-// Narrow: each warp copies for itself, kKeys positions at a time, the next ones while it works.  Three CTAs of four
-// warps hold 190 KB of an SM, about half of it in flight.
+// Narrow: every warp is a worker of its own, with its own copies: kKeys positions at a time, the next ones while it
+// works.  Three CTAs of four warps hold 200 KB of an SM, about half of it in flight.
 template <int F, int HD>
 struct Narrow {
   static constexpr int kKeys = F == kKvF16 && HD == 128 ? 16 : 32;
@@ -16,7 +16,6 @@ struct Narrow {
   static constexpr int kStages = 16 * 1024 / kStage;
   static constexpr int kScales = kStages * Tl::kScaleBytes; // of one warp, after all the tiles
   static constexpr int kSmem = kWarps * (kStages * kStage + kScales) + 1024;
-  static constexpr int kUnit = kWarps * kKeys;
 };
 
 // ---------------------------------------------------------------- one warp's running softmax
@@ -346,8 +345,6 @@ struct NarrowShared {
   uint64_t full[kWarps][Narrow<F, HD>::kStages];
   Ahead ahead[kWarps];
   int abort;
-  int where[kWarps];
-  float ml[kWarps][16][2];
   int32_t cum[kMaxScan + 1];
 };
 
@@ -362,6 +359,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   __shared__ NarrowShared<F, HD> sh;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, tq = lane & 3;
+  const int worker = blockIdx.x * kWarps + warp;
   if (t == 0) {
     for (int i = 0; i < kWarps; ++i)
       for (int j = 0; j < N::kStages; ++j) umma::mbar_init(&sh.full[i][j], F == kKvF16 ? 1 : 33);
@@ -374,20 +372,19 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
   float* scales = reinterpret_cast<float*>(smem + kWarps * N::kStages * N::kStage + warp * N::kScales);
   Ahead& ahead = sh.ahead[warp];
   if (lane == 0) {
-    ahead.w = Walk(p, a, cum);
+    ahead.w = Walk(p, a, cum, worker);
     ahead.key = ahead.end = 0;
   }
   __syncwarp();
   int issued = 0, done = 0;     // tiles copied and used by this warp: stage = count mod kStages
-  // Copy the warp's next tile.  The stage is the one whose tile was used last, so at least one stage is free whenever
-  // no tile is being worked on: the join at the end of a piece uses it.
+  // Copy the warp's next tile into the stage whose tile was used last.
   auto copy = [&]() {
     if (ahead.key >= ahead.end) {
       __syncwarp();
-      if (lane == 0)  // tiles warp, warp + 4, ... of every piece
+      if (lane == 0)
         while (ahead.key >= ahead.end && ahead.w.next(ahead.x, p, a, cum)) {
-          ahead.key = ahead.x.t0 * N::kUnit + warp * KEYS;
-          ahead.end = min(ahead.x.t1 * N::kUnit, ahead.x.limit);
+          ahead.key = ahead.x.t0 * KEYS;
+          ahead.end = min(ahead.x.t1 * KEYS, ahead.x.limit);
         }
       __syncwarp();
       if (ahead.key >= ahead.end) return;
@@ -400,7 +397,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     const uint32_t dst = umma::smem_u32(tiles + s * N::kStage);
     if (lane == 0) {
       umma::mbar_arrive_expect_tx(bar, 2 * Tl::kBytes);
-      ahead.key = pos + kWarps * KEYS;
+      ahead.key = pos + KEYS;
       const CUtensorMap *mk = own ? &maps.ok : &maps.pk, *mv = own ? &maps.ov : &maps.pv;
 #pragma unroll
       for (int b = 0; b < Tl::kBoxes; ++b) {
@@ -424,7 +421,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
 
   Rows<F, HD, FOLD, KEYS> st;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum);
+  Walk w(p, a, cum, worker);
   Piece x;
   while (w.next(x, p, a, cum)) {
     st.clear();
@@ -462,9 +459,9 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
           }
         }
       }
-    const int end = min(x.t1 * N::kUnit, x.limit);
+    const int end = min(x.t1 * KEYS, x.limit);
 #pragma unroll 1
-    for (int key = x.t0 * N::kUnit + warp * KEYS; key < end; key += kWarps * KEYS) {
+    for (int key = x.t0 * KEYS; key < end; key += KEYS) {
       copy();
       const int s = done % N::kStages;
       umma::bounded_wait(&sh.full[warp][s], (done / N::kStages) & 1, &sh.abort, a.err, kErrKvCopy);
@@ -486,43 +483,12 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
       ++done;
     }
     st.finish();
-    // join the four warps' keys: each leaves its rows in its free stage
-    const int free_stage = (done + N::kStages - 1) % N::kStages;
-    float* mine = reinterpret_cast<float*>(tiles + free_stage * N::kStage);
+    float* part = p.part + x.slot * (RT * HD);
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      st.store(mine + (g + 8 * r) * HD, r);
-      if (tq == 0) {
-        sh.ml[warp][g + 8 * r][0] = st.m[r];
-        sh.ml[warp][g + 8 * r][1] = st.l[r];
-      }
+      st.store(part + (g + 8 * r) * HD, r);
+      if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], st.l[r]);
     }
-    if (lane == 0) sh.where[warp] = (int)(reinterpret_cast<uint8_t*>(mine) - smem);
-    __syncthreads();
-    float* part = p.part + x.slot * (RT * HD);
-    float* ml = p.ml + x.slot * (RT * 2);
-    for (int i = t; i < RT * HD / 4; i += 32 * kWarps) {
-      const int row = i / (HD / 4);
-      float mx = sh.ml[0][row][0];
-#pragma unroll
-      for (int k = 1; k < kWarps; ++k) mx = fmaxf(mx, sh.ml[k][row][0]);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      float l = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const float f = mx == -INFINITY ? 1.f : ex2(sh.ml[k][row][0] - mx);
-        const float4 y = reinterpret_cast<const float4*>(smem + sh.where[k])[i];
-        sum.x = fmaf(f, y.x, sum.x);
-        sum.y = fmaf(f, y.y, sum.y);
-        sum.z = fmaf(f, y.z, sum.z);
-        sum.w = fmaf(f, y.w, sum.w);
-        l = fmaf(f, sh.ml[k][row][1], l);
-      }
-      reinterpret_cast<float4*>(part)[i] = sum;
-      if (i % (HD / 4) == 0) *reinterpret_cast<float2*>(ml + 2 * row) = make_float2(mx, l);
-    }
-    umma::fence_proxy_async_smem();  // the stages take copies again
-    __syncthreads();
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&sh.abort) grace();

@@ -12,6 +12,8 @@
 // Tensor memory: S and P of tile r at column 64 r, Q at 128 + 64 r, O at 256 + 128 r.
 #pragma once
 
+#include <type_traits>
+
 #include "attn_common.cuh"
 
 namespace uaii_b200 {
@@ -56,7 +58,7 @@ __device__ void wide_copy(const PrefixAttnArgs& a, const Plan& p, const Maps& ma
   using Wd = Wide<F, HD>;
   using Tl = typename Wd::Tl;
   const int lane = threadIdx.x & 31;
-  Walk w(p, a, cum);
+  Walk w(p, a, cum, blockIdx.x);
   Piece x;
   int count = 0;
   while (w.next(x, p, a, cum)) {
@@ -104,7 +106,7 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32
   const int lane = threadIdx.x & 31, cw = ((int)threadIdx.x - Wd::kSoft) >> 5;  // keys 16 cw .. 16 cw + 15
   const int mi = lane >> 3, r8 = lane & 7, tq = lane & 3;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum);
+  Walk w(p, a, cum, blockIdx.x);
   Piece x;
   int count = 0;
   while (w.next(x, p, a, cum)) {
@@ -208,7 +210,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
   using Wd = Wide<F, HD>;
   constexpr uint32_t kIdS = umma::idesc_f16_f32(128, kTile), kIdO = umma::idesc_f16_f32(128, HD);
   const uint32_t tm = sh.tmem;
-  Walk w(p, a, cum);
+  Walk w(p, a, cum, blockIdx.x);
   Piece x;
   int count = 0, pieces = 0;
   uint32_t p_seen[2] = {0, 0}, o_made[2] = {0, 0};
@@ -216,8 +218,14 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
     umma::bounded_wait(bar, parity, &sh.abort, a.err, kErrKvCopy);
     umma::tc_fence_after();
   };
+  // The whole warp stays together and one lane issues: the descriptors then live in uniform registers.
+  auto commit = [&](uint64_t* bar) {
+    if (umma::elect_one()) umma::mma_commit(bar);
+    __syncwarp();
+  };
   auto scores = [&](int r, int stage) {  // S_r = Q K^T
     const uint64_t k = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp));
+    if (umma::elect_one()) {
 #pragma unroll
     for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part) {
       const uint32_t q = tm + 128 + (SPLIT_Q ? 64 * part : p.split_keys ? 0 : 64 * r);
@@ -226,16 +234,21 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
         umma::mma_f16_ts(tm + 64 * r, q + 8 * ks, k + (uint64_t)(((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4), kIdS, part | ks);
     }
     umma::mma_commit(&sh.s_full[r]);
+    }
+    __syncwarp();
   };
   auto outputs = [&](int r, int stage, bool first) {  // O_r += P V
     wait(&sh.p_full[r], p_seen[r]++ & 1);
     const uint64_t v = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp + Wd::kOpK));
+    if (umma::elect_one()) {
 #pragma unroll
     for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
 #pragma unroll
       for (int ks = 0; ks < kTile / 16; ++ks)
         umma::mma_f16_ts(tm + 256 + 128 * r, tm + 64 * r + 32 * part + 8 * ks, v + 2 * ks, kIdO, !first || part || ks);
     umma::mma_commit(&sh.o_done[r]);
+    }
+    __syncwarp();
     ++o_made[r];
   };
   while (w.next(x, p, a, cum)) {
@@ -251,14 +264,14 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
         scores(r, o);
         if (i >= 1) {
           outputs(r ^ 1, o ^ 1, i < 3);
-          umma::mma_commit(&sh.op_empty[o ^ 1]);
+          commit(&sh.op_empty[o ^ 1]);
         }
       } else {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           if (i > 0) {
             outputs(r, o ^ 1, i == 1);
-            if (r == 1) umma::mma_commit(&sh.op_empty[o ^ 1]);
+            if (r == 1) commit(&sh.op_empty[o ^ 1]);
             wait(&sh.o_done[r], (o_made[r] - 1) & 1);
           }
           scores(r, o);
@@ -272,7 +285,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
       outputs(0, o, n == 1);
       outputs(1, o, n == 1);
     }
-    umma::mma_commit(&sh.op_empty[o]);
+    commit(&sh.op_empty[o]);
   }
 }
 
@@ -289,6 +302,40 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Two f32 operations in one instruction (each rounded as usual).
+__device__ __forceinline__ uint64_t pair_bits(float2 a) { return ((uint64_t)__float_as_uint(a.y) << 32) | __float_as_uint(a.x); }
+__device__ __forceinline__ float2 pair_of(uint64_t v) {
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)), "l"(pair_bits(c)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(pair_bits(a)), "l"(pair_bits(b)));
+  return pair_of(d);
+}
+
+// The largest sum of a tile's weights for which every weight, with a V scale below 2, is an f16.  (At or below the
+// reference weights are at most 2^8 and their sum 2^14.)
+constexpr float kMostSum = 23000.f;
 
 // Operand position -> dimension: K's words hold four consecutive dimensions of a byte row, which lie in two chunks of an
 // operand row.  Even positions keep their neighbour.
@@ -361,7 +408,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32
   const uint32_t tm = sh.tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's 32 lanes of tensor memory
   const uint32_t ts = tm + 64 * r, to = tm + 256 + 128 * r;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum);
+  Walk w(p, a, cum, blockIdx.x);
   Piece x;
   int count = 0;            // key tiles of the CTA
   uint32_t mine = 0;        // key tiles of this warpgroup
@@ -384,83 +431,94 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32
       umma::bounded_wait(&sh.s_full[r], mine & 1, &sh.abort, a.err, kErrKvCopy);
       umma::tc_fence_after();
       float s[kTile];
-      tmem_ld32(ts, reinterpret_cast<uint32_t*>(s));
-      tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(s) + 32);
-      umma::tmem_ld_wait();
+      auto load = [&]() {
+        tmem_ld32(ts, reinterpret_cast<uint32_t*>(s));
+        tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(s) + 32);
+        umma::tmem_ld_wait();
+      };
+      load();
       const bool masked = pos0 + kTile > x.fewest;
       const int seen = masked ? lim - pos0 : kTile;
-      if constexpr (F == kKvF16) {
-#pragma unroll
-        for (int j = 0; j < kTile; ++j) s[j] *= base;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kTile; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(&sh.kf[o][j]);
-          s[j] *= f.x; s[j + 1] *= f.y; s[j + 2] *= f.z; s[j + 3] *= f.w;
-        }
-      }
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < kTile; ++j)
-          if (j >= seen) s[j] = -INFINITY;
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * row_f;
-      float shrink_o = 1.f;
-      if (F != kKvF16 && sh.vtop[o] != vtop) {
-        shrink_o = vtop / sh.vtop[o];
-        vtop = sh.vtop[o];
-      }
-      if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
-        const float t = ceilf(top), c = ex2(m - t);
-        l *= c;
-        shrink_o *= c;
-        m = t;
-      }
-      if (i != first && __any_sync(0xffffffffu, shrink_o != 1.f)) {  // S came after the last products: O is at rest
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t y[32];
-          tmem_ld32(to + 32 * c, y);
-          umma::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
-          umma::tmem_st32(to + 32 * c, y);
-        }
-      }
-      const float off = kLift - (m == -INFINITY ? 0.f : m);
-      float sum[4] = {};
-#pragma unroll
-      for (int j = 0; j < kTile; ++j) {
-        s[j] = ex2(fmaf(s[j], row_f, off));
-        sum[j & 3] += s[j];
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if constexpr (F != kKvF16) {
-#pragma unroll
-        for (int j = 0; j < kTile; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(&sh.vf[o][j]);
-          s[j] *= f.x; s[j + 1] *= f.y; s[j + 2] *= f.z; s[j + 3] *= f.w;
-        }
-        if (masked) {
-#pragma unroll
-          for (int j = 0; j < kTile; ++j)
-            if (j >= seen) s[j] = 0.f;  // whatever the scale there
-        }
-      }
+      // Weights against the reference as it is, and the operand made of them; their sum tells whether one is too large.
+      // No maximum is made then.  (cut: columns from `seen` on get no weight, whatever their scale is.)
       uint32_t pk[32];
+      auto weights = [&](auto cut) {
+        const float off = kLift - (m == -INFINITY ? 0.f : m);
+        float2 sum[2] = {};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const __half2 e = __floats2half2_rn(s[2 * j], s[2 * j + 1]);
-        pk[j] = half2_bits(e);
-        if constexpr (SPLIT_Q) {
-          const float2 z = __half22float2(e);
-          s[2 * j] -= z.x;
-          s[2 * j + 1] -= z.y;
+        for (int j = 0; j < kTile; j += 4) {
+          float4 f = make_float4(base, base, base, base), v = make_float4(1.f, 1.f, 1.f, 1.f);
+          if constexpr (F != kKvF16) {
+            f = *reinterpret_cast<const float4*>(&sh.kf[o][j]);
+            v = *reinterpret_cast<const float4*>(&sh.vf[o][j]);
+          }
+          if constexpr (SPLIT_Q) f = make_float4(f.x * row_f, f.y * row_f, f.z * row_f, f.w * row_f);
+          float2 w[2] = {fma2(make_float2(s[j], s[j + 1]), make_float2(f.x, f.y), make_float2(off, off)),
+                         fma2(make_float2(s[j + 2], s[j + 3]), make_float2(f.z, f.w), make_float2(off, off))};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            w[k] = make_float2(ex2(w[k].x), ex2(w[k].y));
+            if constexpr (cut.value) {
+              if (j + 2 * k >= seen) w[k].x = 0.f;
+              if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
+            }
+            sum[k] = add2(sum[k], w[k]);
+            if constexpr (F != kKvF16) {
+              w[k] = mul2(w[k], k ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
+              if constexpr (cut.value) {
+                if (j + 2 * k >= seen) w[k].x = 0.f;
+                if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
+              }
+            }
+            const __half2 e = __floats2half2_rn(w[k].x, w[k].y);
+            pk[j / 2 + k] = half2_bits(e);
+            if constexpr (SPLIT_Q) {  // what the rounding left
+              const float2 z = __half22float2(e);
+              s[j + 2 * k] = w[k].x - z.x;
+              s[j + 2 * k + 1] = w[k].y - z.y;
+            }
+          }
         }
+        return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      };
+      float sum = 0.f, vtop_now = vtop;
+      if constexpr (F != kKvF16) vtop_now = sh.vtop[o];
+      bool slow = __any_sync(0xffffffffu, masked || m == -INFINITY || vtop_now != vtop);
+      if (!slow) {
+        sum = weights(std::false_type{});
+        slow = __any_sync(0xffffffffu, !(sum <= kMostSum));
+        if (slow) load();  // S is still in tensor memory
       }
+      if (slow) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kTile; ++j) {
+          float f = base;
+          if constexpr (F != kKvF16) f = sh.kf[o][j];
+          if (j < seen) top = fmaxf(top, s[j] * (f * row_f));
+        }
+        float shrink_o = vtop / vtop_now;
+        vtop = vtop_now;
+        if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
+          const float t = ceilf(top), c = ex2(m - t);
+          l *= c;
+          shrink_o *= c;
+          m = t;
+        }
+        if (i != first && __any_sync(0xffffffffu, shrink_o != 1.f)) {  // S came after the last products: O is at rest
+#pragma unroll 1
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t y[16];
+            umma::tmem_ld16(to + 16 * c, y);
+            umma::tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
+            tmem_st16(to + 16 * c, y);
+          }
+        }
+        sum = weights(std::true_type{});
+      }
+      l += sum;
       umma::tmem_st32(ts, pk);
       if constexpr (SPLIT_Q) {
 #pragma unroll
@@ -540,7 +598,7 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
   if (t < Wd::kSoft) wide_softmax<F, HD, kSplitQ, Q>(a, p, cum, sh);
   else if (t < Wd::kSoft + Wd::kConvert) wide_convert<F, HD>(a, p, cum, ops, raw, sh);
   else if (warp == kCopyWarp) wide_copy<F, HD>(a, p, maps, cum, raw, sh);
-  else if ((t & 31) == 0) wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh);
+  else wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh);
   __syncwarp();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&sh.abort) grace();

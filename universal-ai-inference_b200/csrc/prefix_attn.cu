@@ -9,8 +9,8 @@
 //
 // Work.  An item is a tile of query rows that read the same keys: (kv head, rows of the whole batch) over the
 // prefix, (sequence, kv head, rows) over own positions.  Its keys come in units; the units of all items, laid end to
-// end, are dealt out evenly to the CTAs, so a CTA's share starts and ends inside items.  Every piece of an item leaves
-// its unnormalised sums, row maxima and denominators in the workspace (slot = item + CTA, unique because each next
+// end, are dealt out evenly to the workers (CTAs or warps), so a share starts and ends inside items.  Every piece of an item leaves
+// its unnormalised sums, row maxima and denominators in the workspace (slot = item + worker, unique because each next
 // piece raises one of the two), and a last kernel joins the pieces of each row in a fixed order.
 //
 // Two tilings, one kernel each.  Bytes become exact f16 operands (the row scales act on scores and probabilities);
@@ -54,53 +54,98 @@ __global__ void __launch_bounds__(1024) unit_sums_kernel(const __grid_constant__
   if (t == 0) cum[0] = 0;
 }
 
-// out = sum over a row's pieces of 2^(m - M) o / sum of 2^(m - M) l, prefix pieces first.  One warp per row.  px, po:
-// the plans of the kernels that took the prefix and the own items.
-template <int HD, typename Q>
+// Where one row's pieces lie: `n` of them, piece k's row at first + (k / subs) * stride + (k % subs) * sub.
+struct Pieces {
+  const float* part;
+  const float* ml;
+  int64_t first, stride;
+  int n, subs, sub;
+  __device__ int64_t row(int k) const { return first + (subs == 1 ? k : k >> 1) * stride + (subs == 1 ? 0 : (k & 1) * sub); }
+};
+
+// out = sum over a row's pieces of 2^(m - M) o / sum of 2^(m - M) l.  WARPS warps per row; the pieces are taken in the
+// order of the workers, prefix first, a warp every WARPS-th.  px, po: the plans of the kernels that took the prefix and
+// the own items.
+template <int HD, typename Q, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan px,
                                                    const __grid_constant__ Plan po, const int32_t* __restrict__ cum) {
-  constexpr int N = HD / 32;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= a.B * a.T * a.H) return;
-  const int64_t h = row % a.H, bt = row / a.H, b = bt / a.T, t = bt % a.T;
-  const int64_t kvh = h / po.G, g = h % po.G;
+  constexpr int N = HD / 32, kRows = 4 / WARPS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wr = warp % WARPS;
+  const int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS;
+  const bool live = row < a.B * a.T * a.H;
+  const int h = (int)(row % a.H), bt = live ? (int)(row / a.H) : 0, b = bt / (int)a.T, t = bt - b * (int)a.T;
+  const int kvh = h / po.G, g = h - kvh * po.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the pieces are there from here on
-  float mx = -INFINITY, l = 0.f, o[N] = {};
-#pragma unroll 1
-  for (int own = px.prefix_items ? 0 : 1; own < 2; ++own) {
+  Pieces q[2];
+#pragma unroll
+  for (int own = 0; own < 2; ++own) {
     const Plan& p = own ? po : px;
-    const int rho = (int)(own ? t * p.G + g : bt * p.G + g), j = rho / p.rt, in = rho - j * p.rt;
+    q[own].n = 0;
+    if (!live || (!own && px.prefix_items == 0)) continue;
+    const int rho = own ? t * p.G + g : bt * p.G + g, j = rho / p.rt, in = rho - j * p.rt;
     const int per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
     const int total = prefix + (per ? cum[a.B] * per : 0);
     int64_t item;
     int u0, units;
     if (own) {
       units = cum[b + 1] - cum[b];
-      item = p.prefix_items + b * per + kvh * p.own_nrt + j;
-      u0 = prefix + cum[b] * per + ((int)kvh * p.own_nrt + j) * units;
+      item = (int64_t)p.prefix_items + (int64_t)b * per + kvh * p.own_nrt + j;
+      u0 = prefix + cum[b] * per + (kvh * p.own_nrt + j) * units;
     } else {
       units = p.prefix_units;
       item = kvh * p.prefix_nrt + j;
       u0 = (int)item * units;
     }
     if (units == 0) continue;
-    const int first = share_of(u0, total, p.grid), last = share_of(u0 + units - 1, total, p.grid);
-    for (int k = first * p.subs; k < (last + 1) * p.subs; ++k) {
-      const int64_t r = (item + k / p.subs) * p.slot_rows + (k % p.subs) * p.rt + in;
-      const float2 ml = *reinterpret_cast<const float2*>(p.ml + 2 * r);
-      const float* src = p.part + r * HD + N * lane;
-      const float mn = fmaxf(mx, ml.x), safe = mn == -INFINITY ? 0.f : mn;
-      const float fo = ex2(mx - safe), fn = ex2(ml.x - safe);
-      mx = mn;
-      l = l * fo + ml.y * fn;
+    const int c0 = share_of(u0, total, p.workers), c1 = share_of(u0 + units - 1, total, p.workers);
+    q[own] = Pieces{p.part, p.ml, (item + c0) * p.slot_rows + in, p.slot_rows, (c1 - c0 + 1) * p.subs, p.subs, p.rt};
+  }
+  // the row's reference, a piece a lane
+  const int n = q[0].n + q[1].n;
+  float mx = -INFINITY;
+  for (int k = lane; k < n; k += 32) {
+    const Pieces& s = k < q[0].n ? q[0] : q[1];
+    mx = fmaxf(mx, s.ml[2 * s.row(k < q[0].n ? k : k - q[0].n)]);
+  }
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = o[i] * fo + src[i] * fn;
+  for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+  const float safe = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f, o[N] = {};
+#pragma unroll 4
+  for (int k = wr; k < n; k += WARPS) {
+    const Pieces& s = k < q[0].n ? q[0] : q[1];
+    const int64_t r = s.row(k < q[0].n ? k : k - q[0].n);
+    const float2 ml = *reinterpret_cast<const float2*>(s.ml + 2 * r);
+    float y[N];
+    if constexpr (N == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(s.part + r * HD + N * lane);
+    else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(s.part + r * HD + N * lane);
+    const float f = ex2(ml.x - safe);
+    l = fmaf(f, ml.y, l);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = fmaf(f, y[i], o[i]);
+  }
+  if constexpr (WARPS > 1) {
+    __shared__ float all[WARPS][HD + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) all[wr][N * lane + i] = o[i];
+    if (lane == 0) all[wr][HD] = l;
+    __syncthreads();
+    if (wr != 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) {
+      l += all[w][HD];
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] += all[w][N * lane + i];
     }
   }
-  Q* out = static_cast<Q*>(a.out) + row * HD + N * lane;
+  if (!live) return;
+  Q y[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) out[i] = (Q)(l == 0.f ? 0.f : __fdiv_rn(o[i], l));
+  for (int i = 0; i < N; ++i) y[i] = (Q)(l == 0.f ? 0.f : __fdiv_rn(o[i], l));
+  Q* out = static_cast<Q*>(a.out) + row * HD + N * lane;
+  if constexpr (sizeof(y) == 16) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
+  else if constexpr (sizeof(y) == 8) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
+  else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
 }
 
 // ---------------------------------------------------------------- host side
@@ -166,7 +211,7 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     p.rt = w ? (p.split_keys ? 128 : 256) : a.half && rows > 8 ? 16 : 8;
     p.slot_rows = w ? 256 : p.rt;
     p.subs = p.split_keys ? 2 : 1;
-    p.unit = w ? kTile : kWarps * narrow_keys(a);
+    p.unit = w ? kTile : narrow_keys(a);
     p.own_nrt = own ? (own_rows + p.rt - 1) / p.rt : 0;
     p.prefix_nrt = prefix ? (prefix_rows + p.rt - 1) / p.rt : 0;
     p.prefix_units = prefix ? (int)((a.prefix_len + p.unit - 1) / p.unit) : 0;
@@ -174,10 +219,11 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     const int64_t own_items = a.B * a.own.heads * p.own_nrt;
     const int64_t most = (int64_t)p.prefix_items * p.prefix_units + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
     l.most = most > l.most ? most : l.most;
-    const int full = kSms * (w ? 1 : kNarrowCtas);
-    p.grid = (int)(most < full ? most : full);
+    const int each = w ? 1 : kWarps, full = kSms * (w ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
+    p.grid = (int)(most < full * each ? (most + each - 1) / each : full);
+    p.workers = p.grid * each;
     if (p.grid == 0) continue;
-    const int64_t slot_rows = (p.prefix_items + own_items + p.grid) * p.slot_rows;
+    const int64_t slot_rows = (p.prefix_items + own_items + p.workers) * p.slot_rows;
     p.part = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * a.own.hd));
     p.ml = reinterpret_cast<float*>(ws + used);
@@ -220,8 +266,11 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
                                        : run(narrow_attn_kernel<F, HD, true, __half>, smem, threads, a, p, maps, given, cum, st);
     if (e != cudaSuccess) return e;
   }
+  // four warps a row where the rows alone would leave most of the GPU idle
+  const int64_t rows = a.B * a.T * a.H;
+  const bool few = rows <= 4 * kSms;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((a.B * a.T * a.H + 3) / 4));
+  cfg.gridDim = dim3((unsigned)(few ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute early{};
@@ -230,8 +279,9 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
   cfg.attrs = &early;
   cfg.numAttrs = 1;
   const int32_t* sums = cum;
-  return a.half ? cudaLaunchKernelEx(&cfg, join_kernel<HD, __half>, a, l.of_prefix(), l.of_own(), sums)
-                : cudaLaunchKernelEx(&cfg, join_kernel<HD, float>, a, l.of_prefix(), l.of_own(), sums);
+  if (a.half)
+    return cudaLaunchKernelEx(&cfg, few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>, a, l.of_prefix(), l.of_own(), sums);
+  return cudaLaunchKernelEx(&cfg, few ? join_kernel<HD, float, 4> : join_kernel<HD, float, 1>, a, l.of_prefix(), l.of_own(), sums);
 }
 
 template <int F>
