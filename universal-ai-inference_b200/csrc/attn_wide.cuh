@@ -25,21 +25,23 @@ struct Wide {
   static constexpr int kRaw = 2 * Tl::kBytes;                       // K, then V
   static constexpr int kRawStages = kRaw > 16384 ? 2 : 3;
   static constexpr int kOpK = kTile * HD * 2, kOp = 2 * kOpK;       // K as [HD / 64][64 keys][128 B], V as [HD][128 B]
-  static constexpr int kSmem = 2 * kOp + kRawStages * kRaw + 1024;
+  static constexpr int kOps = 4;                                    // operand stages
+  static constexpr int kSmem = kOps * kOp + kRawStages * kRaw + 1024;
   static constexpr int kSoft = 256, kConvert = 128, kThreads = kSoft + kConvert + 64;
 };
 
 template <int F, int HD>
 struct WideShared {
   static constexpr int kRawStages = Wide<F, HD>::kRawStages;
-  uint64_t raw_full[kRawStages], raw_empty[kRawStages], op_full[2], op_empty[2];
+  static constexpr int kOps = Wide<F, HD>::kOps;
+  uint64_t raw_full[kRawStages], raw_empty[kRawStages], op_full[kOps], op_empty[kOps];
   uint64_t q_full, s_full[2], p_full[2], o_done[2];
   uint32_t tmem;
   int abort;
   alignas(16) float raw_scale[kRawStages][2][kTile];
-  alignas(16) float kf[2][kTile];   // K scale * softmax scale * log2(e)
-  alignas(16) float vf[2][kTile];   // V scale * 2 / vtop: below 2
-  float vtop[2];
+  alignas(16) float kf[kOps][kTile];   // K scale * softmax scale * log2(e)
+  alignas(16) float vf[kOps][kTile];   // V scale * 2 / vtop: below 2
+  float vtop[kOps];
   int32_t cum[kMaxScan + 1];
 };
 
@@ -112,9 +114,9 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32
   while (w.next(x, p, a, cum)) {
     float vtop = 0x1p-100f;
     for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
-      const int s = count % Wd::kRawStages, o = count & 1, left = x.limit - (x.t0 + i) * kTile;
+      const int s = count % Wd::kRawStages, o = count % Wd::kOps, left = x.limit - (x.t0 + i) * kTile;
       umma::bounded_wait(&sh.raw_full[s], (count / Wd::kRawStages) & 1, &sh.abort, a.err, kErrKvCopy);
-      umma::bounded_wait(&sh.op_empty[o], ((count >> 1) & 1) ^ 1, &sh.abort, a.err, kErrKvCopy);
+      umma::bounded_wait(&sh.op_empty[o], ((count / Wd::kOps) & 1) ^ 1, &sh.abort, a.err, kErrKvCopy);
       const uint32_t rk = umma::smem_u32(raw + s * Wd::kRaw), rv = rk + Tl::kBytes;
       const uint32_t ok = umma::smem_u32(ops + o * Wd::kOp), ov = ok + Wd::kOpK;
       // K: 16-byte chunk c of an operand row holds positions 8 c ... of the MMA's K axis; chunks of 64 dimensions apart
@@ -256,29 +258,29 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
     if (n <= 0) continue;
     wait(&sh.q_full, pieces++ & 1);
     for (int i = 0; i < n; ++i, ++count) {
-      const int o = count & 1;
-      wait(&sh.op_full[o], (count >> 1) & 1);
+      const int o = count % Wd::kOps, before = (count + Wd::kOps - 1) % Wd::kOps;
+      wait(&sh.op_full[o], (count / Wd::kOps) & 1);
       if (p.split_keys) {
         const int r = i & 1;
         if (i >= 2) wait(&sh.o_done[r], (o_made[r] - 1) & 1);  // P's place is S's
         scores(r, o);
         if (i >= 1) {
-          outputs(r ^ 1, o ^ 1, i < 3);
-          commit(&sh.op_empty[o ^ 1]);
+          outputs(r ^ 1, before, i < 3);
+          commit(&sh.op_empty[before]);
         }
       } else {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           if (i > 0) {
-            outputs(r, o ^ 1, i == 1);
-            if (r == 1) commit(&sh.op_empty[o ^ 1]);
+            outputs(r, before, i == 1);
+            if (r == 1) commit(&sh.op_empty[before]);
             wait(&sh.o_done[r], (o_made[r] - 1) & 1);
           }
           scores(r, o);
         }
       }
     }
-    const int o = (count - 1) & 1;
+    const int o = (count - 1) % Wd::kOps;
     if (p.split_keys) {
       outputs((n - 1) & 1, o, n < 3);
     } else {
@@ -426,8 +428,8 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32
       if (lane == 0) umma::mbar_arrive(&sh.q_full);
     }
     for (int i = first; i < n; i += step, ++mine) {
-      const int at = count + i, o = at & 1, pos0 = (x.t0 + i) * kTile;
-      umma::bounded_wait(&sh.op_full[o], (at >> 1) & 1, &sh.abort, a.err, kErrKvCopy);  // the column factors
+      const int at = count + i, o = at % Wide<F, HD>::kOps, pos0 = (x.t0 + i) * kTile;
+      umma::bounded_wait(&sh.op_full[o], (at / Wide<F, HD>::kOps) & 1, &sh.abort, a.err, kErrKvCopy);  // the column factors
       umma::bounded_wait(&sh.s_full[r], mine & 1, &sh.abort, a.err, kErrKvCopy);
       umma::tc_fence_after();
       float s[kTile];
@@ -570,7 +572,7 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
   constexpr bool kSplitQ = sizeof(Q) == 4;
   extern __shared__ uint8_t dynamic[];
   uint8_t* ops = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(dynamic) + 1023) & ~uintptr_t(1023));
-  uint8_t* raw = ops + 2 * Wd::kOp;
+  uint8_t* raw = ops + Wd::kOps * Wd::kOp;
   __shared__ WideShared<F, HD> sh;
   const int t = threadIdx.x, warp = t >> 5;
   constexpr int kCopyWarp = (Wd::kSoft + Wd::kConvert) / 32, kProductWarp = kCopyWarp + 1;
@@ -579,9 +581,11 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
       umma::mbar_init(&sh.raw_full[i], F == kKvF16 ? 1 : 33);
       umma::mbar_init(&sh.raw_empty[i], Wd::kConvert / 32);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < Wd::kOps; ++i) {
       umma::mbar_init(&sh.op_full[i], Wd::kConvert / 32);
       umma::mbar_init(&sh.op_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       umma::mbar_init(&sh.s_full[i], 1);
       umma::mbar_init(&sh.p_full[i], 4);
       umma::mbar_init(&sh.o_done[i], 1);
