@@ -8,8 +8,9 @@
 // Per key tile of 64: copied bytes -> (four warps) f16 operands in shared memory, K as [key][dim], V transposed to
 // [dim][key] -> S = Q K^T, Q from tensor memory -> (a thread per row) 2^(S - m), weights packed into the tensor memory
 // that held S -> O += P V, P from tensor memory.  Q and P in tensor memory leave shared memory's bandwidth to K and V:
-// with Q there as well, S alone would read 6 KB per 32 cycles of products.
-// Tensor memory: S and P of tile r at column 64 r, Q at 128 + 64 r, O at 256 + 128 r.
+// with Q there as well, S alone would read 6 KB per 32 cycles of products.  S and P go by halves of 32 keys: while a
+// warpgroup makes one half's weights, the other half's products and the next scores are under way.
+// Tensor memory: S and P of tile r, half h at column 64 r + 32 h, Q at 128 + 64 r, O at 256 + 128 r.
 #pragma once
 
 #include <type_traits>
@@ -27,7 +28,7 @@ struct Wide {
   static constexpr int kOpK = kTile * HD * 2, kOp = 2 * kOpK;       // K as [HD / 64][64 keys][128 B], V as [HD][128 B]
   static constexpr int kOps = 4;                                    // operand stages
   static constexpr int kSmem = kOps * kOp + kRawStages * kRaw + 1024;
-  static constexpr int kSoft = 256, kConvert = 128, kThreads = kSoft + kConvert + 64;
+  static constexpr int kSoft = 256, kConvert = 128, kThreads = kSoft + kConvert + 96;
 };
 
 template <int F, int HD>
@@ -35,7 +36,7 @@ struct WideShared {
   static constexpr int kRawStages = Wide<F, HD>::kRawStages;
   static constexpr int kOps = Wide<F, HD>::kOps;
   uint64_t raw_full[kRawStages], raw_empty[kRawStages], op_full[kOps], op_empty[kOps];
-  uint64_t q_full, s_full[2], p_full[2], o_done[2];
+  uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
   uint32_t tmem;
   int abort;
   alignas(16) float raw_scale[kRawStages][2][kTile];
@@ -207,87 +208,72 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32
 
 // ---------------------------------------------------------------- products
 
+// One warp per row tile r: the scores of a half, then, when its weights are there, O += P V; when those products are
+// done, the half of the next key tile takes P's place.  The whole warp stays together and one lane issues: the descriptors
+// then live in uniform registers.
 template <int F, int HD, bool SPLIT_Q>
-__device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, WideShared<F, HD>& sh) {
+__device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, WideShared<F, HD>& sh,
+                              int r) {
   using Wd = Wide<F, HD>;
-  constexpr uint32_t kIdS = umma::idesc_f16_f32(128, kTile), kIdO = umma::idesc_f16_f32(128, HD);
-  const uint32_t tm = sh.tmem;
+  constexpr uint32_t kIdS = umma::idesc_f16_f32(128, kTile / 2), kIdO = umma::idesc_f16_f32(128, HD);
+  const uint32_t tm = sh.tmem, ts = tm + 64 * r, to = tm + 256 + 128 * r;
+  const uint32_t q = tm + 128 + (p.split_keys ? 0 : 64 * r);
   Walk w(p, a, cum, blockIdx.x);
   Piece x;
   int count = 0, pieces = 0;
-  uint32_t p_seen[2] = {0, 0}, o_made[2] = {0, 0};
+  uint32_t mine = 0;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     umma::bounded_wait(bar, parity, &sh.abort, a.err, kErrKvCopy);
     umma::tc_fence_after();
   };
-  // The whole warp stays together and one lane issues: the descriptors then live in uniform registers.
-  auto commit = [&](uint64_t* bar) {
-    if (umma::elect_one()) umma::mma_commit(bar);
-    __syncwarp();
-  };
-  auto scores = [&](int r, int stage) {  // S_r = Q K^T
-    const uint64_t k = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp));
+  auto operand = [&](int o) { return umma::sw128_desc(umma::smem_u32(ops + o * Wd::kOp)); };
+  auto scores = [&](int o, int h) {  // 32 rows (4 KB) of K; 32 bytes a step, 64 dimensions a swizzled block
+    const uint64_t k = operand(o) + (uint64_t)(h * (32 * 128) >> 4);
     if (umma::elect_one()) {
 #pragma unroll
-    for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part) {
-      const uint32_t q = tm + 128 + (SPLIT_Q ? 64 * part : p.split_keys ? 0 : 64 * r);
+      for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)  // 32 bytes a step, 64 dimensions a swizzled block
-        umma::mma_f16_ts(tm + 64 * r, q + 8 * ks, k + (uint64_t)(((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4), kIdS, part | ks);
-    }
-    umma::mma_commit(&sh.s_full[r]);
-    }
-    __syncwarp();
-  };
-  auto outputs = [&](int r, int stage, bool first) {  // O_r += P V
-    wait(&sh.p_full[r], p_seen[r]++ & 1);
-    const uint64_t v = umma::sw128_desc(umma::smem_u32(ops + stage * Wd::kOp + Wd::kOpK));
-    if (umma::elect_one()) {
-#pragma unroll
-    for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
-#pragma unroll
-      for (int ks = 0; ks < kTile / 16; ++ks)
-        umma::mma_f16_ts(tm + 256 + 128 * r, tm + 64 * r + 32 * part + 8 * ks, v + 2 * ks, kIdO, !first || part || ks);
-    umma::mma_commit(&sh.o_done[r]);
+        for (int ks = 0; ks < HD / 16; ++ks)
+          umma::mma_f16_ts(ts + 32 * h, q + 64 * part + 8 * ks, k + (uint64_t)(((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4),
+                           kIdS, part | ks);
+      umma::mma_commit(&sh.s_full[r][h]);
     }
     __syncwarp();
-    ++o_made[r];
   };
   while (w.next(x, p, a, cum)) {
-    const int n = tiles_of(x);
+    const int n = tiles_of(x), first = p.split_keys ? r : 0, step = p.split_keys ? 2 : 1;
     if (n <= 0) continue;
     wait(&sh.q_full, pieces++ & 1);
-    for (int i = 0; i < n; ++i, ++count) {
-      const int o = count % Wd::kOps, before = (count + Wd::kOps - 1) % Wd::kOps;
-      wait(&sh.op_full[o], (count / Wd::kOps) & 1);
-      if (p.split_keys) {
-        const int r = i & 1;
-        if (i >= 2) wait(&sh.o_done[r], (o_made[r] - 1) & 1);  // P's place is S's
-        scores(r, o);
-        if (i >= 1) {
-          outputs(r ^ 1, before, i < 3);
-          commit(&sh.op_empty[before]);
-        }
-      } else {
+    if (first < n) {
+      const int o = (count + first) % Wd::kOps;
+      wait(&sh.op_full[o], ((count + first) / Wd::kOps) & 1);
+      scores(o, 0);
+      scores(o, 1);
+    }
+    for (int i = first; i < n; i += step, ++mine) {
+      const int o = (count + i) % Wd::kOps, on = (count + i + step) % Wd::kOps;
+      const uint64_t v = operand(o) + (Wd::kOpK >> 4);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          if (i > 0) {
-            outputs(r, before, i == 1);
-            if (r == 1) commit(&sh.op_empty[before]);
-            wait(&sh.o_done[r], (o_made[r] - 1) & 1);
-          }
-          scores(r, o);
+      for (int h = 0; h < 2; ++h) {
+        wait(&sh.p_full[r][h], mine & 1);
+        if (umma::elect_one()) {
+#pragma unroll
+          for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+              umma::mma_f16_ts(to, ts + 32 * h + 16 * part + 8 * ks, v + 2 * (2 * h + ks), kIdO, i != first || h || part || ks);
+          umma::mma_commit(&sh.o_done[r][h]);
+          if (h) umma::mma_commit(&sh.op_empty[o]);
+        }
+        __syncwarp();
+        if (i + step < n) {
+          if (h == 0) wait(&sh.op_full[on], ((count + i + step) / Wd::kOps) & 1);
+          wait(&sh.o_done[r][h], mine & 1);
+          scores(on, h);
         }
       }
     }
-    const int o = (count - 1) % Wd::kOps;
-    if (p.split_keys) {
-      outputs((n - 1) & 1, o, n < 3);
-    } else {
-      outputs(0, o, n == 1);
-      outputs(1, o, n == 1);
-    }
-    commit(&sh.op_empty[o]);
+    count += n;
   }
 }
 
@@ -335,8 +321,10 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return pair_of(d);
 }
 
-// The largest sum of a tile's weights for which every weight, with a V scale below 2, is an f16.  (At or below the
-// reference weights are at most 2^8 and their sum 2^14.)
+constexpr int kHalf = kTile / 2;  // keys of a half
+
+// The largest sum of a half's weights for which every weight, with a V scale below 2, is an f16.  (At or below the
+// reference weights are at most 2^8 and their sum 2^13.)
 constexpr float kMostSum = 23000.f;
 
 // Operand position -> dimension: K's words hold four consecutive dimensions of a byte row, which lie in two chunks of an
@@ -428,116 +416,124 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32
       if (lane == 0) umma::mbar_arrive(&sh.q_full);
     }
     for (int i = first; i < n; i += step, ++mine) {
-      const int at = count + i, o = at % Wide<F, HD>::kOps, pos0 = (x.t0 + i) * kTile;
+      const int at = count + i, o = at % Wide<F, HD>::kOps;
       umma::bounded_wait(&sh.op_full[o], (at / Wide<F, HD>::kOps) & 1, &sh.abort, a.err, kErrKvCopy);  // the column factors
-      umma::bounded_wait(&sh.s_full[r], mine & 1, &sh.abort, a.err, kErrKvCopy);
-      umma::tc_fence_after();
-      float s[kTile];
-      auto load = [&]() {
-        tmem_ld32(ts, reinterpret_cast<uint32_t*>(s));
-        tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(s) + 32);
-        umma::tmem_ld_wait();
-      };
-      load();
-      const bool masked = pos0 + kTile > x.fewest;
-      const int seen = masked ? lim - pos0 : kTile;
-      // Weights against the reference as it is, and the operand made of them; their sum tells whether one is too large.
-      // No maximum is made then.  (cut: columns from `seen` on get no weight, whatever their scale is.)
-      uint32_t pk[32];
-      auto weights = [&](auto cut) {
-        const float off = kLift - (m == -INFINITY ? 0.f : m);
-        float2 sum[2] = {};
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const int pos0 = (x.t0 + i) * kTile + kHalf * h;
+        const uint32_t tsh = ts + kHalf * h;
+        umma::bounded_wait(&sh.s_full[r][h], mine & 1, &sh.abort, a.err, kErrKvCopy);
+        umma::tc_fence_after();
+        float s[kHalf];
+        auto load = [&]() {
+          tmem_ld32(tsh, reinterpret_cast<uint32_t*>(s));
+          umma::tmem_ld_wait();
+        };
+        load();
+        const bool masked = pos0 + kHalf > x.fewest;
+        const int seen = masked ? lim - pos0 : kHalf;
+        const float *kf = &sh.kf[o][kHalf * h], *vf = &sh.vf[o][kHalf * h];
+        // Weights against the reference as it is, and the operand made of them; their sum tells whether one is too
+        // large.  No maximum is made then.  (cut: columns from `seen` on get no weight, whatever their scale is.)
+        uint32_t pk[kHalf / 2];
+        auto weights = [&](auto cut) {
+          const float off = kLift - (m == -INFINITY ? 0.f : m);
+          float2 sum[2] = {};
 #pragma unroll
-        for (int j = 0; j < kTile; j += 4) {
-          float4 f = make_float4(base, base, base, base), v = make_float4(1.f, 1.f, 1.f, 1.f);
-          if constexpr (F != kKvF16) {
-            f = *reinterpret_cast<const float4*>(&sh.kf[o][j]);
-            v = *reinterpret_cast<const float4*>(&sh.vf[o][j]);
-          }
-          if constexpr (SPLIT_Q) f = make_float4(f.x * row_f, f.y * row_f, f.z * row_f, f.w * row_f);
-          float2 w[2] = {fma2(make_float2(s[j], s[j + 1]), make_float2(f.x, f.y), make_float2(off, off)),
-                         fma2(make_float2(s[j + 2], s[j + 3]), make_float2(f.z, f.w), make_float2(off, off))};
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            w[k] = make_float2(ex2(w[k].x), ex2(w[k].y));
-            if constexpr (cut.value) {
-              if (j + 2 * k >= seen) w[k].x = 0.f;
-              if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
-            }
-            sum[k] = add2(sum[k], w[k]);
+          for (int j = 0; j < kHalf; j += 4) {
+            float4 f = make_float4(base, base, base, base), v = make_float4(1.f, 1.f, 1.f, 1.f);
             if constexpr (F != kKvF16) {
-              w[k] = mul2(w[k], k ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
+              f = *reinterpret_cast<const float4*>(kf + j);
+              v = *reinterpret_cast<const float4*>(vf + j);
+            }
+            if constexpr (SPLIT_Q) f = make_float4(f.x * row_f, f.y * row_f, f.z * row_f, f.w * row_f);
+            float2 w[2] = {fma2(make_float2(s[j], s[j + 1]), make_float2(f.x, f.y), make_float2(off, off)),
+                           fma2(make_float2(s[j + 2], s[j + 3]), make_float2(f.z, f.w), make_float2(off, off))};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              w[k] = make_float2(ex2(w[k].x), ex2(w[k].y));
               if constexpr (cut.value) {
                 if (j + 2 * k >= seen) w[k].x = 0.f;
                 if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
               }
-            }
-            const __half2 e = __floats2half2_rn(w[k].x, w[k].y);
-            pk[j / 2 + k] = half2_bits(e);
-            if constexpr (SPLIT_Q) {  // what the rounding left
-              const float2 z = __half22float2(e);
-              s[j + 2 * k] = w[k].x - z.x;
-              s[j + 2 * k + 1] = w[k].y - z.y;
+              sum[k] = add2(sum[k], w[k]);
+              if constexpr (F != kKvF16) {
+                w[k] = mul2(w[k], k ? make_float2(v.z, v.w) : make_float2(v.x, v.y));
+                if constexpr (cut.value) {
+                  if (j + 2 * k >= seen) w[k].x = 0.f;
+                  if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
+                }
+              }
+              const __half2 e = __floats2half2_rn(w[k].x, w[k].y);
+              pk[j / 2 + k] = half2_bits(e);
+              if constexpr (SPLIT_Q) {  // what the rounding left
+                const float2 z = __half22float2(e);
+                s[j + 2 * k] = w[k].x - z.x;
+                s[j + 2 * k + 1] = w[k].y - z.y;
+              }
             }
           }
+          return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        };
+        float sum = 0.f, vtop_now = vtop;
+        if constexpr (F != kKvF16) vtop_now = sh.vtop[o];
+        bool slow = __any_sync(0xffffffffu, masked || m == -INFINITY || vtop_now != vtop);
+        if (!slow) {
+          sum = weights(std::false_type{});
+          slow = __any_sync(0xffffffffu, !(sum <= kMostSum));
+          if (slow) load();  // S is still in tensor memory
         }
-        return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      };
-      float sum = 0.f, vtop_now = vtop;
-      if constexpr (F != kKvF16) vtop_now = sh.vtop[o];
-      bool slow = __any_sync(0xffffffffu, masked || m == -INFINITY || vtop_now != vtop);
-      if (!slow) {
-        sum = weights(std::false_type{});
-        slow = __any_sync(0xffffffffu, !(sum <= kMostSum));
-        if (slow) load();  // S is still in tensor memory
-      }
-      if (slow) {
-        float top = -INFINITY;
+        if (slow) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < kTile; ++j) {
-          float f = base;
-          if constexpr (F != kKvF16) f = sh.kf[o][j];
-          if (j < seen) top = fmaxf(top, s[j] * (f * row_f));
-        }
-        float shrink_o = vtop / vtop_now;
-        vtop = vtop_now;
-        if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
-          const float t = ceilf(top), c = ex2(m - t);
-          l *= c;
-          shrink_o *= c;
-          m = t;
-        }
-        if (i != first && __any_sync(0xffffffffu, shrink_o != 1.f)) {  // S came after the last products: O is at rest
+          for (int j = 0; j < kHalf; ++j) {
+            float f = base;
+            if constexpr (F != kKvF16) f = kf[j];
+            if (j < seen) top = fmaxf(top, s[j] * (f * row_f));
+          }
+          float shrink_o = vtop / vtop_now;
+          vtop = vtop_now;
+          if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
+            const float t = ceilf(top), c = ex2(m - t);
+            l *= c;
+            shrink_o *= c;
+            m = t;
+          }
+          if ((h || i != first) && __any_sync(0xffffffffu, shrink_o != 1.f)) {
+            // the products made so far, up to those of the half before, rest
+            umma::bounded_wait(&sh.o_done[r][h ^ 1], (h ? mine : mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
+            umma::tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < HD / 16; ++c) {
-            uint32_t y[16];
-            umma::tmem_ld16(to + 16 * c, y);
-            umma::tmem_ld_wait();
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t y[16];
+              umma::tmem_ld16(to + 16 * c, y);
+              umma::tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
-            tmem_st16(to + 16 * c, y);
+              for (int j = 0; j < 16; ++j) y[j] = __float_as_uint(__uint_as_float(y[j]) * shrink_o);
+              tmem_st16(to + 16 * c, y);
+            }
           }
+          sum = weights(std::true_type{});
         }
-        sum = weights(std::true_type{});
-      }
-      l += sum;
-      umma::tmem_st32(ts, pk);
-      if constexpr (SPLIT_Q) {
+        l += sum;
+        tmem_st16(tsh, pk);
+        if constexpr (SPLIT_Q) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) pk[j] = half2_bits(__floats2half2_rn(s[2 * j], s[2 * j + 1]));
-        umma::tmem_st32(ts + 32, pk);
+          for (int j = 0; j < kHalf / 2; ++j) pk[j] = half2_bits(__floats2half2_rn(s[2 * j], s[2 * j + 1]));
+          tmem_st16(tsh + kHalf / 2, pk);
+        }
+        umma::tmem_st_wait();
+        umma::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) umma::mbar_arrive(&sh.p_full[r][h]);
       }
-      umma::tmem_st_wait();
-      umma::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) umma::mbar_arrive(&sh.p_full[r]);
     }
     count += n > 0 ? n : 0;
     const int64_t at = x.slot * 256 + 128 * r + row;
     float* part = p.part + at * HD;
     *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m, l);
     if (n > first) {
-      umma::bounded_wait(&sh.o_done[r], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
+      umma::bounded_wait(&sh.o_done[r][1], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
       umma::tc_fence_after();
       const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
 #pragma unroll
@@ -583,12 +579,14 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
     }
     for (int i = 0; i < Wd::kOps; ++i) {
       umma::mbar_init(&sh.op_full[i], Wd::kConvert / 32);
-      umma::mbar_init(&sh.op_empty[i], 1);
+      umma::mbar_init(&sh.op_empty[i], p.split_keys ? 1 : 2);
     }
     for (int i = 0; i < 2; ++i) {
-      umma::mbar_init(&sh.s_full[i], 1);
-      umma::mbar_init(&sh.p_full[i], 4);
-      umma::mbar_init(&sh.o_done[i], 1);
+      for (int h = 0; h < 2; ++h) {
+        umma::mbar_init(&sh.s_full[i][h], 1);
+        umma::mbar_init(&sh.p_full[i][h], 4);
+        umma::mbar_init(&sh.o_done[i][h], 1);
+      }
     }
     umma::mbar_init(&sh.q_full, 8);
     sh.abort = 0;
@@ -602,7 +600,7 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
   if (t < Wd::kSoft) wide_softmax<F, HD, kSplitQ, Q>(a, p, cum, sh);
   else if (t < Wd::kSoft + Wd::kConvert) wide_convert<F, HD>(a, p, cum, ops, raw, sh);
   else if (warp == kCopyWarp) wide_copy<F, HD>(a, p, maps, cum, raw, sh);
-  else wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh);
+  else wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh, warp - kProductWarp);
   __syncwarp();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&sh.abort) grace();
