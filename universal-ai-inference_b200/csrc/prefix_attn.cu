@@ -54,14 +54,45 @@ __global__ void __launch_bounds__(1024) unit_sums_kernel(const __grid_constant__
   if (t == 0) cum[0] = 0;
 }
 
-// Where one row's pieces lie: `n` of them, piece k's row at first + (k / subs) * stride + (k % subs) * sub.
+// Where one row's pieces lie: n of them, piece k's row at `first` + k * stride (+ odd * sub where an item has two parts).
 struct Pieces {
   const float* part;
   const float* ml;
-  int64_t first, stride;
-  int n, subs, sub;
-  __device__ int64_t row(int k) const { return first + (subs == 1 ? k : k >> 1) * stride + (subs == 1 ? 0 : (k & 1) * sub); }
+  int64_t first;
+  int n, stride, odd, sub;
+  __device__ __forceinline__ int64_t row(int k) const { return first + (int64_t)(k >> odd) * stride + (k & odd) * sub; }
 };
+
+template <bool OWN>
+__device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan& p, const int32_t* __restrict__ cum, int b, int rho,
+                                            int kvh) {
+  Pieces q{};
+  if (!OWN && p.prefix_items == 0) return q;
+  const int j = rho / p.rt, per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
+  const int total = prefix + (per ? cum[a.B] * per : 0);
+  int64_t item;
+  int u0, units;
+  if (OWN) {
+    const int before = cum[b];
+    units = cum[b + 1] - before;
+    item = (int64_t)p.prefix_items + (int64_t)b * per + kvh * p.own_nrt + j;
+    u0 = prefix + before * per + (kvh * p.own_nrt + j) * units;
+  } else {
+    units = p.prefix_units;
+    item = kvh * p.prefix_nrt + j;
+    u0 = (int)item * units;
+  }
+  if (units == 0) return q;
+  const int c0 = share_of(u0, total, p.workers), c1 = share_of(u0 + units - 1, total, p.workers);
+  q.part = p.part;
+  q.ml = p.ml;
+  q.first = (item + c0) * p.slot_rows + (rho - j * p.rt);
+  q.n = (c1 - c0 + 1) * p.subs;
+  q.stride = p.slot_rows;
+  q.odd = p.subs - 1;
+  q.sub = p.rt;
+  return q;
+}
 
 // out = sum over a row's pieces of 2^(m - M) o / sum of 2^(m - M) l.  WARPS warps per row; the pieces are taken in the
 // order of the workers, prefix first, a warp every WARPS-th.  px, po: the plans of the kernels that took the prefix and
@@ -71,59 +102,36 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
                                                    const __grid_constant__ Plan po, const int32_t* __restrict__ cum) {
   constexpr int N = HD / 32, kRows = 4 / WARPS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wr = warp % WARPS;
-  const int64_t row = (int64_t)blockIdx.x * kRows + warp / WARPS;
-  const bool live = row < a.B * a.T * a.H;
-  const int h = (int)(row % a.H), bt = live ? (int)(row / a.H) : 0, b = bt / (int)a.T, t = bt - b * (int)a.T;
+  const int rows = (int)(a.B * a.T * a.H), row = (int)blockIdx.x * kRows + warp / WARPS;
+  const bool live = row < rows;
+  const int bt = live ? row / (int)a.H : 0, h = live ? row - bt * (int)a.H : 0, b = bt / (int)a.T, t = bt - b * (int)a.T;
   const int kvh = h / po.G, g = h - kvh * po.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the pieces are there from here on
-  Pieces q[2];
-#pragma unroll
-  for (int own = 0; own < 2; ++own) {
-    const Plan& p = own ? po : px;
-    q[own].n = 0;
-    if (!live || (!own && px.prefix_items == 0)) continue;
-    const int rho = own ? t * p.G + g : bt * p.G + g, j = rho / p.rt, in = rho - j * p.rt;
-    const int per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
-    const int total = prefix + (per ? cum[a.B] * per : 0);
-    int64_t item;
-    int u0, units;
-    if (own) {
-      units = cum[b + 1] - cum[b];
-      item = (int64_t)p.prefix_items + (int64_t)b * per + kvh * p.own_nrt + j;
-      u0 = prefix + cum[b] * per + (kvh * p.own_nrt + j) * units;
-    } else {
-      units = p.prefix_units;
-      item = kvh * p.prefix_nrt + j;
-      u0 = (int)item * units;
-    }
-    if (units == 0) continue;
-    const int c0 = share_of(u0, total, p.workers), c1 = share_of(u0 + units - 1, total, p.workers);
-    q[own] = Pieces{p.part, p.ml, (item + c0) * p.slot_rows + in, p.slot_rows, (c1 - c0 + 1) * p.subs, p.subs, p.rt};
-  }
+  const Pieces qp = pieces_of<false>(a, px, cum, b, bt * po.G + g, kvh), qo = pieces_of<true>(a, po, cum, b, t * po.G + g, kvh);
   // the row's reference, a piece a lane
-  const int n = q[0].n + q[1].n;
   float mx = -INFINITY;
-  for (int k = lane; k < n; k += 32) {
-    const Pieces& s = k < q[0].n ? q[0] : q[1];
-    mx = fmaxf(mx, s.ml[2 * s.row(k < q[0].n ? k : k - q[0].n)]);
-  }
+  for (int k = lane; k < qp.n; k += 32) mx = fmaxf(mx, qp.ml[2 * qp.row(k)]);
+  for (int k = lane; k < qo.n; k += 32) mx = fmaxf(mx, qo.ml[2 * qo.row(k)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
   const float safe = mx == -INFINITY ? 0.f : mx;
   float l = 0.f, o[N] = {};
+  auto add = [&](const Pieces& s) {
 #pragma unroll 4
-  for (int k = wr; k < n; k += WARPS) {
-    const Pieces& s = k < q[0].n ? q[0] : q[1];
-    const int64_t r = s.row(k < q[0].n ? k : k - q[0].n);
-    const float2 ml = *reinterpret_cast<const float2*>(s.ml + 2 * r);
-    float y[N];
-    if constexpr (N == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(s.part + r * HD + N * lane);
-    else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(s.part + r * HD + N * lane);
-    const float f = ex2(ml.x - safe);
-    l = fmaf(f, ml.y, l);
+    for (int k = wr; k < s.n; k += WARPS) {
+      const int64_t r = s.row(k);
+      const float2 ml = *reinterpret_cast<const float2*>(s.ml + 2 * r);
+      float y[N];
+      if constexpr (N == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(s.part + r * HD + N * lane);
+      else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(s.part + r * HD + N * lane);
+      const float f = ex2(ml.x - safe);
+      l = fmaf(f, ml.y, l);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = fmaf(f, y[i], o[i]);
-  }
+      for (int i = 0; i < N; ++i) o[i] = fmaf(f, y[i], o[i]);
+    }
+  };
+  add(qp);
+  add(qo);
   if constexpr (WARPS > 1) {
     __shared__ float all[WARPS][HD + 1];
 #pragma unroll
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
   Q y[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = (Q)(l == 0.f ? 0.f : __fdiv_rn(o[i], l));
-  Q* out = static_cast<Q*>(a.out) + row * HD + N * lane;
+  Q* out = static_cast<Q*>(a.out) + (int64_t)row * HD + N * lane;
   if constexpr (sizeof(y) == 16) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(y);
   else if constexpr (sizeof(y) == 8) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(y);
   else *reinterpret_cast<uint32_t*>(out) = *reinterpret_cast<const uint32_t*>(y);
