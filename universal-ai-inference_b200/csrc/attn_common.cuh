@@ -16,7 +16,7 @@ constexpr int kSms = 148;
 constexpr int kTile = 64;        // wide: keys of a tile
 constexpr int kWarps = 4;        // narrow: warps of a CTA
 constexpr int kNarrowCtas = 3;   // narrow: CTAs per SM (wide: one)
-constexpr int kMaxScan = 1024;   // sequences whose tile counts a CTA sums itself
+constexpr int kMaxScan = 512;    // sequences whose unit counts a CTA sums itself
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^(s - m + 8) (in sums and denominators alike), and m follows the running maximum only when that
 // rises by more than 6: the sums are then seldom rescaled, weights stay below 2^14 (2^15 with V's scale, a fraction
@@ -115,6 +115,64 @@ __device__ __forceinline__ uint32_t piece(uint32_t base, int r, int c) {
   else return base + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
+// The sequences: len[b] cached positions (clamped to the cache), and cum[b] units of one row tile and kv head before
+// sequence b.
+struct Seqs {
+  const int32_t* cum;
+  const int32_t* len;
+};
+struct SeqTables {
+  int32_t cum[kMaxScan + 1], len[kMaxScan], sum[kMaxScan / 32];
+};
+
+__device__ __forceinline__ int units_of(int len, int unit) { return (len + unit - 1) / unit; }
+
+// Inclusive sums of the units of 32 sequences, one a lane.
+__device__ __forceinline__ int scan32(int n) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, n, o);
+    if (lane >= o) n += y;
+  }
+  return n;
+}
+
+// Every CTA makes the tables of up to kMaxScan sequences itself (larger batches: `given`, cum and then len); CTA 0 leaves
+// the sums at `out` for the joining kernel.  For all threads of the CTA.
+__device__ __forceinline__ Seqs sequences(const PrefixAttnArgs& a, const Plan& p, const int32_t* given, SeqTables& t, int32_t* out) {
+  if (given) return Seqs{given, given + a.B + 1};
+  if (p.own_nrt == 0) return Seqs{nullptr, nullptr};
+  const int lane = threadIdx.x & 31, B = (int)a.B;
+  for (int c = threadIdx.x >> 5; 32 * c < B; c += blockDim.x >> 5) {
+    const int b = 32 * c + lane, len = b < B ? own_length(a, b, blockIdx.x == 0) : 0;
+    const int n = scan32(b < B ? units_of(len, p.unit) : 0);
+    if (b < B) {
+      t.len[b] = len;
+      t.cum[b + 1] = n;
+    }
+    if (lane == 31) t.sum[c] = n;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x >> 5; 32 * c < B; c += blockDim.x >> 5) {
+    int before = 0;
+    for (int i = lane; i < c; i += 32) before += t.sum[i];
+    before = __reduce_add_sync(0xffffffffu, before);
+    const int b = 32 * c + lane;
+    if (b < B) {
+      const int n = t.cum[b + 1] + before;
+      t.cum[b + 1] = n;
+      if (blockIdx.x == 0) out[b + 1] = n;
+    }
+  }
+  if (threadIdx.x == 0) {
+    t.cum[0] = 0;
+    if (blockIdx.x == 0) out[0] = 0;
+  }
+  __syncthreads();
+  return Seqs{t.cum, t.len};
+}
+
 // ---------------------------------------------------------------- the walk over a worker's pieces
 
 struct Piece {
@@ -141,9 +199,9 @@ __device__ __forceinline__ int share_of(int u, int total, int n) {
 struct Walk {
   int u, end, b, worker;
   Walk() = default;
-  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const int32_t* cum, int worker_) : b(0), worker(worker_) {
+  __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const Seqs& q, int worker_) : b(0), worker(worker_) {
     const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
-    const int total = prefix + (per ? cum[a.B] * per : 0);
+    const int total = prefix + (per ? q.cum[a.B] * per : 0);
     u = share_start(worker, total, p.workers);
     end = share_start(worker + 1, total, p.workers);
     if (end > prefix) {  // the last sequence whose units start at or before the first own unit
@@ -151,21 +209,21 @@ struct Walk {
       int lo = 0, hi = (int)a.B - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
-        if (cum[mid] * per <= first) lo = mid;
+        if (q.cum[mid] * per <= first) lo = mid;
         else hi = mid - 1;
       }
       b = lo;
     }
   }
-  __device__ __forceinline__ bool next(Piece& x, const Plan& p, const PrefixAttnArgs& a, const int32_t* cum) {
+  __device__ __forceinline__ bool next(Piece& x, const Plan& p, const PrefixAttnArgs& a, const Seqs& q) {
     if (u >= end) return false;
     const int prefix = p.prefix_items * p.prefix_units;
     int in, units;
     if (u >= prefix) {
       const int per = (int)a.own.heads * p.own_nrt, v = u - prefix;
-      while (cum[b + 1] * per <= v) ++b;
-      units = cum[b + 1] - cum[b];
-      const int rest = v - cum[b] * per, j = rest / units;
+      while (q.cum[b + 1] * per <= v) ++b;
+      units = q.cum[b + 1] - q.cum[b];
+      const int rest = v - q.cum[b] * per, j = rest / units;
       in = rest - j * units;
       x.slot = p.prefix_items + (int64_t)b * per + j;
       x.own = 1;
@@ -174,7 +232,7 @@ struct Walk {
       x.seq = b;
       x.z = b * (int)a.own.heads + x.kvh;
       const int first = x.rt * p.rt / p.G, last = (min((x.rt + 1) * p.rt, p.own_rows) - 1) / p.G;  // tokens
-      const int seen = own_length(a, b, false) - (int)a.T + 1;
+      const int seen = q.len[b] - (int)a.T + 1;
       x.limit = seen + last;
       x.fewest = seen + first;
     } else {
@@ -208,35 +266,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint6
 __device__ __noinline__ void grace() {
   const long long t0 = clock64();
   while (clock64() - t0 < 20000000LL) {}
-}
-
-// The sequences' unit counts, summed: cum[b] units of one row tile and kv head lie before sequence b.  Every CTA sums
-// up to kMaxScan sequences itself; CTA 0 leaves the sums for the joining kernel.
-__device__ const int32_t* unit_sums(const PrefixAttnArgs& a, const Plan& p, const int32_t* given, int32_t* shared,
-                                    int32_t* out) {
-  if (given || p.own_nrt == 0) return given;
-  const int t = threadIdx.x, lane = t & 31;
-  if (t < 32) {
-    int sum = 0;
-    for (int b0 = 0; b0 < (int)a.B; b0 += 32) {
-      const int b = b0 + lane;
-      int n = b < a.B ? (own_length(a, b, blockIdx.x == 0) + p.unit - 1) / p.unit : 0;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, n, o);
-        if (lane >= o) n += y;
-      }
-      if (b < a.B) {
-        shared[b + 1] = sum + n;
-        if (blockIdx.x == 0) out[b + 1] = sum + n;
-      }
-      sum += __shfl_sync(0xffffffffu, n, 31);
-    }
-    if (lane == 0) {
-      shared[0] = 0;
-      if (blockIdx.x == 0) out[0] = 0;
-    }
-  }
-  return shared;
 }
 
 // q row of logical row `row` of an item (null past the end) and the positions it sees.

@@ -333,6 +333,37 @@ __device__ __forceinline__ void zero_v(uint8_t* v, int from, int to, int thread,
 
 // ---------------------------------------------------------------- narrow
 
+// Two or four consecutive elements of a query row as f32 (vec: one load).
+__device__ __forceinline__ void pair_of_row(const float* p, bool vec, float& a, float& b) {
+  if (vec) {
+    const float2 x = *reinterpret_cast<const float2*>(p);
+    a = x.x; b = x.y;
+  } else {
+    a = p[0]; b = p[1];
+  }
+}
+__device__ __forceinline__ void pair_of_row(const __half* p, bool vec, float& a, float& b) {
+  __half2 x;
+  if (vec) x = *reinterpret_cast<const __half2*>(p);
+  else x = __halves2half2(p[0], p[1]);
+  a = __low2float(x); b = __high2float(x);
+}
+__device__ __forceinline__ void four_of_row(const float* p, bool vec, float (&v)[4]) {
+  if (vec) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[i];
+}
+__device__ __forceinline__ void four_of_row(const __half* p, bool vec, float (&v)[4]) {
+  __half h[4];
+  if (vec) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = p[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __half2float(h[i]);
+}
+
 // What a warp copies next: position `key` of piece x, up to `end`.  Kept in shared memory: it is used once a tile.
 struct Ahead {
   Walk w;
@@ -345,13 +376,14 @@ struct NarrowShared {
   uint64_t full[kWarps][Narrow<F, HD>::kStages];
   Ahead ahead[kWarps];
   int abort;
-  int32_t cum[kMaxScan + 1];
+  SeqTables seqs;
 };
 
 template <int F, int HD, bool FOLD, typename Q>
 __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     narrow_attn_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan p, const __grid_constant__ Maps maps,
                        const int32_t* given, int32_t* cum_out) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using N = Narrow<F, HD>;
   using Tl = typename N::Tl;
   constexpr int KEYS = N::kKeys, RT = FOLD ? 8 : 16, kPer = FOLD ? 1 : 2;
@@ -366,13 +398,14 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     sh.abort = 0;
     umma::fence_barrier_init();
   }
-  const int32_t* cum = unit_sums(a, p, given, sh.cum, cum_out);
+  const Seqs cum = sequences(a, p, given, sh.seqs, cum_out);
   __syncthreads();
   uint8_t* tiles = smem + warp * N::kStages * N::kStage;
   float* scales = reinterpret_cast<float*>(smem + kWarps * N::kStages * N::kStage + warp * N::kScales);
   Ahead& ahead = sh.ahead[warp];
+  Walk w(p, a, cum, worker);
   if (lane == 0) {
-    ahead.w = Walk(p, a, cum, worker);
+    ahead.w = w;
     ahead.key = ahead.end = 0;
   }
   __syncwarp();
@@ -421,44 +454,55 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
 
   Rows<F, HD, FOLD, KEYS> st;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum, worker);
   Piece x;
   while (w.next(x, p, a, cum)) {
-    st.clear();
     uint32_t qa[HD / 16][4];
-    const Q* src[2];
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      src[r] = q_row<Q>(a, p, x, g + 8 * r, st.lim[r]);
-      st.f[r] = base;
-    }
-    float shrink = 1.f;
-    if constexpr (FOLD && sizeof(Q) == 4) {
-      uint32_t mx = 0;
-      if (src[0])
+      // this lane's part of query row g + 8 r: elements 2 tq, 2 tq + 1 (+ 8) of every step's K axis, which are
+      // dimensions 4 tq ... of K's words in bytes
+      const Q* src = q_row<Q>(a, p, x, g + 8 * r, st.lim[r]);
+      float v[HD / 16][4] = {};
+      if (src) {
 #pragma unroll
-        for (int d = 0; d < HD / 4; ++d) mx = max(mx, __float_as_uint((float)src[0][4 * d + tq]) & 0x7fffffffu);
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      shrink = row_shrink(mx);
-      st.f[0] = base / shrink;
-    }
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {  // elements 2 tq, 2 tq + 1 (+ 8): dimensions 4 tq ... of K's words in bytes
-        const int d = F == kKvF16 ? 16 * ks + 8 * h + 2 * tq : 16 * ks + 4 * tq + 2 * h;
-#pragma unroll
-        for (int r = 0; r < kPer; ++r) {
-          const float y0 = src[r] ? (float)src[r][d] * shrink : 0.f, y1 = src[r] ? (float)src[r][d + 1] * shrink : 0.f;
-          const __half2 lead = __floats2half2_rn(y0, y1);
-          qa[ks][2 * h + r] = half2_bits(lead);
-          if constexpr (FOLD) {
-            const float2 z = __half22float2(lead);
-            qa[ks][2 * h + 1] = half2_bits(__floats2half2_rn(y0 - z.x, y1 - z.y));
+        for (int ks = 0; ks < HD / 16; ++ks) {
+          if constexpr (F == kKvF16) {
+            pair_of_row(src + 16 * ks + 2 * tq, a.q_vec, v[ks][0], v[ks][1]);
+            pair_of_row(src + 16 * ks + 8 + 2 * tq, a.q_vec, v[ks][2], v[ks][3]);
+          } else {
+            four_of_row(src + 16 * ks + 4 * tq, a.q_vec, v[ks]);
           }
         }
       }
+      st.f[r] = base;
+      if constexpr (FOLD && sizeof(Q) == 4) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = max(mx, __float_as_uint(v[ks][i]) & 0x7fffffffu);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float shrink = row_shrink(mx);
+        st.f[r] = base / shrink;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[ks][i] *= shrink;
+      }
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const __half2 lead = __floats2half2_rn(v[ks][2 * h], v[ks][2 * h + 1]);
+          qa[ks][2 * h + r] = half2_bits(lead);
+          if constexpr (FOLD) {
+            const float2 z = __half22float2(lead);
+            qa[ks][2 * h + 1] = half2_bits(__floats2half2_rn(v[ks][2 * h] - z.x, v[ks][2 * h + 1] - z.y));
+          }
+        }
+    }
+    st.clear();
     const int end = min(x.t1 * KEYS, x.limit);
 #pragma unroll 1
     for (int key = x.t0 * KEYS; key < end; key += KEYS) {
@@ -490,7 +534,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
       if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], st.l[r]);
     }
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // no grid of this call ends before the one it followed
   if (*(volatile int*)&sh.abort) grace();
 }
 

@@ -4,7 +4,7 @@
 // tile's products while the other's exponentials are made.
 //   rows split   the item's 256 rows are the two tiles, and every key tile serves both (f16 queries, many rows)
 //   keys split   the item's 128 rows are both, and each takes every other key tile (f32 queries, whose leading parts and
-//                rests are two operands added into one accumulator; or up to 128 rows)
+//                rests are two operands added into one acseqsulator; or up to 128 rows)
 // Per key tile of 64: copied bytes -> (four warps) f16 operands in shared memory, K as [key][dim], V transposed to
 // [dim][key] -> S = Q K^T, Q from tensor memory -> (a thread per row) 2^(S - m), weights packed into the tensor memory
 // that held S -> O += P V, P from tensor memory.  Q and P in tensor memory leave shared memory's bandwidth to K and V:
@@ -43,7 +43,7 @@ struct WideShared {
   alignas(16) float kf[kOps][kTile];   // K scale * softmax scale * log2(e)
   alignas(16) float vf[kOps][kTile];   // V scale * 2 / vtop: below 2
   float vtop[kOps];
-  int32_t cum[kMaxScan + 1];
+  SeqTables seqs;
 };
 
 __device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -56,15 +56,15 @@ __device__ __forceinline__ int tiles_of(const Piece& x) { return min(x.t1, (x.li
 // ---------------------------------------------------------------- copies
 
 template <int F, int HD>
-__device__ void wide_copy(const PrefixAttnArgs& a, const Plan& p, const Maps& maps, const int32_t* cum, uint8_t* raw,
+__device__ void wide_copy(const PrefixAttnArgs& a, const Plan& p, const Maps& maps, const Seqs& seqs, uint8_t* raw,
                           WideShared<F, HD>& sh) {
   using Wd = Wide<F, HD>;
   using Tl = typename Wd::Tl;
   const int lane = threadIdx.x & 31;
-  Walk w(p, a, cum, blockIdx.x);
+  Walk w(p, a, seqs, blockIdx.x);
   Piece x;
   int count = 0;
-  while (w.next(x, p, a, cum)) {
+  while (w.next(x, p, a, seqs)) {
     const KvCache& c = x.own ? a.own : a.prefix;
     const CUtensorMap *mk = x.own ? &maps.ok : &maps.pk, *mv = x.own ? &maps.ov : &maps.pv;
     for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
@@ -101,7 +101,7 @@ __device__ void wide_copy(const PrefixAttnArgs& a, const Plan& p, const Maps& ma
 // ---------------------------------------------------------------- bytes to operands
 
 template <int F, int HD>
-__device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, uint8_t* raw,
+__device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs& seqs, uint8_t* ops, uint8_t* raw,
                              WideShared<F, HD>& sh) {
   using Wd = Wide<F, HD>;
   using Tl = typename Wd::Tl;
@@ -109,10 +109,10 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32
   const int lane = threadIdx.x & 31, cw = ((int)threadIdx.x - Wd::kSoft) >> 5;  // keys 16 cw .. 16 cw + 15
   const int mi = lane >> 3, r8 = lane & 7, tq = lane & 3;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum, blockIdx.x);
+  Walk w(p, a, seqs, blockIdx.x);
   Piece x;
   int count = 0;
-  while (w.next(x, p, a, cum)) {
+  while (w.next(x, p, a, seqs)) {
     float vtop = 0x1p-100f;
     for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
       const int s = count % Wd::kRawStages, o = count % Wd::kOps, left = x.limit - (x.t0 + i) * kTile;
@@ -212,13 +212,13 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const int32
 // done, the half of the next key tile takes P's place.  The whole warp stays together and one lane issues: the descriptors
 // then live in uniform registers.
 template <int F, int HD, bool SPLIT_Q>
-__device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, uint8_t* ops, WideShared<F, HD>& sh,
+__device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs& seqs, uint8_t* ops, WideShared<F, HD>& sh,
                               int r) {
   using Wd = Wide<F, HD>;
   constexpr uint32_t kIdS = umma::idesc_f16_f32(128, kTile / 2), kIdO = umma::idesc_f16_f32(128, HD);
   const uint32_t tm = sh.tmem, ts = tm + 64 * r, to = tm + 256 + 128 * r;
   const uint32_t q = tm + 128 + (p.split_keys ? 0 : 64 * r);
-  Walk w(p, a, cum, blockIdx.x);
+  Walk w(p, a, seqs, blockIdx.x);
   Piece x;
   int count = 0, pieces = 0;
   uint32_t mine = 0;
@@ -240,7 +240,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const int3
     }
     __syncwarp();
   };
-  while (w.next(x, p, a, cum)) {
+  while (w.next(x, p, a, seqs)) {
     const int n = tiles_of(x), first = p.split_keys ? r : 0, step = p.split_keys ? 2 : 1;
     if (n <= 0) continue;
     wait(&sh.q_full, pieces++ & 1);
@@ -340,51 +340,49 @@ __device__ __forceinline__ int operand_dim(int pos) {
 template <int F, int HD, bool SPLIT_Q, typename Q>
 __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_t taddr) {
   float shrink = 1.f;
-  auto load16 = [&](int g, float (&v)[16]) {  // dimensions 16 g ... 16 g + 15
+  constexpr int kVec = 16 / sizeof(Q), kLoads = 64 / kVec;
+  union Block {
+    uint4 u[kLoads];
+    Q e[64];
+  };
+  auto load = [&](int h, Block& v) {  // dimensions 64 h ..., every load under way before the first is used
     if (src == nullptr) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      for (int i = 0; i < kLoads; ++i) v.u[i] = make_uint4(0, 0, 0, 0);
     } else if (vec) {
-      Q e[16];
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(Q); ++i)
-        reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(src + 16 * g)[i];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = (float)e[i];
+      for (int i = 0; i < kLoads; ++i) v.u[i] = reinterpret_cast<const uint4*>(src + 64 * h)[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = (float)src[16 * g + i];
+      for (int i = 0; i < 64; ++i) v.e[i] = src[64 * h + i];
     }
   };
   if constexpr (SPLIT_Q) {
     uint32_t mx = 0;
-#pragma unroll 2
-    for (int g = 0; g < HD / 16; ++g) {
-      float v[16];
-      load16(g, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = max(mx, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int h = 0; h < HD / 64; ++h) {
+      Block v;
+      load(h, v);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) mx = max(mx, __float_as_uint((float)v.e[i]) & 0x7fffffffu);
     }
     shrink = row_shrink(mx);
   }
 #pragma unroll
   for (int h = 0; h < HD / 64; ++h) {
+    Block v;
+    load(h, v);
     uint32_t c[32];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      float v[16];
-      load16(4 * h + g, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int d = operand_dim<F>(2 * j);
-        const float y0 = v[d] * shrink, y1 = v[d + 1] * shrink;
-        __half2 e = __floats2half2_rn(y0, y1);
-        if (SPLIT_Q && part) {
-          const float2 z = __half22float2(e);
-          e = __floats2half2_rn(y0 - z.x, y1 - z.y);
-        }
-        c[8 * g + j] = half2_bits(e);
+    for (int j = 0; j < 32; ++j) {
+      const int d = operand_dim<F>(2 * j);
+      const float y0 = (float)v.e[d] * shrink, y1 = (float)v.e[d + 1] * shrink;
+      __half2 e = __floats2half2_rn(y0, y1);
+      if (SPLIT_Q && part) {
+        const float2 z = __half22float2(e);
+        e = __floats2half2_rn(y0 - z.x, y1 - z.y);
       }
+      c[j] = half2_bits(e);
     }
     umma::tmem_st32(taddr + 32 * h, c);
   }
@@ -393,16 +391,16 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
 }
 
 template <int F, int HD, bool SPLIT_Q, typename Q>
-__device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, WideShared<F, HD>& sh) {
+__device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs& seqs, WideShared<F, HD>& sh) {
   const int lane = threadIdx.x & 31, warp = (int)threadIdx.x >> 5, r = warp >> 2, row = threadIdx.x & 127;
   const uint32_t tm = sh.tmem + ((uint32_t)(32 * (warp & 3)) << 16);  // this warp's 32 lanes of tensor memory
   const uint32_t ts = tm + 64 * r, to = tm + 256 + 128 * r;
   const float base = a.scale * kLog2e;
-  Walk w(p, a, cum, blockIdx.x);
+  Walk w(p, a, seqs, blockIdx.x);
   Piece x;
   int count = 0;            // key tiles of the CTA
   uint32_t mine = 0;        // key tiles of this warpgroup
-  while (w.next(x, p, a, cum)) {
+  while (w.next(x, p, a, seqs)) {
     const int n = tiles_of(x), step = p.split_keys ? 2 : 1, first = p.split_keys ? r : 0;
     int lim;
     const Q* src = q_row<Q>(a, p, x, p.split_keys ? row : 128 * r + row, lim);
@@ -564,6 +562,7 @@ template <int F, int HD, typename Q>
 __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
     wide_attn_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan p, const __grid_constant__ Maps maps,
                      const int32_t* given, int32_t* cum_out) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // they take the SMs over as this grid leaves them
   using Wd = Wide<F, HD>;
   constexpr bool kSplitQ = sizeof(Q) == 4;
   extern __shared__ uint8_t dynamic[];
@@ -593,16 +592,15 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
     umma::fence_barrier_init();
   }
   if (warp == kProductWarp) umma::tmem_alloc(&sh.tmem, 512);
-  const int32_t* cum = unit_sums(a, p, given, sh.cum, cum_out);
+  const Seqs seqs = sequences(a, p, given, sh.seqs, cum_out);
   umma::tc_fence_before();
   __syncthreads();
   umma::tc_fence_after();
-  if (t < Wd::kSoft) wide_softmax<F, HD, kSplitQ, Q>(a, p, cum, sh);
-  else if (t < Wd::kSoft + Wd::kConvert) wide_convert<F, HD>(a, p, cum, ops, raw, sh);
-  else if (warp == kCopyWarp) wide_copy<F, HD>(a, p, maps, cum, raw, sh);
-  else wide_products<F, HD, kSplitQ>(a, p, cum, ops, sh, warp - kProductWarp);
+  if (t < Wd::kSoft) wide_softmax<F, HD, kSplitQ, Q>(a, p, seqs, sh);
+  else if (t < Wd::kSoft + Wd::kConvert) wide_convert<F, HD>(a, p, seqs, ops, raw, sh);
+  else if (warp == kCopyWarp) wide_copy<F, HD>(a, p, maps, seqs, raw, sh);
+  else wide_products<F, HD, kSplitQ>(a, p, seqs, ops, sh, warp - kProductWarp);
   __syncwarp();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (*(volatile int*)&sh.abort) grace();
   umma::tc_fence_before();
   __syncthreads();

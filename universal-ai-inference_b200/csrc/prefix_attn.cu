@@ -28,27 +28,22 @@ namespace uaii_b200 {
 namespace attn {
 namespace {
 
-// Units of the sequences before each, for batches too large for a CTA's shared memory.
-__global__ void __launch_bounds__(1024) unit_sums_kernel(const __grid_constant__ PrefixAttnArgs a, int unit, int32_t* cum) {
+// The tables of batches too large for a CTA's shared memory: cum [B + 1], then len [B].
+__global__ void __launch_bounds__(1024) sequences_kernel(const __grid_constant__ PrefixAttnArgs a, int unit, int32_t* cum) {
   __shared__ int warp_sum[32];
-  const int t = threadIdx.x, lane = t & 31;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int before = 0;
   for (int64_t b0 = 0; b0 < a.B; b0 += 1024) {
     const int64_t b = b0 + t;
-    int n = b < a.B ? (own_length(a, b, true) + unit - 1) / unit : 0;
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, n, o);
-      if (lane >= o) n += y;
-    }
-    if (lane == 31) warp_sum[t >> 5] = n;
+    const int len = b < a.B ? own_length(a, b, true) : 0, n = scan32(b < a.B ? units_of(len, unit) : 0);
+    if (lane == 31) warp_sum[warp] = n;
     __syncthreads();
-    int all = 0;
-    for (int i = 0; i < 32; ++i) {
-      if (i == (t >> 5)) n += all;
-      all += warp_sum[i];
+    const int s = warp_sum[lane], up_to = __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
+    if (b < a.B) {
+      cum[b + 1] = before + up_to + n;
+      cum[a.B + 1 + b] = len;
     }
-    if (b < a.B) cum[b + 1] = before + n;
-    before += all;
+    before += __reduce_add_sync(0xffffffffu, s);
     __syncthreads();
   }
   if (t == 0) cum[0] = 0;
@@ -191,35 +186,32 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 int narrow_keys(const PrefixAttnArgs& a) { return a.own.fmt == kKvF16 && a.own.hd == 128 ? 16 : 32; }
 
-// Which kernel takes the prefix and which the own items, their plans, and the workspace.
+// The grids of a call and the workspace.  Own items of more than 16 rows: one wide grid for them and the prefix.  Else a
+// grid for the prefix (wide above 16 rows) and a narrow one for the own items.
 struct Layout {
-  Plan narrow, wide;
+  Plan prefix, own;        // prefix.grid 0: none, or own's grid takes the prefix too
   bool prefix_wide = false, own_wide = false;
   size_t bytes = 0;
-  int64_t most = 0;  // units of either kernel, at most
-  const Plan& of_prefix() const { return prefix_wide ? wide : narrow; }
-  const Plan& of_own() const { return own_wide ? wide : narrow; }
+  int64_t most = 0;        // units of a grid, at most
+  const Plan& of_prefix() const { return prefix.grid ? prefix : own; }
 };
 
 Layout lay_out(const PrefixAttnArgs& a, char* ws) {
   Layout l{};
-  const int G = (int)(a.H / a.own.heads);
-  const int own_rows = (int)(a.T * G), prefix_rows = (int)(a.B * own_rows);
+  const int G = (int)(a.H / a.own.heads), own_rows = (int)(a.T * G), prefix_rows = (int)(a.B * own_rows);
   l.own_wide = own_rows > 16;
-  l.prefix_wide = a.prefix_len && prefix_rows > 16;
-  size_t used = up256(sizeof(int32_t) * (size_t)(a.B + 1));
-  for (int w = 0; w < 2; ++w) {
-    Plan& p = w ? l.wide : l.narrow;
-    const bool prefix = a.prefix_len && l.prefix_wide == (w != 0), own = l.own_wide == (w != 0);
+  l.prefix_wide = prefix_rows > 16;
+  size_t used = up256(sizeof(int32_t) * (size_t)(2 * a.B + 1));
+  auto plan = [&](Plan& p, bool wide, bool prefix, bool own) {
+    const int rows = prefix ? prefix_rows : own_rows;
     p.G = G;
     p.own_rows = own_rows;
     p.prefix_rows = prefix_rows;
-    const int rows = prefix ? prefix_rows : own_rows;
-    p.split_keys = w && (!a.half || rows <= 128);
-    p.rt = w ? (p.split_keys ? 128 : 256) : a.half && rows > 8 ? 16 : 8;
-    p.slot_rows = w ? 256 : p.rt;
+    p.split_keys = wide && (!a.half || rows <= 128);
+    p.rt = wide ? (p.split_keys ? 128 : 256) : a.half && rows > 8 ? 16 : 8;
+    p.slot_rows = wide ? 256 : p.rt;
     p.subs = p.split_keys ? 2 : 1;
-    p.unit = w ? kTile : narrow_keys(a);
+    p.unit = wide ? kTile : narrow_keys(a);
     p.own_nrt = own ? (own_rows + p.rt - 1) / p.rt : 0;
     p.prefix_nrt = prefix ? (prefix_rows + p.rt - 1) / p.rt : 0;
     p.prefix_units = prefix ? (int)((a.prefix_len + p.unit - 1) / p.unit) : 0;
@@ -227,27 +219,23 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     const int64_t own_items = a.B * a.own.heads * p.own_nrt;
     const int64_t most = (int64_t)p.prefix_items * p.prefix_units + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
     l.most = most > l.most ? most : l.most;
-    const int each = w ? 1 : kWarps, full = kSms * (w ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
+    const int each = wide ? 1 : kWarps, full = kSms * (wide ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
     p.grid = (int)(most < full * each ? (most + each - 1) / each : full);
     p.workers = p.grid * each;
-    if (p.grid == 0) continue;
     const int64_t slot_rows = (p.prefix_items + own_items + p.workers) * p.slot_rows;
     p.part = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * a.own.hd));
     p.ml = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * 2));
+  };
+  if (l.own_wide) {
+    plan(l.own, true, a.prefix_len > 0, true);
+  } else {
+    if (a.prefix_len) plan(l.prefix, l.prefix_wide, true, false);
+    plan(l.own, false, false, true);
   }
   l.bytes = used;
   return l;
-}
-
-template <typename K>
-cudaError_t run(K kern, int smem, int threads, const PrefixAttnArgs& a, const Plan& p, const Maps& maps, const int32_t* given,
-                int32_t* cum, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  kern<<<(unsigned)p.grid, threads, smem, st>>>(a, p, maps, given, cum);
-  return cudaGetLastError();
 }
 
 bool make_maps(Maps* m, const PrefixAttnArgs& a, int keys) {
@@ -255,41 +243,52 @@ bool make_maps(Maps* m, const PrefixAttnArgs& a, int keys) {
          (!a.prefix_len || (make_map(&m->pk, a.prefix, a.prefix.k, keys) && make_map(&m->pv, a.prefix, a.prefix.v, keys)));
 }
 
+// `early`: launched when the grid before has started; it waits where it needs that one's results.
+template <typename K, typename... Args>
+cudaError_t launch(K kern, unsigned grid, int threads, int smem, bool early, cudaStream_t st, const Args&... args) {
+  if (smem) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 template <int F, int HD>
 cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* given, int32_t* cum, cudaStream_t st) {
   Maps maps;
-  if (l.wide.grid) {
+  auto wide = [&](const Plan& p) -> cudaError_t {
     if (!make_maps(&maps, a, kTile)) return cudaErrorInvalidValue;
-    constexpr int smem = Wide<F, HD>::kSmem, threads = Wide<F, HD>::kThreads;
-    const cudaError_t e = a.half ? run(wide_attn_kernel<F, HD, __half>, smem, threads, a, l.wide, maps, given, cum, st)
-                                 : run(wide_attn_kernel<F, HD, float>, smem, threads, a, l.wide, maps, given, cum, st);
-    if (e != cudaSuccess) return e;
-  }
-  if (l.narrow.grid) {
+    return launch(a.half ? wide_attn_kernel<F, HD, __half> : wide_attn_kernel<F, HD, float>, (unsigned)p.grid, Wide<F, HD>::kThreads,
+                  Wide<F, HD>::kSmem, false, st, a, p, maps, given, cum);
+  };
+  auto narrow = [&](const Plan& p, bool early) -> cudaError_t {
     if (!make_maps(&maps, a, Narrow<F, HD>::kKeys)) return cudaErrorInvalidValue;
-    constexpr int smem = Narrow<F, HD>::kSmem, threads = 32 * kWarps;
-    const Plan& p = l.narrow;
-    const cudaError_t e = !a.half       ? run(narrow_attn_kernel<F, HD, true, float>, smem, threads, a, p, maps, given, cum, st)
-                          : p.rt == 16 ? run(narrow_attn_kernel<F, HD, false, __half>, smem, threads, a, p, maps, given, cum, st)
-                                       : run(narrow_attn_kernel<F, HD, true, __half>, smem, threads, a, p, maps, given, cum, st);
-    if (e != cudaSuccess) return e;
-  }
+    const auto kern = !a.half      ? narrow_attn_kernel<F, HD, true, float>
+                      : p.rt == 16 ? narrow_attn_kernel<F, HD, false, __half>
+                                   : narrow_attn_kernel<F, HD, true, __half>;
+    return launch(kern, (unsigned)p.grid, 32 * kWarps, Narrow<F, HD>::kSmem, early, st, a, p, maps, given, cum);
+  };
+  cudaError_t e = cudaSuccess;
+  if (l.prefix.grid) e = l.prefix_wide ? wide(l.prefix) : narrow(l.prefix, false);
+  if (e == cudaSuccess) e = l.own_wide ? wide(l.own) : narrow(l.own, l.prefix.grid > 0);
+  if (e != cudaSuccess) return e;
   // four warps a row where the rows alone would leave most of the GPU idle
   const int64_t rows = a.B * a.T * a.H;
   const bool few = rows <= 4 * kSms;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(few ? rows : (rows + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = st;
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
+  const auto kern = a.half ? (few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>)
+                           : (few ? join_kernel<HD, float, 4> : join_kernel<HD, float, 1>);
   const int32_t* sums = cum;
-  if (a.half)
-    return cudaLaunchKernelEx(&cfg, few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>, a, l.of_prefix(), l.of_own(), sums);
-  return cudaLaunchKernelEx(&cfg, few ? join_kernel<HD, float, 4> : join_kernel<HD, float, 1>, a, l.of_prefix(), l.of_own(), sums);
+  return launch(kern, (unsigned)(few ? rows : (rows + 3) / 4), 128, 0, true, st, a, l.of_prefix(), l.own, sums);
 }
 
 template <int F>
@@ -308,12 +307,12 @@ cudaError_t launch_prefix_attn(PrefixAttnArgs a, void* ws, int* launches, cudaSt
   a.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.qs.batch % per16 == 0 && a.qs.token % per16 == 0 &&
             a.qs.head % per16 == 0;
   const Layout l = lay_out(a, static_cast<char*>(ws));
-  if (l.most >= (int64_t(1) << 30)) return cudaErrorInvalidValue;  // (a cache of 2^36 positions)
+  if (l.most >= (int64_t(1) << 30)) return cudaErrorInvalidValue;  // (a cache of 2^35 positions)
   int32_t* cum = static_cast<int32_t*>(ws);
   const int32_t* given = nullptr;
-  *launches = 1 + (l.wide.grid > 0) + (l.narrow.grid > 0);
+  *launches = 2 + (l.prefix.grid > 0);
   if (a.B > kMaxScan) {
-    unit_sums_kernel<<<1, 1024, 0, st>>>(a, l.of_own().unit, cum);
+    sequences_kernel<<<1, 1024, 0, st>>>(a, l.own.unit, cum);
     given = cum;
     ++*launches;
   }
