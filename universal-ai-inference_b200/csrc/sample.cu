@@ -7,24 +7,33 @@
 //
 // Masses are whole numbers, w_i = rint(e_i * 2^31), summed in 64 bits: every order of summation gives the same sums,
 // so neither the split over threads nor the order of shared-memory atomics can change the token.  Sampling in index
-// order (not in rank order) draws from the same distribution and needs no sort: the kept set is all logits above a
-// threshold and the first few that equal it, and a radix descent over the logits' ordered bits finds the threshold.
+// order (not in rank order) draws from the same distribution and needs no sort: a weight never falls as its logit
+// rises, so the kept set is all weights above a cut, and of the weights that equal it the first few by logit and index.
+//
+// A cluster of up to eight CTAs holds a row: every logit is read once and its weight kept in shared memory.  The cut is
+// found with one histogram over the weights' leading bits and a ranking of the few weights of one bin; counts, sums and
+// bins of the CTAs meet through distributed shared memory.  A large batch is bound by the exponentials and divisions
+// (about 30 instructions a logit, once each), a single row by the dozen cluster barriers on its way.
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include "serve_kernels.hpp"
 
+namespace cg = cooperative_groups;
+
 namespace uaii_b200 {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kBins = 256;
+constexpr uint32_t kOne = 1u << 31;  // the weight of the largest logit
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const __half* p) { return __half2float(*p); }
 
-// Ordered bits of a logit: larger keys for larger logits, one key for both zeros; a NaN counts as -inf.
+// A NaN counts as -inf, and both zeros are one.
+__device__ __forceinline__ float canonical(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// Ordered bits of a canonical logit: larger keys for larger logits.
 __device__ __forceinline__ uint32_t key_of_logit(float x) {
-  const uint32_t b = __float_as_uint(x != x ? -INFINITY : x + 0.0f);
+  const uint32_t b = __float_as_uint(canonical(x));
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of_key(uint32_t k) {
@@ -33,179 +42,452 @@ __device__ __forceinline__ float logit_of_key(uint32_t k) {
 __device__ __forceinline__ float weight_exp(float x, float m, float heat) {
   return x == m ? 1.0f : expf(__fdiv_rn(__fsub_rn(x, m), heat));
 }
-__device__ __forceinline__ uint64_t weight(float e) { return (uint64_t)__float2ull_rn(__fmul_rn(e, 2147483648.0f)); }
+__device__ __forceinline__ uint32_t weight(float e) { return __float2uint_rn(__fmul_rn(e, 2147483648.0f)); }
 
-struct Cut {
-  uint32_t key;   // kept: keys above it, and the first `ties` indices whose key equals it
-  uint64_t ties;
+// One row's settings.
+struct Setting {
+  bool greedy;
+  float heat, p, least, u;
+  int64_t k;
+};
+__device__ __forceinline__ Setting setting_of(int64_t b, const float* temperature, const int32_t* top_k, const float* top_p,
+                                              const float* min_p, const float* u) {
+  Setting s;
+  const float t = temperature[b];
+  s.greedy = !(t > 0.f);
+  s.heat = s.greedy ? 1.0f : t;
+  s.k = top_k[b];
+  s.p = top_p[b];
+  s.least = min_p[b];
+  s.u = u[b];
+  if (s.greedy || !(s.least <= 1.0f)) s.k = 1;  // the first token alone
+  return s;
+}
+
+__device__ __forceinline__ uint64_t target_of(float u, uint64_t total) {
+  const double w = floor((double)u * (double)total);
+  const uint64_t goal = w > 0.0 ? (uint64_t)w : 0;
+  return goal < total ? goal : total - 1;
+}
+__device__ __forceinline__ uint64_t reach_of(float p, uint64_t mass) {  // at least 1: the first token is always kept
+  const double want = ceil((double)p * (double)mass);
+  return want > 1.0 ? (uint64_t)want : 1;
+}
+
+// ---------------------------------------------------------------- a row in a cluster's shared memory
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048, kList = 1024, kMaxCluster = 8;
+constexpr int kFixed = kBins * 8 + kList * 4;           // dynamic shared memory besides the weights
+constexpr int kMaxSlice = (int)(kSampleMaxVocab / kMaxCluster);  // weights of a CTA
+static_assert(kFixed + 4 * kMaxSlice <= 225 * 1024, "a CTA's shared memory");
+
+// Leading bits of a weight: its exponent and six bits more (monotone; 0 for 0).
+__device__ __forceinline__ int bin_of(uint32_t w) {
+  if (w == 0) return 0;
+  const int e = 31 - __clz(w);
+  return e * 64 + (int)((w << (31 - e)) >> 25 & 63u);
+}
+
+struct Found {        // a cut: weights above `w` are kept, and `need` of those that equal it
+  uint32_t w;
+  uint64_t above;     // count or mass above w
+  uint64_t need, equal;
 };
 
-struct Shared {
-  uint64_t hist[kBins];
-  uint64_t scan[32];
-  uint32_t digit;
+struct RowShared {
+  uint64_t warp[kWarps];
+  uint64_t part[kMaxCluster];     // a number of each CTA
+  uint64_t part2[kMaxCluster];
+  int bin;                        // where the goal falls: the bin, what lies above it, and
   uint64_t above;
+  uint32_t listed;                // the weights of that bin (CTA 0)
+  Found found;
+  uint32_t digit;
+  uint64_t segment[kWarps], ties[kWarps];
 };
 
-__device__ uint64_t block_sum64(uint64_t v, Shared& s) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = v;
-  __syncthreads();
-  uint64_t t = 0;
-  for (int i = 0; i < kThreads / 32; ++i) t += s.scan[i];
-  return t;
-}
+struct Row {
+  cg::cluster_group cluster;
+  RowShared& sh;
+  uint32_t* w;          // this CTA's weights, in index order
+  uint64_t* bins;
+  uint32_t* list;
+  int n;                // weights of this CTA
+  int rank, ctas;
 
-__device__ uint64_t block_exclusive64(uint64_t v, Shared& s) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint64_t inc = v;
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += x;
+  __device__ __forceinline__ uint64_t block_sum(uint64_t v) {
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
+    __syncthreads();
+    uint64_t t = 0;
+    for (int i = 0; i < kWarps; ++i) t += sh.warp[i];
+    return t;
   }
-  __syncthreads();
-  if (lane == 31) s.scan[w] = inc;
-  __syncthreads();
-  uint64_t before = 0;
-  for (int i = 0; i < w; ++i) before += s.scan[i];
-  return before + inc - v;
-}
+  // Publish this CTA's number to every CTA's array (a cluster barrier has to follow).
+  __device__ __forceinline__ void tell(uint64_t* array, uint64_t v) {
+    if ((int)threadIdx.x < ctas) cluster.map_shared_rank(array, threadIdx.x)[rank] = v;
+  }
+  __device__ __forceinline__ uint64_t sum_of(const uint64_t* array) const {
+    uint64_t t = 0;
+    for (int i = 0; i < ctas; ++i) t += array[i];
+    return t;
+  }
 
-// The smallest leading part of the ranking whose size (a count of tokens, or their mass) reaches `goal` > 0: four
-// passes of eight bits, each adding the tokens that share the digits found so far into 256 bins.
-template <bool MASS, typename X>
-__device__ Cut find_cut(const X* row, int64_t V, float m, float heat, uint64_t goal, Shared& s) {
-  uint32_t prefix = 0;
-  uint64_t above = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.hist[i] = 0;
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-      const float x = logit(row + i);
-      const uint32_t k = key_of_logit(x);
-      if (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
-      const uint64_t add = MASS ? weight(weight_exp(logit_of_key(k), m, heat)) : 1;
-      if (add) atomicAdd(reinterpret_cast<unsigned long long*>(&s.hist[(k >> shift) & 255]), (unsigned long long)add);
+  // The cut at which the leading weights reach `goal` (in tokens, or in mass).  `least`: weights below it cannot matter.
+  template <bool MASS>
+  __device__ Found find(uint64_t goal, uint32_t least) {
+    const int t = threadIdx.x;
+    // weights in [lo, hi] are binned: by leading bits at first, then, should a bin hold more than the list does, by
+    // equal parts of its range
+    uint32_t lo = least ? least : 1, hi = kOne;
+    int shift = -1;
+    uint64_t above = 0;
+    for (;;) {
+      auto bin = [&](uint32_t x) { return shift < 0 ? bin_of(x) : (int)((x - lo) >> shift); };
+      for (int i = t; i < kBins; i += kThreads) bins[i] = 0;
+      if (t == 0) sh.listed = 0;
+      __syncthreads();
+      for (int i = t; i < n; i += kThreads) {
+        const uint32_t x = w[i];
+        if (x >= lo && x <= hi)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&bins[bin(x)]), MASS ? (unsigned long long)x : 1ull);
+      }
+      cluster.sync();
+      // each CTA adds up its share of the bins, from the top share (rank 0) down
+      const int share = kBins / ctas, top = kBins - 1 - rank * share;
+      uint64_t sum = 0;
+      constexpr int kPer = kBins / kThreads;  // bins of a thread at most (one CTA)
+      uint64_t mine[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        mine[i] = 0;
+        const int d = t * kPer + i;
+        if (d < share)
+          for (int c = 0; c < ctas; ++c) mine[i] += cluster.map_shared_rank(bins, c)[top - d];
+        sum += mine[i];
+      }
+      uint64_t inc = sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if ((t & 31) >= o) inc += y;
+      }
+      if ((t & 31) == 31) sh.warp[t >> 5] = inc;
+      __syncthreads();
+      uint64_t before = inc - sum, all = 0;
+      for (int i = 0; i < kWarps; ++i) {
+        if (i < (t >> 5)) before += sh.warp[i];
+        all += sh.warp[i];
+      }
+      tell(sh.part, all);
+      cluster.sync();
+      before += above;
+      for (int c = 0; c < rank; ++c) before += sh.part[c];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (before < goal && goal <= before + mine[i]) {
+          for (int c = 0; c < ctas; ++c) {
+            RowShared* to = cluster.map_shared_rank(&sh, c);
+            to->bin = top - (t * kPer + i);
+            to->above = before;
+          }
+        }
+        before += mine[i];
+      }
+      cluster.sync();
+      const int at = sh.bin;
+      above = sh.above;
+      uint32_t from, to;  // the bin's weights
+      if (shift < 0) {
+        const int e = at >> 6;
+        from = e >= 6 ? (uint32_t)(64 + (at & 63)) << (e - 6) : (uint32_t)(64 + (at & 63)) >> (6 - e);
+        to = e >= 6 ? from + ((1u << (e - 6)) - 1) : from;
+      } else {
+        from = lo + ((uint32_t)at << shift);
+        to = from + ((1u << shift) - 1);
+      }
+      from = max(from, lo);
+      to = min(to, hi);
+      // the bin's weights meet in CTA 0, which ranks them
+      RowShared* first = cluster.map_shared_rank(&sh, 0);
+      uint32_t* all_list = cluster.map_shared_rank(list, 0);
+      for (int i = t; i < n; i += kThreads) {
+        const uint32_t x = w[i];
+        if (x >= from && x <= to) {
+          const uint32_t j = atomicAdd(&first->listed, 1u);
+          if (j < kList) all_list[j] = x;
+        }
+      }
+      cluster.sync();
+      const uint32_t listed = first->listed;
+      if (listed <= kList || from == to) {
+        if (rank == 0) {
+          if (from == to) {
+            if (t == 0) sh.found = Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, listed};
+          } else {
+            for (uint32_t i = t; i < listed; i += kThreads) {
+              const uint32_t x = list[i];
+              uint64_t over = above, equal = 0;
+              for (uint32_t j = 0; j < listed; ++j) {
+                const uint32_t y = list[j];
+                over += y > x ? (MASS ? y : 1u) : 0u;
+                equal += y == x;
+              }
+              const uint64_t each = MASS ? x : 1;
+              if (over < goal && goal <= over + equal * each)  // (tokens of the same weight write the same)
+                sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
+            }
+          }
+        }
+        cluster.sync();
+        const Found f = first->found;
+        cluster.sync();
+        return f;
+      }
+      lo = from;
+      hi = to;
+      const int bits = 32 - __clz(to - from);
+      shift = bits > 11 ? bits - 11 : 0;
+      cluster.sync();
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint64_t sum = above;
-      int d = kBins - 1;
-      for (; d > 0 && sum + s.hist[d] < goal; --d) sum += s.hist[d];
-      s.digit = (uint32_t)d;
-      s.above = sum;
-    }
-    __syncthreads();
-    prefix |= s.digit << shift;
-    above = s.above;
   }
-  const uint64_t each = MASS ? weight(weight_exp(logit_of_key(prefix), m, heat)) : 1;
-  return Cut{prefix, each ? (goal - above + each - 1) / each : 1};
-}
+};
 
 template <typename X>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ logits, int64_t V, int64_t ld,
+__global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ logits, int64_t V, int64_t ld, int slice, bool vec,
                                                           const float* __restrict__ temperature,
                                                           const int32_t* __restrict__ top_k,
                                                           const float* __restrict__ top_p,
                                                           const float* __restrict__ min_p, const float* __restrict__ u,
                                                           int32_t* __restrict__ tokens, float* __restrict__ probs,
                                                           int32_t* __restrict__ kept) {
-  __shared__ Shared s;
-  const int64_t b = blockIdx.x;
-  const X* row = logits + b * ld;
+  extern __shared__ uint4 dynamic[];
+  __shared__ RowShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int64_t b = blockIdx.x / ctas, begin = (int64_t)rank * slice;
+  const int n = (int)max(int64_t(0), min((int64_t)slice, V - begin));
+  uint64_t* bins = reinterpret_cast<uint64_t*>(dynamic);
+  uint32_t* list = reinterpret_cast<uint32_t*>(bins + kBins);
+  uint32_t* w = list + kList;
+  Row row{cluster, sh, w, bins, list, n, rank, ctas};
+  const X* x = logits + b * ld + begin;
+  const Setting s = setting_of(b, temperature, top_k, top_p, min_p, u);
+
+  // the logits, read once, and their largest
   uint32_t top = 0;
-  for (int64_t i = threadIdx.x; i < V; i += kThreads) top = max(top, key_of_logit(logit(row + i)));
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) s.scan[threadIdx.x >> 5] = top;
+  constexpr int kVec = 16 / sizeof(X);
+  const int whole = vec ? n / kVec * kVec : 0;
+  for (int i = t * kVec; i < whole; i += kThreads * kVec) {
+    X v[kVec];
+    *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(x + i));
+    float f[kVec];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      f[j] = canonical((float)v[j]);
+      top = max(top, key_of_logit(f[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; j += 4) *reinterpret_cast<float4*>(w + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+  }
+  for (int i = whole + t; i < n; i += kThreads) {
+    const float f = canonical(logit(x + i));
+    top = max(top, key_of_logit(f));
+    w[i] = __float_as_uint(f);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) sh.warp[warp] = top;
   __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) top = max(top, (uint32_t)s.scan[i]);
-  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) top = max(top, (uint32_t)sh.warp[i]);
+  row.tell(sh.part, top);
+  cluster.sync();
+  for (int i = 0; i < ctas; ++i) top = max(top, (uint32_t)sh.part[i]);
   const float m = logit_of_key(top);
-  if (m == -INFINITY) {  // no token has any mass
-    if (threadIdx.x == 0) {
+  if (m == -INFINITY) {  // no token has any mass (the same in every CTA)
+    if (rank == 0 && t == 0) {
       tokens[b] = -1;
       if (probs) probs[b] = 0.f;
       if (kept) kept[b] = 0;
     }
     return;
   }
-  const float heat_in = temperature[b];
-  const bool greedy = !(heat_in > 0.f);
-  const float heat = greedy ? 1.0f : heat_in;
-  const int64_t k = greedy ? 1 : top_k[b];
-  const float p = top_p[b], least = min_p[b];
-  Cut cut{0, 0};
-  bool cut_set = false;
-  if (k > 0 && k < V) {
-    cut = k == 1 ? Cut{top, 1} : find_cut<false>(row, V, m, heat, (uint64_t)k, s);
-    cut_set = true;
+
+  // weights in place of the logits
+  uint64_t mass = 0;
+  uint32_t some = 0;
+  for (int i = t; i < n; i += kThreads) {
+    const float f = __uint_as_float(w[i]);
+    const uint32_t y = f == -INFINITY ? 0 : weight(weight_exp(f, m, s.heat));
+    w[i] = y;
+    mass += y;
+    some += y != 0;
   }
-  if (!(p >= 1.0f) && k != 1) {
-    uint64_t mass = 0;
-    for (int64_t i = threadIdx.x; i < V; i += kThreads) {
-      const uint32_t key = key_of_logit(logit(row + i));
-      if (key > cut.key || !cut_set) mass += weight(weight_exp(logit_of_key(key), m, heat));
+  mass = row.block_sum(mass);
+  some = (uint32_t)row.block_sum(some);
+  row.tell(sh.part2, mass);
+  cluster.sync();
+  row.tell(sh.part, some);
+  mass = row.sum_of(sh.part2);
+  cluster.sync();
+  const uint64_t positive = row.sum_of(sh.part);
+  cluster.sync();  // part and part2 are free again
+
+  // the cut: none (w 0), or weights above cut.w and `need` of the `equal` ones at it
+  Found cut{0, 0, 0, 0};
+  const bool by_count = s.k > 0 && s.k < V;
+  if (s.k == 1) {
+    cut = Found{kOne, 0, 1, 2};  // whether there is another does not matter
+  } else if (by_count && (uint64_t)s.k < positive) {
+    cut = row.find<false>((uint64_t)s.k, 0);
+  }
+  if (!(s.p >= 1.0f) && s.k != 1) {
+    uint64_t z = mass;
+    if (cut.w) {  // the mass of the first k
+      uint64_t v = 0;
+      for (int i = t; i < n; i += kThreads) v += w[i] > cut.w ? w[i] : 0;
+      v = row.block_sum(v);
+      row.tell(sh.part2, v);
+      cluster.sync();
+      z = row.sum_of(sh.part2) + cut.need * cut.w;
+      cluster.sync();
     }
-    mass = block_sum64(mass, s);
-    if (cut_set) mass += cut.ties * weight(weight_exp(logit_of_key(cut.key), m, heat));
-    const double want = ceil((double)p * (double)mass);
-    const uint64_t reach = want > 0.0 ? (uint64_t)want : 0;  // p <= 0 or NaN: the first token alone
-    cut = reach ? find_cut<true>(row, V, m, heat, reach, s) : Cut{top, 1};
-    cut_set = true;
+    const uint64_t goal = reach_of(s.p, z);
+    // Weights below (z - goal) / V add up to less than z - goal: the goal is reached above them.
+    cut = row.find<true>(goal, (uint32_t)max((z - goal) / (uint64_t)V, (uint64_t)cut.w));
   }
-  if (!(least <= 1.0f)) {  // min_p above 1 or NaN: the first token alone
-    cut = Cut{top, 1};
-    cut_set = true;
-  }
-  const float e_tie = cut_set ? weight_exp(logit_of_key(cut.key), m, heat) : 0.f;
-  const uint64_t w_tie = weight(e_tie), tie_max = cut.key == top || e_tie >= least ? cut.ties : 0;
-  // 1 and e: kept above the cut; 2: equals it
-  auto side = [&](uint32_t key, float& e) {
-    if (cut_set && key <= cut.key) return key == cut.key ? 2 : 0;
-    e = weight_exp(logit_of_key(key), m, heat);
-    return e >= least ? 1 : 0;
-  };
-  // kept mass and ties of each thread's run of indices
-  const int64_t run = (V + kThreads - 1) / kThreads, i0 = min(V, run * threadIdx.x), i1 = min(V, i0 + run);
-  uint64_t mass = 0, ties = 0, count = 0;
-  for (int64_t i = i0; i < i1; ++i) {
-    float e = 0.f;
-    const int f = side(key_of_logit(logit(row + i)), e);
-    if (f == 1) {
-      mass += weight(e);
-      ++count;
-    }
-    ties += f == 2;
-  }
-  const uint64_t ties_before = block_exclusive64(ties, s);
-  const uint64_t my_ties = min(ties_before + ties, tie_max) - min(ties_before, tie_max);
-  mass += my_ties * w_tie;
-  count += my_ties;
-  const uint64_t before = block_exclusive64(mass, s);
-  const uint64_t total = block_sum64(mass, s);
-  const uint64_t n_kept = block_sum64(count, s);
-  const double w = floor((double)u[b] * (double)total);
-  uint64_t goal = w > 0.0 ? (uint64_t)w : 0;
-  if (goal >= total) goal = total - 1;
-  if (before <= goal && goal < before + mass) {  // this thread's run holds the token
-    uint64_t sum = before, t = ties_before;
-    for (int64_t i = i0; i < i1; ++i) {
-      float e = 0.f;
-      const int f = side(key_of_logit(logit(row + i)), e);
-      uint64_t add = f == 1 ? weight(e) : 0;
-      if (f == 2) add = t++ < tie_max ? w_tie : 0;
-      sum += add;
-      if (sum > goal) {
-        tokens[b] = (int32_t)i;
-        if (probs) probs[b] = (float)((double)add / (double)total);
-        if (kept) kept[b] = (int32_t)n_kept;
-        break;
+  // of the weights at the cut: those whose logit is above `edge`, and the first `ties` with that logit
+  uint32_t edge = 0;
+  uint64_t ties = 0;
+  const bool partial = cut.w != 0 && cut.need < cut.equal;
+  if (s.k == 1) {  // the first of the largest
+    edge = top;
+    ties = 1;
+  } else if (partial) {  // eight bits of the key at a time, over the logits read again
+    uint64_t need = cut.need;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = t; i < 256; i += kThreads) bins[i] = 0;
+      __syncthreads();
+      for (int i = t; i < n; i += kThreads) {
+        if (w[i] != cut.w) continue;
+        const uint32_t k = key_of_logit(logit(x + i));
+        if (shift < 24 && (k >> (shift + 8)) != (edge >> (shift + 8))) continue;
+        atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(k >> shift) & 255]), 1ull);
       }
+      cluster.sync();
+      if (t < 32) {  // every CTA adds up the same numbers: lane l has digits 255 - 8 l and down
+        uint64_t c[8], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          c[i] = 0;
+          for (int r = 0; r < ctas; ++r) c[i] += cluster.map_shared_rank(bins, r)[255 - 8 * lane - i];
+          sum += c[i];
+        }
+        uint64_t inc = sum;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += y;
+        }
+        uint64_t before = inc - sum;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < need && need <= before + c[i]) {
+            sh.digit = 255 - 8 * lane - i;
+            sh.above = before;
+          }
+          before += c[i];
+        }
+      }
+      cluster.sync();
+      edge |= sh.digit << shift;
+      need -= sh.above;
+    }
+    ties = need;
+  }
+
+  // Kept or not: 1 kept, 2 at the edge (kept if among the first `ties` there), 0 not.  A weight equal to min_p's, which
+  // rounding may have brought there from below, is told by its exponential.
+  const float least = s.k == 1 ? 0.f : s.least;
+  const uint32_t w_least = least > 0.f ? weight(least) : 0;
+  auto side = [&](int i) {
+    const uint32_t y = w[i];
+    if (y < cut.w || y < w_least) return 0;
+    if (least > 0.f && y == w_least && !(weight_exp(canonical(logit(x + i)), m, s.heat) >= least)) return 0;
+    if (y > cut.w || !partial) return 1;
+    const uint32_t k = key_of_logit(logit(x + i));
+    return k > edge ? 1 : k == edge ? 2 : 0;
+  };
+  // masses and ties of each warp's run of indices
+  const int run = (n + kWarps - 1) / kWarps, i0 = min(n, run * warp), i1 = min(n, i0 + run);
+  uint64_t seg_mass = 0;
+  uint32_t seg_ties = 0, seg_count = 0;
+  for (int i = i0 + lane; i < i1; i += 32) {
+    const int f = side(i);
+    seg_mass += f == 1 ? w[i] : 0;
+    seg_count += f == 1;
+    seg_ties += f == 2;
+  }
+  for (int o = 16; o > 0; o >>= 1) seg_mass += __shfl_xor_sync(0xffffffffu, seg_mass, o);
+  seg_ties = __reduce_add_sync(0xffffffffu, seg_ties);
+  seg_count = __reduce_add_sync(0xffffffffu, seg_count);
+  if (lane == 0) {
+    sh.segment[warp] = seg_mass;
+    sh.ties[warp] = seg_ties;
+  }
+  const uint64_t cta_count = row.block_sum(lane == 0 ? seg_count : 0);  // (its barriers also cover segment and ties)
+  uint64_t cta_mass = 0, cta_ties = 0;
+  for (int i = 0; i < kWarps; ++i) {
+    cta_mass += sh.segment[i];
+    cta_ties += sh.ties[i];
+  }
+  row.tell(sh.part, cta_mass);
+  row.tell(sh.part2, cta_ties | cta_count << 32);
+  cluster.sync();
+  uint64_t total = 0, all_count = 0, all_ties = 0, before = 0, ties_before = 0;
+  for (int c = 0; c < ctas; ++c) {
+    const uint64_t more = sh.part2[c] & 0xffffffffu;
+    if (c < rank) ties_before += more;
+    const uint64_t in = min(all_ties + more, ties) - min(all_ties, ties), add = sh.part[c] + in * cut.w;
+    if (c < rank) before += add;
+    total += add;
+    all_ties += more;
+    all_count += (sh.part2[c] >> 32) + in;
+  }
+  const uint64_t goal = target_of(s.u, total);
+  if (rank == 0 && t == 0 && kept) {
+    // tokens without mass count too, where nothing cuts them off
+    uint64_t count = all_count;
+    if (cut.w == 0 && !(least > 0.f)) count = by_count ? min((uint64_t)s.k, (uint64_t)V) : (uint64_t)V;
+    else if (cut.w == 0 && by_count) count = min(count, (uint64_t)s.k);
+    kept[b] = (int32_t)count;
+  }
+  for (int i = 0; i < warp; ++i) {
+    const uint64_t more = sh.ties[i];
+    before += sh.segment[i] + (min(ties_before + more, ties) - min(ties_before, ties)) * cut.w;
+    ties_before += more;
+  }
+  const uint64_t mine = sh.segment[warp] + (min(ties_before + sh.ties[warp], ties) - min(ties_before, ties)) * cut.w;
+  if (before <= goal && goal < before + mine) {  // this warp's run holds the token
+    for (int i = i0; i < i1; i += 32) {
+      const int f = i + lane < i1 ? side(i + lane) : 0;
+      const uint32_t at_edge = __ballot_sync(0xffffffffu, f == 2);
+      const uint64_t my_tie = ties_before + __popc(at_edge & ((1u << lane) - 1));
+      const uint64_t add = f == 1 ? w[i + lane] : f == 2 && my_tie < ties ? cut.w : 0;
+      uint64_t inc = add;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      if (goal >= before + inc - add && goal < before + inc) {
+        tokens[b] = (int32_t)(begin + i + lane);
+        if (probs) probs[b] = (float)((double)add / (double)total);
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+      ties_before += __popc(at_edge);
+      if (before > goal) break;
     }
   }
+  cluster.sync();  // no CTA leaves while another reads its memory
 }
 
 }  // namespace
@@ -213,13 +495,31 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
 cudaError_t launch_sample(const void* logits, bool half, int64_t B, int64_t V, int64_t ld, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tokens,
                           float* probs, int32_t* kept, cudaStream_t st) {
-  if (half)
-    sample_kernel<<<(unsigned)B, kThreads, 0, st>>>(static_cast<const __half*>(logits), V, ld, temperature, top_k,
-                                                    top_p, min_p, u, tokens, probs, kept);
-  else
-    sample_kernel<<<(unsigned)B, kThreads, 0, st>>>(static_cast<const float*>(logits), V, ld, temperature, top_k,
-                                                    top_p, min_p, u, tokens, probs, kept);
-  return cudaGetLastError();
+  const size_t esz = half ? 2 : 4;
+  // CTAs of a row: 4096 logits each where that is enough, eight at most
+  int ctas = 1;
+  while (ctas < kMaxCluster && V > 4096 * (int64_t)ctas) ctas *= 2;
+  const int64_t slice = ((V + ctas - 1) / ctas + 7) / 8 * 8;
+  if (slice > kMaxSlice) return cudaErrorInvalidValue;
+  const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && ld * (int64_t)esz % 16 == 0;
+  const int smem = kFixed + (int)slice * 4;
+  auto run = [&](auto kern, const auto* x) -> cudaError_t {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(B * ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {(unsigned)ctas, 1, 1};
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, x, V, ld, (int)slice, vec, temperature, top_k, top_p, min_p, u, tokens, probs, kept);
+  };
+  return half ? run(sample_kernel<__half>, static_cast<const __half*>(logits))
+              : run(sample_kernel<float>, static_cast<const float*>(logits));
 }
 
 }  // namespace uaii_b200

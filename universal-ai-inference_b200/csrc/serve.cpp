@@ -128,6 +128,8 @@ Error MoeCudaBackend::sample(const void* logits, bool half, int64_t B, int64_t V
                              int32_t* tokens, float* probs, int32_t* kept) {
   std::lock_guard<std::mutex> lk(mu_);
   if (B < 0 || V <= 0 || V >= kMaxCount || B >= kMaxCount) return invalid("sample: batch >= 0 and 0 < vocab < 2^31");
+  if (V > kSampleMaxVocab)
+    return Error::make(ErrorCode::NotImplemented, "sample: vocab above " + std::to_string(kSampleMaxVocab));
   if (ld < V) return invalid("sample: rows overlap (ld < vocab)");
   if (B == 0) return Error::success();
   for (const void* p : {logits, static_cast<const void*>(temperature), static_cast<const void*>(top_k),
