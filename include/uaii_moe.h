@@ -480,7 +480,7 @@ UAII_MOE_API int uaii_moe_prefix_attention(uaii_moe_backend* b, const uaii_moe_k
  * index whose running mass over the kept indices, in index order, exceeds floor(u * mass(kept)); probs[i] =
  * w / mass(kept) and kept[i] = the number of kept tokens (either may be NULL).  A temperature that is not above 0
  * takes the first largest logit.  NaN logits count as -inf; a row without any other gives token -1, probability 0 and
- * kept 0.  vocab up to 409600.  temperature, top_k, top_p, min_p, u: one per row.  Extends the reference's sampler
+ * kept 0.  vocab up to 400000.  temperature, top_k, top_p, min_p, u: one per row.  Extends the reference's sampler
  * (libs/uaii-runtime/src/sampling.cpp:22-128), which draws its own numbers and sorts on the host. */
 UAII_MOE_API int uaii_moe_sample(uaii_moe_backend* b, const void* logits, int dtype, int64_t batch, int64_t vocab,
                                  int64_t ld, const float* temperature, const int32_t* top_k, const float* top_p,

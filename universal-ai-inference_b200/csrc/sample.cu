@@ -39,10 +39,32 @@ __device__ __forceinline__ uint32_t key_of_logit(float x) {
 __device__ __forceinline__ float logit_of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-__device__ __forceinline__ float weight_exp(float x, float m, float heat) {
-  return x == m ? 1.0f : expf(__fdiv_rn(__fsub_rn(x, m), heat));
-}
 __device__ __forceinline__ uint32_t weight(float e) { return __float2uint_rn(__fmul_rn(e, 2147483648.0f)); }
+
+// exp((x - m) / heat), each step rounded once, for x <= m.
+struct Heat {
+  float m, h, r;
+  bool plain;  // h far from the ends of the range
+  // Correctly rounded quotient by a divisor used often, from its correctly rounded reciprocal and fused residuals
+  // (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  Quotients so
+  // small that a residual would round are below the last place of the exponential's argument 0 anyway.
+  __device__ __forceinline__ float quotient(float a, float q) const {
+    q = fmaf(fmaf(-q, h, a), r, q);
+    return fmaf(fmaf(-q, h, a), r, q);
+  }
+  __device__ __forceinline__ float exp_of(float x) const {
+    if (x == m) return 1.0f;
+    const float a = __fsub_rn(x, m);
+    return expf(plain ? quotient(a, __fmul_rn(a, r)) : __fdiv_rn(a, h));
+  }
+  // The weight; 0 without an exponential where that is below 2^-32 (e^-23) by far.
+  __device__ __forceinline__ uint32_t weight_of(float x) const {
+    const float a = __fsub_rn(x, m), q = __fmul_rn(a, r);
+    if (plain && q < -24.0f) return 0;
+    if (x == m) return kOne;
+    return weight(expf(plain ? quotient(a, q) : __fdiv_rn(a, h)));
+  }
+};
 
 // One row's settings.
 struct Setting {
@@ -77,16 +99,16 @@ __device__ __forceinline__ uint64_t reach_of(float p, uint64_t mass) {  // at le
 // ---------------------------------------------------------------- a row in a cluster's shared memory
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = 2048, kList = 1024, kMaxCluster = 8;
-constexpr int kFixed = kBins * 8 + kList * 4;           // dynamic shared memory besides the weights
+constexpr int kBins = kThreads, kList = 1024, kMaxCluster = 8;
+constexpr int kFixed = 3 * kBins * 8 + 3 * kList * 4;            // dynamic shared memory besides the weights
 constexpr int kMaxSlice = (int)(kSampleMaxVocab / kMaxCluster);  // weights of a CTA
 static_assert(kFixed + 4 * kMaxSlice <= 225 * 1024, "a CTA's shared memory");
 
-// Leading bits of a weight: its exponent and six bits more (monotone; 0 for 0).
+// Leading bits of a weight: its exponent and four bits more (monotone; 0 for 0).
 __device__ __forceinline__ int bin_of(uint32_t w) {
   if (w == 0) return 0;
   const int e = 31 - __clz(w);
-  return e * 64 + (int)((w << (31 - e)) >> 25 & 63u);
+  return e * 16 + (int)((w << (31 - e)) >> 27 & 15u);
 }
 
 struct Found {        // a cut: weights above `w` are kept, and `need` of those that equal it
@@ -97,25 +119,32 @@ struct Found {        // a cut: weights above `w` are kept, and `need` of those 
 
 struct RowShared {
   uint64_t warp[kWarps];
-  uint64_t part[kMaxCluster];     // a number of each CTA
-  uint64_t part2[kMaxCluster];
-  int bin;                        // where the goal falls: the bin, what lies above it, and
+  uint64_t part[5][kMaxCluster];  // numbers of each CTA, a row for each purpose
+  int bin;                        // where the goal falls: the bin, and what lies above it
   uint64_t above;
-  uint32_t listed;                // the weights of that bin (CTA 0)
+  uint32_t listed[2];             // weights of that bin
   Found found;
-  uint32_t digit;
   uint64_t segment[kWarps], ties[kWarps];
 };
+enum Purpose { kTop, kMass, kSome, kHead, kTail };
 
+// What the CTAs of a cluster add up is read by each of them for itself, so that one cluster barrier is enough: bins and
+// lists come in two sets, used in turn, and a set is written again only after the barrier of the other's use.
 struct Row {
   cg::cluster_group cluster;
   RowShared& sh;
-  uint32_t* w;          // this CTA's weights, in index order
-  uint64_t* bins;
-  uint32_t* list;
-  int n;                // weights of this CTA
+  uint32_t* w;          // this CTA's weights, in index order; zeros up to a multiple of four
+  uint2* bins;          // [2][kBins]: a bin's sum of low halves and of high halves (32-bit atomics are native)
+  uint64_t* sums;       // [kBins] of all CTAs
+  uint32_t* list;       // [2][kList] of this CTA, and [kList] of all
+  int quads;            // fours of weights of this CTA
   int rank, ctas;
+  int set;
 
+  template <typename F>
+  __device__ __forceinline__ void each4(F&& f) const {  // f(index, weight) in fours, whole CTA
+    for (int q = threadIdx.x; q < quads; q += kThreads) f(4 * q, reinterpret_cast<const uint4*>(w)[q]);
+  }
   __device__ __forceinline__ uint64_t block_sum(uint64_t v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     __syncthreads();
@@ -126,13 +155,63 @@ struct Row {
     return t;
   }
   // Publish this CTA's number to every CTA's array (a cluster barrier has to follow).
-  __device__ __forceinline__ void tell(uint64_t* array, uint64_t v) {
-    if ((int)threadIdx.x < ctas) cluster.map_shared_rank(array, threadIdx.x)[rank] = v;
+  __device__ __forceinline__ void tell(Purpose p, uint64_t v) {
+    if ((int)threadIdx.x < ctas) cluster.map_shared_rank(sh.part[p], threadIdx.x)[rank] = v;
   }
-  __device__ __forceinline__ uint64_t sum_of(const uint64_t* array) const {
+  __device__ __forceinline__ uint64_t sum_of(Purpose p) const {
     uint64_t t = 0;
-    for (int i = 0; i < ctas; ++i) t += array[i];
+    for (int i = 0; i < ctas; ++i) t += sh.part[p][i];
     return t;
+  }
+  __device__ __forceinline__ uint2* next_bins() {
+    set ^= 1;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) bins[set * kBins + i] = make_uint2(0, 0);
+    if (threadIdx.x == 0) sh.listed[set] = 0;
+    __syncthreads();
+    return bins + set * kBins;
+  }
+  // The bin, from the highest down, at which the cluster's bins reach `goal`: sh.bin and sh.above (plus `above`).  Half of
+  // the threads read the even CTAs' bins and half the odd ones', two bins at a time and 512 bytes a warp: scattered reads
+  // of distributed shared memory took 10 us.
+  __device__ __forceinline__ void reach(uint64_t goal, uint64_t above) {
+    const int t = threadIdx.x, at = t & (kBins / 2 - 1), odd = t / (kBins / 2);
+    uint4 y[kMaxCluster / 2];
+#pragma unroll
+    for (int k = 0; k < kMaxCluster / 2; ++k) {
+      y[k] = make_uint4(0, 0, 0, 0);
+      if (2 * k + odd < ctas) y[k] = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins + set * kBins, 2 * k + odd))[at];
+    }
+    uint64_t two[2] = {};
+#pragma unroll
+    for (int k = 0; k < kMaxCluster / 2; ++k) {
+      two[0] += y[k].x + ((uint64_t)y[k].y << 16);
+      two[1] += y[k].z + ((uint64_t)y[k].w << 16);
+    }
+    if (odd) {
+      sums[2 * at] = two[0];
+      sums[2 * at + 1] = two[1];
+    }
+    __syncthreads();
+    if (!odd) {
+      sums[2 * at] += two[0];
+      sums[2 * at + 1] += two[1];
+    }
+    __syncthreads();
+    const uint64_t mine = sums[kBins - 1 - t];
+    uint64_t inc = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((t & 31) >= o) inc += v;
+    }
+    if ((t & 31) == 31) sh.warp[t >> 5] = inc;
+    __syncthreads();
+    uint64_t before = above + inc - mine;
+    for (int i = 0; i < (t >> 5); ++i) before += sh.warp[i];
+    if (before < goal && goal <= before + mine) {
+      sh.bin = kBins - 1 - t;
+      sh.above = before;
+    }
+    __syncthreads();
   }
 
   // The cut at which the leading weights reach `goal` (in tokens, or in mass).  `least`: weights below it cannot matter.
@@ -145,111 +224,88 @@ struct Row {
     int shift = -1;
     uint64_t above = 0;
     for (;;) {
-      auto bin = [&](uint32_t x) { return shift < 0 ? bin_of(x) : (int)((x - lo) >> shift); };
-      for (int i = t; i < kBins; i += kThreads) bins[i] = 0;
-      if (t == 0) sh.listed = 0;
-      __syncthreads();
-      for (int i = t; i < n; i += kThreads) {
-        const uint32_t x = w[i];
-        if (x >= lo && x <= hi)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&bins[bin(x)]), MASS ? (unsigned long long)x : 1ull);
-      }
-      cluster.sync();
-      // each CTA adds up its share of the bins, from the top share (rank 0) down
-      const int share = kBins / ctas, top = kBins - 1 - rank * share;
-      uint64_t sum = 0;
-      constexpr int kPer = kBins / kThreads;  // bins of a thread at most (one CTA)
-      uint64_t mine[kPer];
+      uint2* mine = next_bins();
+      each4([&](int, uint4 v) {
+        if (max(max(v.x, v.y), max(v.z, v.w)) < lo) return;
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        mine[i] = 0;
-        const int d = t * kPer + i;
-        if (d < share)
-          for (int c = 0; c < ctas; ++c) mine[i] += cluster.map_shared_rank(bins, c)[top - d];
-        sum += mine[i];
-      }
-      uint64_t inc = sum;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((t & 31) >= o) inc += y;
-      }
-      if ((t & 31) == 31) sh.warp[t >> 5] = inc;
-      __syncthreads();
-      uint64_t before = inc - sum, all = 0;
-      for (int i = 0; i < kWarps; ++i) {
-        if (i < (t >> 5)) before += sh.warp[i];
-        all += sh.warp[i];
-      }
-      tell(sh.part, all);
-      cluster.sync();
-      before += above;
-      for (int c = 0; c < rank; ++c) before += sh.part[c];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (before < goal && goal <= before + mine[i]) {
-          for (int c = 0; c < ctas; ++c) {
-            RowShared* to = cluster.map_shared_rank(&sh, c);
-            to->bin = top - (t * kPer + i);
-            to->above = before;
+        for (int j = 0; j < 4; ++j)
+          if (x[j] >= lo && x[j] <= hi) {  // (50000 halves of 16 bits add up to less than 2^32)
+            uint2* to = &mine[shift < 0 ? bin_of(x[j]) : (int)((x[j] - lo) >> shift)];
+            atomicAdd(&to->x, MASS ? x[j] & 0xffffu : 1u);
+            if (MASS) atomicAdd(&to->y, x[j] >> 16);
           }
-        }
-        before += mine[i];
-      }
+      });
       cluster.sync();
+      reach(goal, above);
       const int at = sh.bin;
       above = sh.above;
       uint32_t from, to;  // the bin's weights
       if (shift < 0) {
-        const int e = at >> 6;
-        from = e >= 6 ? (uint32_t)(64 + (at & 63)) << (e - 6) : (uint32_t)(64 + (at & 63)) >> (6 - e);
-        to = e >= 6 ? from + ((1u << (e - 6)) - 1) : from;
+        const int e = at >> 4;
+        from = e >= 4 ? (uint32_t)(16 + (at & 15)) << (e - 4) : (uint32_t)(16 + (at & 15)) >> (4 - e);
+        to = e >= 4 ? from + ((1u << (e - 4)) - 1) : from;
       } else {
         from = lo + ((uint32_t)at << shift);
         to = from + ((1u << shift) - 1);
       }
       from = max(from, lo);
       to = min(to, hi);
-      // the bin's weights meet in CTA 0, which ranks them
-      RowShared* first = cluster.map_shared_rank(&sh, 0);
-      uint32_t* all_list = cluster.map_shared_rank(list, 0);
-      for (int i = t; i < n; i += kThreads) {
-        const uint32_t x = w[i];
-        if (x >= from && x <= to) {
-          const uint32_t j = atomicAdd(&first->listed, 1u);
-          if (j < kList) all_list[j] = x;
-        }
-      }
-      cluster.sync();
-      const uint32_t listed = first->listed;
-      if (listed <= kList || from == to) {
-        if (rank == 0) {
-          if (from == to) {
-            if (t == 0) sh.found = Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, listed};
-          } else {
-            for (uint32_t i = t; i < listed; i += kThreads) {
-              const uint32_t x = list[i];
-              uint64_t over = above, equal = 0;
-              for (uint32_t j = 0; j < listed; ++j) {
-                const uint32_t y = list[j];
-                over += y > x ? (MASS ? y : 1u) : 0u;
-                equal += y == x;
-              }
-              const uint64_t each = MASS ? x : 1;
-              if (over < goal && goal <= over + equal * each)  // (tokens of the same weight write the same)
-                sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
-            }
+      // the bin's weights: every CTA lists its own, then reads all lists and ranks them
+      uint32_t* own = list + set * kList;
+      each4([&](int, uint4 v) {
+        if (max(max(v.x, v.y), max(v.z, v.w)) < from) return;
+        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (x[j] >= from && x[j] <= to) {
+            const uint32_t k = atomicAdd(&sh.listed[set], 1u);
+            if (k < kList) own[k] = x[j];
           }
+      });
+      cluster.sync();
+      uint32_t count[kMaxCluster], listed = 0;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) count[c] = c < ctas ? cluster.map_shared_rank(&sh, c)->listed[set] : 0;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) listed += count[c];
+      if (from == to) return Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, listed};
+      if (listed <= kList) {
+        uint32_t* all = list + 2 * kList;
+        for (uint32_t i = t; i < listed; i += kThreads) {
+          uint32_t at_ = i;
+          int c = 0;
+#pragma unroll
+          for (int k = 0; k + 1 < kMaxCluster; ++k)
+            if (c == k && at_ >= count[k]) {
+              at_ -= count[k];
+              c = k + 1;
+            }
+          all[i] = cluster.map_shared_rank(own, c)[at_];
         }
-        cluster.sync();
-        const Found f = first->found;
-        cluster.sync();
+        __syncthreads();
+        for (uint32_t i = t; i < listed; i += kThreads) {
+          const uint32_t x = all[i];
+          uint64_t over = above;
+          uint32_t equal = 0;
+          for (uint32_t j = 0; j < listed; ++j) {
+            const uint32_t y = all[j];
+            over += y > x ? (MASS ? y : 1u) : 0u;
+            equal += y == x;
+          }
+          const uint64_t each = MASS ? x : 1;
+          if (over < goal && goal <= over + equal * each)  // (tokens of the same weight write the same)
+            sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
+        }
+        __syncthreads();
+        const Found f = sh.found;
+        __syncthreads();
         return f;
       }
       lo = from;
       hi = to;
       const int bits = 32 - __clz(to - from);
-      shift = bits > 11 ? bits - 11 : 0;
-      cluster.sync();
+      shift = bits > 9 ? bits - 9 : 0;
     }
   }
 };
@@ -268,10 +324,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t b = blockIdx.x / ctas, begin = (int64_t)rank * slice;
   const int n = (int)max(int64_t(0), min((int64_t)slice, V - begin));
-  uint64_t* bins = reinterpret_cast<uint64_t*>(dynamic);
-  uint32_t* list = reinterpret_cast<uint32_t*>(bins + kBins);
-  uint32_t* w = list + kList;
-  Row row{cluster, sh, w, bins, list, n, rank, ctas};
+  uint2* bins = reinterpret_cast<uint2*>(dynamic);
+  uint64_t* sums = reinterpret_cast<uint64_t*>(bins + 2 * kBins);
+  uint32_t* list = reinterpret_cast<uint32_t*>(sums + kBins);
+  uint32_t* w = list + 3 * kList;
+  Row row{cluster, sh, w, bins, sums, list, (n + 3) / 4, rank, ctas, 0};
   const X* x = logits + b * ld + begin;
   const Setting s = setting_of(b, temperature, top_k, top_p, min_p, u);
 
@@ -296,13 +353,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
     top = max(top, key_of_logit(f));
     w[i] = __float_as_uint(f);
   }
+  if (n + t < 4 * row.quads) w[n + t] = 0xff800000u;  // -inf
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) sh.warp[warp] = top;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) top = max(top, (uint32_t)sh.warp[i]);
-  row.tell(sh.part, top);
+  row.tell(kTop, top);
   cluster.sync();
-  for (int i = 0; i < ctas; ++i) top = max(top, (uint32_t)sh.part[i]);
+  for (int i = 0; i < ctas; ++i) top = max(top, (uint32_t)sh.part[kTop][i]);
   const float m = logit_of_key(top);
   if (m == -INFINITY) {  // no token has any mass (the same in every CTA)
     if (rank == 0 && t == 0) {
@@ -314,24 +372,23 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   }
 
   // weights in place of the logits
+  const Heat heat{m, s.heat, __fdiv_rn(1.0f, s.heat), s.heat >= 0x1p-30f && s.heat <= 0x1p30f};
   uint64_t mass = 0;
   uint32_t some = 0;
-  for (int i = t; i < n; i += kThreads) {
-    const float f = __uint_as_float(w[i]);
-    const uint32_t y = f == -INFINITY ? 0 : weight(weight_exp(f, m, s.heat));
-    w[i] = y;
-    mass += y;
-    some += y != 0;
-  }
+  row.each4([&](int i, uint4 v) {
+    const uint4 y = {heat.weight_of(__uint_as_float(v.x)), heat.weight_of(__uint_as_float(v.y)),
+                     heat.weight_of(__uint_as_float(v.z)), heat.weight_of(__uint_as_float(v.w))};
+    *reinterpret_cast<uint4*>(w + i) = y;
+    mass += ((uint64_t)y.x + y.y) + ((uint64_t)y.z + y.w);
+    some += (y.x != 0) + (y.y != 0) + (y.z != 0) + (y.w != 0);
+  });
   mass = row.block_sum(mass);
   some = (uint32_t)row.block_sum(some);
-  row.tell(sh.part2, mass);
+  row.tell(kMass, mass);
+  row.tell(kSome, some);
   cluster.sync();
-  row.tell(sh.part, some);
-  mass = row.sum_of(sh.part2);
-  cluster.sync();
-  const uint64_t positive = row.sum_of(sh.part);
-  cluster.sync();  // part and part2 are free again
+  mass = row.sum_of(kMass);
+  const uint64_t positive = row.sum_of(kSome);
 
   // the cut: none (w 0), or weights above cut.w and `need` of the `equal` ones at it
   Found cut{0, 0, 0, 0};
@@ -345,12 +402,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
     uint64_t z = mass;
     if (cut.w) {  // the mass of the first k
       uint64_t v = 0;
-      for (int i = t; i < n; i += kThreads) v += w[i] > cut.w ? w[i] : 0;
-      v = row.block_sum(v);
-      row.tell(sh.part2, v);
+      row.each4([&](int, uint4 y) {
+        v += ((uint64_t)(y.x > cut.w ? y.x : 0) + (y.y > cut.w ? y.y : 0)) + ((uint64_t)(y.z > cut.w ? y.z : 0) + (y.w > cut.w ? y.w : 0));
+      });
+      row.tell(kHead, row.block_sum(v));
       cluster.sync();
-      z = row.sum_of(sh.part2) + cut.need * cut.w;
-      cluster.sync();
+      z = row.sum_of(kHead) + cut.need * cut.w;
     }
     const uint64_t goal = reach_of(s.p, z);
     // Weights below (z - goal) / V add up to less than z - goal: the goal is reached above them.
@@ -366,41 +423,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   } else if (partial) {  // eight bits of the key at a time, over the logits read again
     uint64_t need = cut.need;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = t; i < 256; i += kThreads) bins[i] = 0;
-      __syncthreads();
-      for (int i = t; i < n; i += kThreads) {
-        if (w[i] != cut.w) continue;
-        const uint32_t k = key_of_logit(logit(x + i));
-        if (shift < 24 && (k >> (shift + 8)) != (edge >> (shift + 8))) continue;
-        atomicAdd(reinterpret_cast<unsigned long long*>(&bins[(k >> shift) & 255]), 1ull);
-      }
-      cluster.sync();
-      if (t < 32) {  // every CTA adds up the same numbers: lane l has digits 255 - 8 l and down
-        uint64_t c[8], sum = 0;
+      uint2* mine = row.next_bins();
+      row.each4([&](int i, uint4 v) {
+        const uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          c[i] = 0;
-          for (int r = 0; r < ctas; ++r) c[i] += cluster.map_shared_rank(bins, r)[255 - 8 * lane - i];
-          sum += c[i];
+        for (int j = 0; j < 4; ++j) {
+          if (y[j] != cut.w) continue;
+          const uint32_t k = key_of_logit(logit(x + i + j));
+          if (shift == 24 || (k >> (shift + 8)) == (edge >> (shift + 8))) atomicAdd(&mine[(k >> shift) & 255].x, 1u);
         }
-        uint64_t inc = sum;
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += y;
-        }
-        uint64_t before = inc - sum;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (before < need && need <= before + c[i]) {
-            sh.digit = 255 - 8 * lane - i;
-            sh.above = before;
-          }
-          before += c[i];
-        }
-      }
+      });
       cluster.sync();
-      edge |= sh.digit << shift;
+      row.reach(need, 0);
+      edge |= (uint32_t)sh.bin << shift;
       need -= sh.above;
+      __syncthreads();
     }
     ties = need;
   }
@@ -412,20 +449,26 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   auto side = [&](int i) {
     const uint32_t y = w[i];
     if (y < cut.w || y < w_least) return 0;
-    if (least > 0.f && y == w_least && !(weight_exp(canonical(logit(x + i)), m, s.heat) >= least)) return 0;
+    if (least > 0.f && y == w_least && !(heat.exp_of(canonical(logit(x + i))) >= least)) return 0;
     if (y > cut.w || !partial) return 1;
     const uint32_t k = key_of_logit(logit(x + i));
     return k > edge ? 1 : k == edge ? 2 : 0;
   };
-  // masses and ties of each warp's run of indices
-  const int run = (n + kWarps - 1) / kWarps, i0 = min(n, run * warp), i1 = min(n, i0 + run);
+  // masses and ties of each warp's run of indices, four of them a lane
+  const uint32_t low = max(cut.w, w_least);
+  const int run = (row.quads + kWarps - 1) / kWarps, q0 = min(row.quads, run * warp), q1 = min(row.quads, q0 + run);
   uint64_t seg_mass = 0;
   uint32_t seg_ties = 0, seg_count = 0;
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const int f = side(i);
-    seg_mass += f == 1 ? w[i] : 0;
-    seg_count += f == 1;
-    seg_ties += f == 2;
+  for (int q = q0 + lane; q < q1; q += 32) {
+    const uint4 v = reinterpret_cast<const uint4*>(w)[q];
+    if (max(max(v.x, v.y), max(v.z, v.w)) < low) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = 4 * q + j, f = i < n ? side(i) : 0;
+      seg_mass += f == 1 ? w[i] : 0;
+      seg_count += f == 1;
+      seg_ties += f == 2;
+    }
   }
   for (int o = 16; o > 0; o >>= 1) seg_mass += __shfl_xor_sync(0xffffffffu, seg_mass, o);
   seg_ties = __reduce_add_sync(0xffffffffu, seg_ties);
@@ -440,18 +483,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
     cta_mass += sh.segment[i];
     cta_ties += sh.ties[i];
   }
-  row.tell(sh.part, cta_mass);
-  row.tell(sh.part2, cta_ties | cta_count << 32);
+  row.tell(kTail, cta_mass);
+  row.tell(kTop, cta_ties | cta_count << 32);
   cluster.sync();
   uint64_t total = 0, all_count = 0, all_ties = 0, before = 0, ties_before = 0;
   for (int c = 0; c < ctas; ++c) {
-    const uint64_t more = sh.part2[c] & 0xffffffffu;
+    const uint64_t more = sh.part[kTop][c] & 0xffffffffu;
     if (c < rank) ties_before += more;
-    const uint64_t in = min(all_ties + more, ties) - min(all_ties, ties), add = sh.part[c] + in * cut.w;
+    const uint64_t in = min(all_ties + more, ties) - min(all_ties, ties), add = sh.part[kTail][c] + in * cut.w;
     if (c < rank) before += add;
     total += add;
     all_ties += more;
-    all_count += (sh.part2[c] >> 32) + in;
+    all_count += (sh.part[kTop][c] >> 32) + in;
   }
   const uint64_t goal = target_of(s.u, total);
   if (rank == 0 && t == 0 && kept) {
@@ -468,26 +511,48 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   }
   const uint64_t mine = sh.segment[warp] + (min(ties_before + sh.ties[warp], ties) - min(ties_before, ties)) * cut.w;
   if (before <= goal && goal < before + mine) {  // this warp's run holds the token
-    for (int i = i0; i < i1; i += 32) {
-      const int f = i + lane < i1 ? side(i + lane) : 0;
-      const uint32_t at_edge = __ballot_sync(0xffffffffu, f == 2);
-      const uint64_t my_tie = ties_before + __popc(at_edge & ((1u << lane) - 1));
-      const uint64_t add = f == 1 ? w[i + lane] : f == 2 && my_tie < ties ? cut.w : 0;
-      uint64_t inc = add;
+    for (int q = q0; q < q1; q += 32) {
+      uint64_t add[4] = {}, sum = 0;
+      int f[4] = {}, edges = 0;
+      if (q + lane < q1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = 4 * (q + lane) + j;
+          f[j] = i < n ? side(i) : 0;
+          edges += f[j] == 2;
+        }
+      }
+      int upto = edges;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      uint64_t tie = ties_before + upto - edges;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (f[j] == 1) add[j] = w[4 * (q + lane) + j];
+        if (f[j] == 2) add[j] = tie++ < ties ? cut.w : 0;
+        sum += add[j];
+      }
+      uint64_t inc = sum;
       for (int o = 1; o < 32; o <<= 1) {
         const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
       }
-      if (goal >= before + inc - add && goal < before + inc) {
-        tokens[b] = (int32_t)(begin + i + lane);
-        if (probs) probs[b] = (float)((double)add / (double)total);
+      uint64_t at = before + inc - sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (goal >= at && goal < at + add[j]) {
+          tokens[b] = (int32_t)(begin + 4 * (q + lane) + j);
+          if (probs) probs[b] = (float)((double)add[j] / (double)total);
+        }
+        at += add[j];
       }
       before += __shfl_sync(0xffffffffu, inc, 31);
-      ties_before += __popc(at_edge);
+      ties_before += __shfl_sync(0xffffffffu, upto, 31);
       if (before > goal) break;
     }
   }
-  cluster.sync();  // no CTA leaves while another reads its memory
 }
 
 }  // namespace

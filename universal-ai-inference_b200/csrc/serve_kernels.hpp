@@ -62,7 +62,7 @@ size_t prefix_attn_ws(const PrefixAttnArgs& a);
 cudaError_t launch_prefix_attn(PrefixAttnArgs a, void* ws, int* launches, cudaStream_t st);
 
 // A row's weights lie in the shared memory of eight SMs.
-constexpr int64_t kSampleMaxVocab = 8 * 51200;
+constexpr int64_t kSampleMaxVocab = 8 * 50000;
 // One token per row of logits [B, V] (f16 when half, else f32; rows ld elements apart); probs and kept may be null.
 cudaError_t launch_sample(const void* logits, bool half, int64_t B, int64_t V, int64_t ld, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* tokens,
