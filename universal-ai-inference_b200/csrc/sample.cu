@@ -99,8 +99,9 @@ __device__ __forceinline__ uint64_t reach_of(float p, uint64_t mass) {  // at le
 // ---------------------------------------------------------------- a row in a cluster's shared memory
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
-constexpr int kBins = kThreads, kList = 1024, kMaxCluster = 8;
-constexpr int kFixed = 3 * kBins * 8 + 3 * kList * 4;            // dynamic shared memory besides the weights
+constexpr int kBins = 512, kList = 1024, kMaxCluster = 8;
+constexpr int kGroups = kThreads / (kBins / 2);         // threads that read the same bins, of different CTAs
+constexpr int kFixed = (2 + kGroups) * kBins * 8 + 3 * kList * 4;  // dynamic shared memory besides the weights
 constexpr int kMaxSlice = (int)(kSampleMaxVocab / kMaxCluster);  // weights of a CTA
 static_assert(kFixed + 4 * kMaxSlice <= 225 * 1024, "a CTA's shared memory");
 
@@ -135,7 +136,7 @@ struct Row {
   RowShared& sh;
   uint32_t* w;          // this CTA's weights, in index order; zeros up to a multiple of four
   uint2* bins;          // [2][kBins]: a bin's sum of low halves and of high halves (32-bit atomics are native)
-  uint64_t* sums;       // [kBins] of all CTAs
+  uint64_t* sums;       // [kGroups][kBins]
   uint32_t* list;       // [2][kList] of this CTA, and [kList] of all
   int quads;            // fours of weights of this CTA
   int rank, ctas;
@@ -170,34 +171,32 @@ struct Row {
     __syncthreads();
     return bins + set * kBins;
   }
-  // The bin, from the highest down, at which the cluster's bins reach `goal`: sh.bin and sh.above (plus `above`).  Half of
-  // the threads read the even CTAs' bins and half the odd ones', two bins at a time and 512 bytes a warp: scattered reads
-  // of distributed shared memory took 10 us.
+  // The bin, from the highest down, at which the cluster's bins reach `goal`: sh.bin and sh.above (plus `above`).  Remote
+  // shared memory gave 4 to 5 bytes a cycle to an SM, so bins are read in 512-byte pieces and are no more than
+  // 512: 1024 took 4 us more, 256 left longer lists to rank (381 against 341 us at 256 rows of 151936).
   __device__ __forceinline__ void reach(uint64_t goal, uint64_t above) {
-    const int t = threadIdx.x, at = t & (kBins / 2 - 1), odd = t / (kBins / 2);
-    uint4 y[kMaxCluster / 2];
+    constexpr int kEach = kMaxCluster / kGroups;
+    const int t = threadIdx.x, at = t % (kBins / 2), group = t / (kBins / 2);
+    uint4 y[kEach];
 #pragma unroll
-    for (int k = 0; k < kMaxCluster / 2; ++k) {
+    for (int k = 0; k < kEach; ++k) {
       y[k] = make_uint4(0, 0, 0, 0);
-      if (2 * k + odd < ctas) y[k] = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins + set * kBins, 2 * k + odd))[at];
+      const int c = k * kGroups + group;
+      if (c < ctas) y[k] = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins + set * kBins, c))[at];
     }
     uint64_t two[2] = {};
 #pragma unroll
-    for (int k = 0; k < kMaxCluster / 2; ++k) {
+    for (int k = 0; k < kEach; ++k) {
       two[0] += y[k].x + ((uint64_t)y[k].y << 16);
       two[1] += y[k].z + ((uint64_t)y[k].w << 16);
     }
-    if (odd) {
-      sums[2 * at] = two[0];
-      sums[2 * at + 1] = two[1];
-    }
+    sums[group * kBins + 2 * at] = two[0];
+    sums[group * kBins + 2 * at + 1] = two[1];
     __syncthreads();
-    if (!odd) {
-      sums[2 * at] += two[0];
-      sums[2 * at + 1] += two[1];
-    }
-    __syncthreads();
-    const uint64_t mine = sums[kBins - 1 - t];
+    uint64_t mine = 0;
+    if (t < kBins)
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) mine += sums[k * kBins + kBins - 1 - t];
     uint64_t inc = mine;
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -214,10 +213,58 @@ struct Row {
     __syncthreads();
   }
 
+  __device__ __forceinline__ void put(uint32_t x) {  // into this CTA's list
+    const uint32_t k = atomicAdd(&sh.listed[set], 1u);
+    if (k < kList) list[set * kList + k] = x;
+  }
+  // Of the numbers that the CTAs have listed, the one at which the leading ones reach `goal`, `above` lying above them
+  // all.  False, with their count in f->equal, if they are more than a list holds.
+  template <bool MASS>
+  __device__ bool rank_listed(uint64_t goal, uint64_t above, Found* f) {
+    const int t = threadIdx.x;
+    cluster.sync();
+    uint32_t count[kMaxCluster], listed = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) count[c] = c < ctas ? cluster.map_shared_rank(&sh, c)->listed[set] : 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) listed += count[c];
+    f->equal = listed;
+    if (listed > kList) return false;
+    uint32_t* all = list + 2 * kList;
+    for (uint32_t i = t; i < listed; i += kThreads) {
+      uint32_t j = i;
+      int c = 0;
+#pragma unroll
+      for (int k = 0; k + 1 < kMaxCluster; ++k)
+        if (c == k && j >= count[k]) {
+          j -= count[k];
+          c = k + 1;
+        }
+      all[i] = cluster.map_shared_rank(list + set * kList, c)[j];
+    }
+    __syncthreads();
+    for (uint32_t i = t; i < listed; i += kThreads) {
+      const uint32_t x = all[i];
+      uint64_t over = above;
+      uint32_t equal = 0;
+      for (uint32_t j = 0; j < listed; ++j) {
+        const uint32_t y = all[j];
+        over += y > x ? (MASS ? y : 1u) : 0u;
+        equal += y == x;
+      }
+      const uint64_t each = MASS ? x : 1;
+      if (over < goal && goal <= over + equal * each)  // (the same numbers write the same)
+        sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
+    }
+    __syncthreads();
+    *f = sh.found;
+    __syncthreads();
+    return true;
+  }
+
   // The cut at which the leading weights reach `goal` (in tokens, or in mass).  `least`: weights below it cannot matter.
   template <bool MASS>
   __device__ Found find(uint64_t goal, uint32_t least) {
-    const int t = threadIdx.x;
     // weights in [lo, hi] are binned: by leading bits at first, then, should a bin hold more than the list does, by
     // equal parts of its range
     uint32_t lo = least ? least : 1, hi = kOne;
@@ -251,57 +298,17 @@ struct Row {
       }
       from = max(from, lo);
       to = min(to, hi);
-      // the bin's weights: every CTA lists its own, then reads all lists and ranks them
-      uint32_t* own = list + set * kList;
+      // the bin's weights
       each4([&](int, uint4 v) {
         if (max(max(v.x, v.y), max(v.z, v.w)) < from) return;
         const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (x[j] >= from && x[j] <= to) {
-            const uint32_t k = atomicAdd(&sh.listed[set], 1u);
-            if (k < kList) own[k] = x[j];
-          }
+          if (x[j] >= from && x[j] <= to) put(x[j]);
       });
-      cluster.sync();
-      uint32_t count[kMaxCluster], listed = 0;
-#pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c) count[c] = c < ctas ? cluster.map_shared_rank(&sh, c)->listed[set] : 0;
-#pragma unroll
-      for (int c = 0; c < kMaxCluster; ++c) listed += count[c];
-      if (from == to) return Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, listed};
-      if (listed <= kList) {
-        uint32_t* all = list + 2 * kList;
-        for (uint32_t i = t; i < listed; i += kThreads) {
-          uint32_t at_ = i;
-          int c = 0;
-#pragma unroll
-          for (int k = 0; k + 1 < kMaxCluster; ++k)
-            if (c == k && at_ >= count[k]) {
-              at_ -= count[k];
-              c = k + 1;
-            }
-          all[i] = cluster.map_shared_rank(own, c)[at_];
-        }
-        __syncthreads();
-        for (uint32_t i = t; i < listed; i += kThreads) {
-          const uint32_t x = all[i];
-          uint64_t over = above;
-          uint32_t equal = 0;
-          for (uint32_t j = 0; j < listed; ++j) {
-            const uint32_t y = all[j];
-            over += y > x ? (MASS ? y : 1u) : 0u;
-            equal += y == x;
-          }
-          const uint64_t each = MASS ? x : 1;
-          if (over < goal && goal <= over + equal * each)  // (tokens of the same weight write the same)
-            sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
-        }
-        __syncthreads();
-        const Found f = sh.found;
-        __syncthreads();
-        return f;
-      }
+      Found f;
+      if (rank_listed<MASS>(goal, above, &f)) return f;
+      if (from == to) return Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, f.equal};
       lo = from;
       hi = to;
       const int bits = 32 - __clz(to - from);
@@ -311,7 +318,7 @@ struct Row {
 };
 
 template <typename X>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ logits, int64_t V, int64_t ld, int slice, bool vec,
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict__ logits, int64_t V, int64_t ld, int slice, bool vec,
                                                           const float* __restrict__ temperature,
                                                           const int32_t* __restrict__ top_k,
                                                           const float* __restrict__ top_p,
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   const int n = (int)max(int64_t(0), min((int64_t)slice, V - begin));
   uint2* bins = reinterpret_cast<uint2*>(dynamic);
   uint64_t* sums = reinterpret_cast<uint64_t*>(bins + 2 * kBins);
-  uint32_t* list = reinterpret_cast<uint32_t*>(sums + kBins);
+  uint32_t* list = reinterpret_cast<uint32_t*>(sums + kGroups * kBins);
   uint32_t* w = list + 3 * kList;
   Row row{cluster, sh, w, bins, sums, list, (n + 3) / 4, rank, ctas, 0};
   const X* x = logits + b * ld + begin;
@@ -420,7 +427,19 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   if (s.k == 1) {  // the first of the largest
     edge = top;
     ties = 1;
-  } else if (partial) {  // eight bits of the key at a time, over the logits read again
+  } else if (partial && cut.equal <= kList) {  // their logits, read again
+    (void)row.next_bins();
+    row.each4([&](int i, uint4 v) {
+      const uint32_t y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (y[j] == cut.w) row.put(key_of_logit(logit(x + i + j)));
+    });
+    Found f;
+    (void)row.rank_listed<false>(cut.need, 0, &f);
+    edge = f.w;
+    ties = f.need;
+  } else if (partial) {  // eight bits of the keys at a time
     uint64_t need = cut.need;
     for (int shift = 24; shift >= 0; shift -= 8) {
       uint2* mine = row.next_bins();
@@ -446,8 +465,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
   // rounding may have brought there from below, is told by its exponential.
   const float least = s.k == 1 ? 0.f : s.least;
   const uint32_t w_least = least > 0.f ? weight(least) : 0;
-  auto side = [&](int i) {
-    const uint32_t y = w[i];
+  auto side = [&](int i, uint32_t y) {
+    if (i >= n) return 0;
     if (y < cut.w || y < w_least) return 0;
     if (least > 0.f && y == w_least && !(heat.exp_of(canonical(logit(x + i))) >= least)) return 0;
     if (y > cut.w || !partial) return 1;
@@ -464,8 +483,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
     if (max(max(v.x, v.y), max(v.z, v.w)) < low) continue;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int i = 4 * q + j, f = i < n ? side(i) : 0;
-      seg_mass += f == 1 ? w[i] : 0;
+      const uint32_t y = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+      const int f = side(4 * q + j, y);
+      seg_mass += f == 1 ? y : 0;
       seg_count += f == 1;
       seg_ties += f == 2;
     }
@@ -517,8 +537,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const X* __restrict__ 
       if (q + lane < q1) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int i = 4 * (q + lane) + j;
-          f[j] = i < n ? side(i) : 0;
+          f[j] = side(4 * (q + lane) + j, w[4 * (q + lane) + j]);
           edges += f[j] == 2;
         }
       }
