@@ -433,7 +433,7 @@ UAII_MOE_API int uaii_moe_profile_read(uaii_moe_backend* b, double* phase_ms, ui
 #define UAII_MOE_KV_E4M3 33
 
 /* One layer's cache, owned by the caller: k, v [batch, n_kv_heads, max_seq, head_dim] f16 or bytes, dense, 16-byte
- * aligned; k_scale, v_scale f32 [batch, n_kv_heads, max_seq] (NULL for f16).  head_dim 64 or 128. */
+ * aligned; k_scale, v_scale f32 [batch, n_kv_heads, max_seq] (NULL for f16).  head_dim 64 or 128; batch * n_kv_heads up to 65535. */
 typedef struct uaii_moe_kv_cache {
   int32_t fmt;
   int32_t head_dim;

@@ -19,6 +19,7 @@ namespace uaii_b200 {
 namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
+constexpr int kRows = 2;  // rows of a thread, loaded together
 
 __device__ __forceinline__ void load8(const float* p, bool vec, float (&x)[8]) {
   if (vec) {
@@ -79,32 +80,40 @@ __device__ __forceinline__ float store_row8(const float (&x)[8], void* row, int 
   }
 }
 
-// One group of HD / 8 lanes per (token, head, K or V); heads fastest, so a group's neighbours read on.
+// One group of HD / 8 lanes per row: grid (tokens x heads of a sequence, heads fastest; sequence; K or V), kRows groups
+// of heads x tokens a block apart for each thread, their loads under way together.
 template <int F, int HD, typename X>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __restrict__ k, const X* __restrict__ v,
-                                                        int64_t T, RowView s, const int32_t* __restrict__ pos,
+                                                        int T, RowView s, const int32_t* __restrict__ pos,
                                                         const int32_t* __restrict__ n_new, bool vec, int* err) {
-  constexpr int kLanes = HD / 8;
-  const int64_t id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
-  const int lane8 = threadIdx.x % kLanes;
-  const int64_t rows = c.batch * T * c.heads;
-  const bool live = id < 2 * rows;
-  const bool is_v = id >= rows;
-  const int64_t r = live ? (is_v ? id - rows : id) : 0;
-  const int64_t h = r % c.heads, t = (r / c.heads) % T, b = r / (c.heads * T);
-  const int64_t at = (int64_t)pos[b] + t;
-  bool write = live && (n_new == nullptr || t < n_new[b]);
-  if (write && (at < 0 || at >= c.max_seq)) {
-    if (lane8 == 0) atomicExch(err, kErrKvPosition);
-    write = false;
-  }
-  float x[8] = {};
-  if (write) load8((is_v ? v : k) + b * s.batch + t * s.token + h * s.head + 8 * lane8, vec, x);
-  const int64_t row = (b * c.heads + h) * c.max_seq + at;
+  constexpr int kLanes = HD / 8, kGroups = 256 / kLanes;
+  const int lane8 = threadIdx.x % kLanes, heads = (int)c.heads, b = blockIdx.y;
+  const bool is_v = blockIdx.z != 0;
+  const X* from = (is_v ? v : k) + b * s.batch + 8 * lane8;
+  const int count = n_new ? min(n_new[b], T) : T, start = pos[b], rows = count * heads;
+  char* out = static_cast<char*>(is_v ? c.v : c.k);
+  float* scales = is_v ? c.v_scale : c.k_scale;
   constexpr int kBytes = F == kKvF16 ? 2 * HD : HD;
-  const float sc =
-      store_row8<F, HD>(x, write ? static_cast<char*>(is_v ? c.v : c.k) + row * kBytes : nullptr, lane8);
-  if (F != kKvF16 && write && lane8 == 0) (is_v ? c.v_scale : c.k_scale)[row] = sc;
+  float x[kRows][8] = {};
+  int64_t row[kRows];  // of the cache; -1: none
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int r = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes, t = r / heads, h = r - t * heads;
+    const int64_t at = (int64_t)start + t;
+    row[i] = -1;
+    if (r >= rows) continue;
+    if (at < 0 || at >= c.max_seq) {
+      if (lane8 == 0) atomicExch(err, kErrKvPosition);
+      continue;
+    }
+    row[i] = ((int64_t)b * heads + h) * c.max_seq + at;
+    load8(from + t * s.token + h * s.head, vec, x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const float sc = store_row8<F, HD>(x[i], row[i] >= 0 ? out + row[i] * kBytes : nullptr, lane8);
+    if (F != kKvF16 && row[i] >= 0 && lane8 == 0) scales[row[i]] = sc;
+  }
 }
 
 template <int F>
@@ -125,42 +134,63 @@ __device__ __forceinline__ void put8(__half* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
 
-// A thread takes 8 values of one row.
+// Positions of one (sequence, head) plane, K or V: grid (positions; plane; K or V).  A thread takes 16 values of a row,
+// kRows rows a block apart.
 template <int F, int HD, typename Y>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvCache c, int64_t pos0, int64_t n, Y* __restrict__ k_out,
-                                                      Y* __restrict__ v_out) {
-  constexpr int kLanes = HD / 8;
-  const int64_t rows = c.batch * c.heads * n;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < 2 * rows * kLanes; id += (int64_t)gridDim.x * 256) {
-    const int64_t q = id / kLanes;
-    const int lane8 = (int)(id % kLanes);
-    const bool is_v = q >= rows;
-    const int64_t r = is_v ? q - rows : q;
-    const int64_t bh = r / n, row = bh * c.max_seq + pos0 + (r - bh * n);
-    float x[8];
-    if constexpr (F == kKvF16) {
-      load8(static_cast<const __half*>(is_v ? c.v : c.k) + row * HD + 8 * lane8, true, x);
-    } else {
-      const float sc = (is_v ? c.v_scale : c.k_scale)[row];
-      const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const char*>(is_v ? c.v : c.k) + row * HD + 8 * lane8);
+__global__ void __launch_bounds__(256) kv_read_kernel(KvCache c, int64_t pos0, int n, Y* __restrict__ k_out, Y* __restrict__ v_out) {
+  constexpr int kLanes = HD / 16, kGroups = 256 / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const bool is_v = blockIdx.z != 0;
+  const int64_t plane = (int64_t)blockIdx.y * c.max_seq + pos0;
+  const char* from = static_cast<const char*>(is_v ? c.v : c.k);
+  const float* scales = is_v ? c.v_scale : c.k_scale;
+  Y* to = (is_v ? v_out : k_out) + (int64_t)blockIdx.y * n * HD + 16 * lane;
+  constexpr int kLoads = F == kKvF16 ? 2 : 1;  // of 16 bytes
+  uint4 w[kRows][kLoads];
+  float sc[kRows];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = value_of<F>(((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u, sc);
+  for (int i = 0; i < kRows; ++i) {
+    const int j = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes;
+    sc[i] = 0.f;
+    if (j >= n) continue;
+    const uint4* src = reinterpret_cast<const uint4*>(from + (plane + j) * (HD * kLoads)) + lane * kLoads;
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) w[i][l] = __ldcs(src + l);
+    if (F != kKvF16) sc[i] = __ldcs(scales + plane + j);
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int j = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes;
+    if (j >= n) continue;
+    float x[2][8];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const uint4 q = w[i][F == kKvF16 ? k / 8 : 0];
+      if constexpr (F == kKvF16) {
+        const int e = k & 7;
+        const uint32_t u = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
+        x[k / 8][e] = __half2float(__ushort_as_half((unsigned short)(e & 1 ? u >> 16 : u & 0xffffu)));
+      } else {
+        const uint32_t u = k < 4 ? q.x : k < 8 ? q.y : k < 12 ? q.z : q.w;
+        x[k / 8][k & 7] = value_of<F>((u >> (8 * (k & 3))) & 255u, sc[i]);
+      }
     }
-    put8((is_v ? v_out : k_out) + r * HD + 8 * lane8, x);
+    put8(to + (int64_t)j * HD, x[0]);
+    put8(to + (int64_t)j * HD + 8, x[1]);
   }
 }
 
 template <int F, typename X>
 cudaError_t append_fmt(const KvCache& c, const X* k, const X* v, int64_t T, const RowView& s, const int32_t* pos,
                        const int32_t* n_new, int* err, cudaStream_t st) {
-  const int lanes = c.hd / 8;
-  const int64_t blocks = (2 * c.batch * T * c.heads * lanes + 255) / 256;
-  if (blocks > 0x7fffffff) return cudaErrorInvalidValue;
+  const int64_t per = kRows * (256 / (c.hd / 8)), blocks = (T * c.heads + per - 1) / per;
+  if (blocks > 0x7fffffff || c.batch > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, (unsigned)c.batch, 2);
   const size_t m = 16 / sizeof(X);  // 16-byte loads where every row starts on such a boundary
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 && s.batch % m == 0 &&
                    s.token % m == 0 && s.head % m == 0;
-  if (c.hd == 128) kv_append_kernel<F, 128, X><<<(unsigned)blocks, 256, 0, st>>>(c, k, v, T, s, pos, n_new, vec, err);
-  else kv_append_kernel<F, 64, X><<<(unsigned)blocks, 256, 0, st>>>(c, k, v, T, s, pos, n_new, vec, err);
+  if (c.hd == 128) kv_append_kernel<F, 128, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, err);
+  else kv_append_kernel<F, 64, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, err);
   return cudaGetLastError();
 }
 
@@ -175,10 +205,11 @@ cudaError_t append_any(const KvCache& c, const void* k, const void* v, int64_t T
 
 template <int F, typename Y>
 cudaError_t read_fmt(const KvCache& c, int64_t pos0, int64_t n, Y* k, Y* v, cudaStream_t st) {
-  const int64_t blocks = (2 * c.batch * c.heads * n * (c.hd / 8) + 255) / 256;
-  const unsigned g = (unsigned)(blocks < 148 * 64 ? blocks : 148 * 64);
-  if (c.hd == 128) kv_read_kernel<F, 128, Y><<<g, 256, 0, st>>>(c, pos0, n, k, v);
-  else kv_read_kernel<F, 64, Y><<<g, 256, 0, st>>>(c, pos0, n, k, v);
+  const int64_t per = kRows * (256 / (c.hd / 16)), blocks = (n + per - 1) / per;
+  if (c.batch * c.heads > 65535) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)blocks, (unsigned)(c.batch * c.heads), 2);
+  if (c.hd == 128) kv_read_kernel<F, 128, Y><<<grid, 256, 0, st>>>(c, pos0, (int)n, k, v);
+  else kv_read_kernel<F, 64, Y><<<grid, 256, 0, st>>>(c, pos0, (int)n, k, v);
   return cudaGetLastError();
 }
 

@@ -37,7 +37,7 @@ Error kv_cache_from_c(const char* op, const uaii_moe_kv_cache* s, KvCache* out) 
   if (s->head_dim != 64 && s->head_dim != 128)
     return Error::make(ErrorCode::NotImplemented, o + ": head_dim must be 64 or 128");
   if (s->batch <= 0 || s->n_kv_heads <= 0 || s->max_seq <= 0 || s->batch >= kMaxCount || s->n_kv_heads >= kMaxCount ||
-      s->max_seq >= kMaxCount || s->batch * s->n_kv_heads >= kMaxCount)
+      s->max_seq >= kMaxCount || s->batch > kKvMaxPlanes || s->batch * s->n_kv_heads > kKvMaxPlanes)
     return invalid(o + ": cache sizes out of range");
   if (!is_device_ptr(s->k) || !is_device_ptr(s->v)) return invalid(o + ": the cache must be device memory");
   if (!aligned(s->k, 16) || !aligned(s->v, 16)) return invalid(o + ": the cache must start on a 16-byte boundary");

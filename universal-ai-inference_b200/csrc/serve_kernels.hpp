@@ -15,6 +15,9 @@ namespace uaii_b200 {
 // (value = (byte - 128) * scale, or e4m3(byte) * scale).  The values of the C ABI.
 enum KvFormat { kKvF16 = 1, kKvI8 = 32, kKvE4M3 = 33 };
 
+// (sequence, kv head) planes of a cache: one dimension of a grid.
+constexpr int64_t kKvMaxPlanes = 65535;
+
 // Codes in the backend's device error word for arguments that only the device can see.
 constexpr int kErrKvPosition = 32;  // kv_append: a position outside the cache
 constexpr int kErrKvLength = 33;    // attention: a length outside the cache

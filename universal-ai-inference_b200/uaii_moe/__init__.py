@@ -203,19 +203,25 @@ def ptr(a) -> int | None:
     raise TypeError(f"cannot take the address of {type(a)}")
 
 
+def _torch():
+    """torch, which whoever holds a tensor has imported (this module does not need it)."""
+    import sys
+    return sys.modules["torch"]
+
+
 def _dtype_code(t) -> int:
     """UAII_MOE_DTYPE_* of a torch tensor's element type (f32 or f16)."""
-    name = str(t.dtype)
-    if name == "torch.float32":
+    d = t.dtype
+    if d is _torch().float32:
         return DTYPE_F32
-    if name == "torch.float16":
+    if d is _torch().float16:
         return DTYPE_F16
-    raise TypeError(f"expected float32 or float16, got {name}")
+    raise TypeError(f"expected float32 or float16, got {d}")
 
 
 def _rows(t, *shape):
     """Element strides (batch, token, head) of a [batch, token, head, head_dim] view with a dense last dimension."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"expected shape {shape}, got {tuple(t.shape)}")
     sb, st, sh, sd = t.stride()
     if sd != 1:
@@ -224,14 +230,16 @@ def _rows(t, *shape):
 
 
 def _whole(t, what, *shape):
-    """Address of a dense int32 / f32 vector or matrix of a known shape."""
-    if tuple(t.shape) != shape:
+    """Address of a dense tensor of a known shape."""
+    if t.shape != shape:
         raise ValueError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
-    return ptr(t)
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: tensor must be contiguous")
+    return t.data_ptr()
 
 
 def _typed(t, what, dtype, *shape):
-    if str(t.dtype) != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
     return _whole(t, what, *shape)
 
@@ -239,12 +247,13 @@ def _typed(t, what, dtype, *shape):
 def kv_cache(fmt: int, k, v, k_scale=None, v_scale=None) -> KVCache:
     """A KV cache over CUDA tensors k, v [batch, n_kv_heads, max_seq, head_dim] (float16 for F16, uint8 for KV_I8 and
     KV_E4M3) and, for the 8-bit formats, float32 scales [batch, n_kv_heads, max_seq].  Keeps the tensors alive."""
-    want = "torch.float16" if fmt == F16 else "torch.uint8"
+    T = _torch()
+    want = T.float16 if fmt == F16 else T.uint8
     b, h, s, d = k.shape
     c = KVCache(fmt, d, b, h, s, _typed(k, "k", want, b, h, s, d), _typed(v, "v", want, b, h, s, d))
     if fmt != F16:
-        c.k_scale = _typed(k_scale, "k_scale", "torch.float32", b, h, s)
-        c.v_scale = _typed(v_scale, "v_scale", "torch.float32", b, h, s)
+        c.k_scale = _typed(k_scale, "k_scale", T.float32, b, h, s)
+        c.v_scale = _typed(v_scale, "v_scale", T.float32, b, h, s)
     c._keep = (k, v, k_scale, v_scale)
     return c
 
@@ -406,8 +415,8 @@ class Backend:
         if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
             raise ValueError("k and v must have the same shape, strides and type")
         _check(lib.uaii_moe_kv_append(self._h, byref(cache), k.data_ptr(), v.data_ptr(), _dtype_code(k), t, sb, st, sh,
-                                      _typed(pos, "pos", "torch.int32", b),
-                                      None if n_new is None else _typed(n_new, "n_new", "torch.int32", b)))
+                                      _typed(pos, "pos", _torch().int32, b),
+                                      None if n_new is None else _typed(n_new, "n_new", _torch().int32, b)))
 
     def kv_read(self, cache: KVCache, pos0: int, n: int, k_out, v_out):
         """Positions [pos0, pos0 + n) into k_out, v_out [batch, n_kv_heads, n, head_dim] (f32 or f16)."""
@@ -426,7 +435,7 @@ class Backend:
         if out.dtype != q.dtype:
             raise ValueError("out must have q's type")
         _check(lib.uaii_moe_prefix_attention(self._h, None if prefix is None else byref(prefix), prefix_len, byref(own),
-                                             _typed(own_len, "own_len", "torch.int32", b), q.data_ptr(),
+                                             _typed(own_len, "own_len", _torch().int32, b), q.data_ptr(),
                                              _dtype_code(q), h, t, sb, st, sh, scale, _whole(out, "out", b, t, h, d)))
 
     def sample(self, logits, temperature, top_k, top_p, min_p, u, tokens, probs=None, kept=None):
@@ -435,7 +444,7 @@ class Backend:
         b, v = logits.shape
         if logits.stride(1) != 1 and v > 1:
             raise ValueError("a row of logits must be dense")
-        f, i = "torch.float32", "torch.int32"
+        f, i = _torch().float32, _torch().int32
         _check(lib.uaii_moe_sample(self._h, logits.data_ptr(), _dtype_code(logits), b, v,
                                    logits.stride(0) if b > 1 else v,
                                    _typed(temperature, "temperature", f, b), _typed(top_k, "top_k", i, b),
