@@ -553,6 +553,23 @@ UAII_MOE_API int uaii_moe_decoder_step(uaii_moe_decoder* d, const int32_t* token
 UAII_MOE_API int uaii_moe_decoder_generate(uaii_moe_decoder* d, const int32_t* tokens, int64_t steps, int32_t* out);
 UAII_MOE_API int64_t uaii_moe_decoder_position(const uaii_moe_decoder* d);
 
+/* A serving decoder: its caches in kv_fmt (UAII_MOE_F16, UAII_MOE_KV_I8 or UAII_MOE_KV_E4M3), written by kv_append and
+ * read by prefix_attention, with room for a prefix of up to prefix_max positions per layer that every sequence shares.
+ * Steps, set_kv (positions after the prefix) and generate work as above; fill_kv does not. */
+UAII_MOE_API int uaii_moe_decoder_create_serving(uaii_moe_backend* b, const uaii_moe_decoder_config* cfg, int kv_fmt,
+                                                 int64_t prefix_max, const uaii_moe_decoder_block* blocks,
+                                                 const float* output_norm, const void* token_embd, int embd_fmt,
+                                                 const void* output, int output_fmt, uaii_moe_decoder** out);
+/* The shared prefix of layer `layer`: f32 k, v [n_kv_heads, n_pos, head_dim] (host or device), rotated to positions
+ * 0 .. n_pos - 1 already.  The sequences' own positions follow it; give every layer the same n_pos. */
+UAII_MOE_API int uaii_moe_decoder_set_prefix(uaii_moe_decoder* d, int64_t layer, const float* k, const float* v,
+                                             int64_t n_pos);
+/* One step whose next tokens are drawn by uaii_moe_sample from the step's logits: temperature, top_k, top_p, min_p, u,
+ * next and probs (or NULL) are device arrays [batch]; logits as in uaii_moe_decoder_step. */
+UAII_MOE_API int uaii_moe_decoder_step_sampled(uaii_moe_decoder* d, const int32_t* tokens, const float* temperature,
+                                               const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                                               int32_t* next, float* probs, float* logits);
+
 /* Device-side synthetic inputs (no reference counterpart): uaii_moe_fill_normal's draws
  * written on the backend's stream (equal to the host generator's up to the last bit of the
  * device's double-precision log/sin/cos), and uaii_moe_quantize_rows on the device (the same

@@ -19,6 +19,9 @@ cudaError_t launch_add_rmsnorm(float* x, const float* delta, const float* w, int
 cudaError_t launch_rope_append(const float* qkv, int64_t B, int64_t H, int64_t Hkv, int64_t hd, const float* freq,
                                int64_t pos, int mode, float* q_out, void* kc, void* vc, int64_t max_seq,
                                cudaStream_t st);
+// The same rotation in place at position pos + shift, and own_pos[b] = pos, own_len[b] = pos + 1.
+cudaError_t launch_rope_rows(float* qkv, int64_t B, int64_t H, int64_t Hkv, int64_t hd, const float* freq, int64_t pos,
+                             int64_t shift, int mode, int32_t* own_pos, int32_t* own_len, cudaStream_t st);
 // Splits (of 128 positions) of the attention over len positions; partial buffers hold
 // B*H*splits*hd (po) and B*H*splits (pm, pl) floats.
 int attn_splits(int64_t len);

@@ -156,6 +156,31 @@ __global__ void rope_append_kernel(const float* __restrict__ qkv, int64_t H, int
   }
 }
 
+// RoPE of q and k in place, in a qkv buffer laid out as above, at position pos + shift (a serving decoder's prefix lies
+// before its own positions); own_pos[b] = pos and own_len[b] = pos + 1 for the kernels that append and attend next.
+__global__ void rope_rows_kernel(float* __restrict__ qkv, int64_t H, int64_t Hkv, int64_t hd, const float* __restrict__ freq,
+                                 int64_t pos, int64_t shift, int mode, int32_t* __restrict__ own_pos,
+                                 int32_t* __restrict__ own_len) {
+  const int64_t b = blockIdx.x;
+  const int half = (int)(hd / 2), pairs = (int)(H + Hkv) * half;
+  float* row = qkv + b * (H + 2 * Hkv) * hd;
+  const float fpos = (float)(pos + shift);
+  for (int p = threadIdx.x; p < pairs; p += blockDim.x) {  // heads of q, then of k: they lie back to back
+    const int h = p / half, i = p - h * half;
+    float s, c;
+    sincosf(__fmul_rn(fpos, freq[i]), &s, &c);
+    const int ia = mode == 2 ? i : 2 * i, ib = mode == 2 ? i + half : 2 * i + 1;
+    float oa, ob;
+    rotate(row[h * hd + ia], row[h * hd + ib], c, s, oa, ob);
+    row[h * hd + ia] = oa;
+    row[h * hd + ib] = ob;
+  }
+  if (threadIdx.x == 0) {
+    own_pos[b] = (int32_t)pos;
+    own_len[b] = (int32_t)pos + 1;
+  }
+}
+
 // ---- attention of one new position over the cache (attention_kv_f32, transformer.cpp:227-345:
 // scores q.k * scale, softmax over positions 0..len-1, sum of p * v), on the tensor cores.
 // CTA (split, kv head, b) handles kAttnChunk positions for the G = H / Hkv query heads that
@@ -630,6 +655,13 @@ cudaError_t launch_rope_append(const float* qkv, int64_t B, int64_t H, int64_t H
   if (hd % 2 || pos < 0 || pos >= max_seq) return cudaErrorInvalidValue;
   rope_append_kernel<<<(unsigned)B, 256, 0, st>>>(qkv, H, Hkv, hd, freq, pos, mode, q_out, static_cast<__half*>(kc),
                                                   static_cast<__half*>(vc), max_seq);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_rope_rows(float* qkv, int64_t B, int64_t H, int64_t Hkv, int64_t hd, const float* freq, int64_t pos,
+                             int64_t shift, int mode, int32_t* own_pos, int32_t* own_len, cudaStream_t st) {
+  if (hd % 2 || pos < 0 || shift < 0) return cudaErrorInvalidValue;
+  rope_rows_kernel<<<(unsigned)B, 256, 0, st>>>(qkv, H, Hkv, hd, freq, pos, shift, mode, own_pos, own_len);
   return cudaGetLastError();
 }
 

@@ -17,8 +17,14 @@
 // (MoeCudaBackend::ffn: router, top-k, grouped expert GEMMs, combine), the rest on
 // the kernels of decode_model.cu.  All positions of the batch advance together;
 // the cache holds max_seq positions per sequence in f16.
+//
+// A serving decoder keeps its caches in f16 or 8 bits (kv_append quantises K and V as they are written) with one more
+// cache per layer for a prefix that every sequence shares, attends with prefix_attention, and can sample its tokens.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <exception>
+#include <memory>
 #include <string>
 #include <vector>
 
@@ -26,6 +32,7 @@
 #include "backend.hpp"
 #include "decode_kernels.hpp"
 #include "gguf_format.hpp"
+#include "serve_kernels.hpp"
 
 namespace uaii_b200 {
 
@@ -46,9 +53,17 @@ class Decoder {
   ~Decoder() { release(); }
 
   Error create(MoeCudaBackend* be, const uaii_moe_decoder_config& c, const uaii_moe_decoder_block* blocks,
-               const float* out_norm, const void* embd, int embd_fmt, const void* output, int output_fmt) {
+               const float* out_norm, const void* embd, int embd_fmt, const void* output, int output_fmt,
+               int serve_fmt = 0, int64_t prefix_max = 0) {
     be_ = be;
     cfg_ = c;
+    serve_fmt_ = serve_fmt;
+    prefix_max_ = prefix_max;
+    if (serve_fmt != 0 && serve_fmt != kKvF16 && serve_fmt != kKvI8 && serve_fmt != kKvE4M3)
+      return Error::make(ErrorCode::NotImplemented, "decoder: cache format must be F16, KV_I8 or KV_E4M3");
+    if (prefix_max < 0) return Error::make(ErrorCode::InvalidArgument, "decoder: prefix positions out of range");
+    if (serve_fmt != 0 && c.batch > kKvMaxPlanes / std::max<int64_t>(c.n_kv_heads, 1))
+      return Error::make(ErrorCode::InvalidArgument, "decoder: too many cache planes");
     const int64_t L = c.n_layers, D = c.d_model, H = c.n_heads, Hkv = c.n_kv_heads, hd = c.head_dim;
     if (L <= 0 || D <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || hd != 128 || c.vocab <= 0 || c.batch <= 0 ||
         c.max_seq <= 0 || (c.rope_mode != 0 && c.rope_mode != 2))
@@ -113,7 +128,7 @@ class Decoder {
     kc_.assign((size_t)L, nullptr);
     vc_.assign((size_t)L, nullptr);
     maps_.assign((size_t)(2 * L), KvMap{});
-    for (int64_t l = 0; l < L; ++l) {
+    for (int64_t l = 0; l < L && !serve_fmt_; ++l) {
       UAII_TRY(dmalloc(&kc_[(size_t)l], kv_bytes, "Malloc(K cache)"));
       UAII_TRY(dmalloc(&vc_[(size_t)l], kv_bytes, "Malloc(V cache)"));
       UAII_CUDA(cudaMemsetAsync(kc_[(size_t)l], 0, kv_bytes, st), "Memset(K cache)");
@@ -121,6 +136,16 @@ class Decoder {
       if (!make_kv_map(maps_[(size_t)(2 * l)].bytes, kc_[(size_t)l], B * Hkv * c.max_seq) ||
           !make_kv_map(maps_[(size_t)(2 * l + 1)].bytes, vc_[(size_t)l], B * Hkv * c.max_seq))
         return Error::make(ErrorCode::Internal, "decoder: KV-cache tensor map");
+    }
+    if (serve_fmt_) {
+      own_.assign((size_t)L, KvCache{});
+      prefix_.assign((size_t)L, KvCache{});
+      for (int64_t l = 0; l < L; ++l) {
+        UAII_TRY(make_cache(&own_[(size_t)l], B, c.max_seq));
+        if (prefix_max_) UAII_TRY(make_cache(&prefix_[(size_t)l], 1, prefix_max_));
+      }
+      UAII_TRY(dmalloc((void**)&own_pos_, sizeof(int32_t) * (size_t)B, "Malloc(positions)"));
+      UAII_TRY(dmalloc((void**)&own_len_, sizeof(int32_t) * (size_t)B, "Malloc(lengths)"));
     }
     UAII_TRY(dmalloc((void**)&x_, sizeof(float) * (size_t)(B * D), "Malloc(x)"));
     UAII_TRY(dmalloc((void**)&n_, sizeof(float) * (size_t)(B * D), "Malloc(n)"));
@@ -152,6 +177,13 @@ class Decoder {
     for (void* p : vc_) (void)cudaFree(p);
     kc_.clear();
     vc_.clear();
+    for (auto* caches : {&own_, &prefix_}) {
+      for (const KvCache& k : *caches)
+        for (void* p : {k.k, k.v, (void*)k.k_scale, (void*)k.v_scale}) (void)cudaFree(p);
+      caches->clear();
+    }
+    for (void* p : {(void*)own_pos_, (void*)own_len_}) (void)cudaFree(p);
+    own_pos_ = own_len_ = nullptr;
     for (void* p : {(void*)freq_, (void*)x_, (void*)n_, (void*)o_, (void*)ff_, (void*)qkv_, (void*)q_, (void*)attn_,
                     (void*)po_, (void*)pm_, (void*)pl_, (void*)logits_, (void*)tokens_, (void*)next_, (void*)err_})
       (void)cudaFree(p);
@@ -166,6 +198,11 @@ class Decoder {
     if (layer < 0 || layer >= cfg_.n_layers || n < 0 || n > cfg_.max_seq || !k || !v)
       return Error::make(ErrorCode::InvalidArgument, "decoder set_kv: layer or position count out of range");
     UAII_CUDA(cudaSetDevice(be_->device()), "SetDevice");
+    if (serve_fmt_) {
+      UAII_TRY(put(own_[(size_t)layer], k, v, n));
+      pos_ = n;
+      return Error::success();
+    }
     const int64_t rows = cfg_.batch * cfg_.n_kv_heads, hd = cfg_.head_dim;
     const size_t bytes = sizeof(float) * (size_t)(rows * n * hd);
     float* tmp = nullptr;
@@ -188,6 +225,7 @@ class Decoder {
   // counter-based); the decode position becomes n.
   Error fill_kv(int64_t n, uint64_t seed) {
     if (n < 0 || n > cfg_.max_seq) return Error::make(ErrorCode::InvalidArgument, "decoder fill_kv: n out of range");
+    if (serve_fmt_) return Error::make(ErrorCode::NotImplemented, "decoder fill_kv: a serving decoder takes set_kv");
     UAII_CUDA(cudaSetDevice(be_->device()), "SetDevice");
     const int64_t rows = cfg_.batch * cfg_.n_kv_heads, hd = cfg_.head_dim;
     for (int64_t l = 0; l < cfg_.n_layers; ++l)
@@ -198,6 +236,35 @@ class Decoder {
     UAII_CUDA(cudaStreamSynchronize(be_->stream()), "StreamSynchronize");
     pos_ = n;
     return Error::success();
+  }
+
+  // The shared prefix of one layer from f32 K and V [kv_heads, n, head_dim] (host or device, already rotated to
+  // positions 0 .. n - 1); own positions follow it.
+  Error set_prefix(int64_t layer, const float* k, const float* v, int64_t n) {
+    if (!serve_fmt_ || prefix_max_ == 0)
+      return Error::make(ErrorCode::InvalidArgument, "decoder set_prefix: created without prefix positions");
+    if (layer < 0 || layer >= cfg_.n_layers || n < 0 || n > prefix_max_ || !k || !v)
+      return Error::make(ErrorCode::InvalidArgument, "decoder set_prefix: layer or position count out of range");
+    UAII_CUDA(cudaSetDevice(be_->device()), "SetDevice");
+    UAII_TRY(put(prefix_[(size_t)layer], k, v, n));
+    prefix_len_ = n;
+    return Error::success();
+  }
+
+  // One step whose tokens are sampled from the logits (sample, one setting per sequence; device arrays).
+  Error step_sampled(const int32_t* tokens, const float* temperature, const int32_t* top_k, const float* top_p,
+                     const float* min_p, const float* u, int32_t* next, float* probs, float* logits) {
+    if (cfg_.vocab > kSampleMaxVocab)
+      return Error::make(ErrorCode::NotImplemented, "decoder step_sampled: vocab above " + std::to_string(kSampleMaxVocab));
+    bool device = !probs || is_device_ptr(probs);  // refused before the step, which would leave a position behind
+    for (const void* p : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p,
+                          (const void*)u, (const void*)next})
+      device = device && is_device_ptr(p);
+    if (!device)
+      return Error::make(ErrorCode::InvalidArgument, "decoder step_sampled: settings and next must be device memory");
+    UAII_TRY(step(tokens, logits, nullptr));
+    return be_->sample(logits_, false, cfg_.batch, cfg_.vocab, cfg_.vocab, temperature, top_k, top_p, min_p, u, next, probs,
+                       nullptr);
   }
 
   // One decode step at the current position for every sequence: tokens [batch] (host or
@@ -220,12 +287,16 @@ class Decoder {
         UAII_TRY(project_into(b.wk, b.wk_fmt, kv_dim_, q_dim_));
         UAII_TRY(project_into(b.wv, b.wv_fmt, kv_dim_, q_dim_ + kv_dim_));
       }
-      UAII_CUDA(launch_rope_append(qkv_, B, H, Hkv, hd, freq_, pos_, cfg_.rope_mode, q_, kc_[(size_t)l],
-                                   vc_[(size_t)l], cfg_.max_seq, st),
-                "rope_append");
-      UAII_CUDA(launch_attn_decode(maps_[(size_t)(2 * l)].bytes, maps_[(size_t)(2 * l + 1)].bytes, q_, B, H, Hkv, hd,
-                                   pos_ + 1, cfg_.max_seq, po_, pm_, pl_, attn_, err_, st),
-                "attention");
+      if (serve_fmt_) {
+        UAII_TRY(serve_attention(l));
+      } else {
+        UAII_CUDA(launch_rope_append(qkv_, B, H, Hkv, hd, freq_, pos_, cfg_.rope_mode, q_, kc_[(size_t)l],
+                                     vc_[(size_t)l], cfg_.max_seq, st),
+                  "rope_append");
+        UAII_CUDA(launch_attn_decode(maps_[(size_t)(2 * l)].bytes, maps_[(size_t)(2 * l + 1)].bytes, q_, B, H, Hkv, hd,
+                                     pos_ + 1, cfg_.max_seq, po_, pm_, pl_, attn_, err_, st),
+                  "attention");
+      }
       UAII_TRY(be_->quant_matmul(attn_, B, q_dim_, b.wo, b.wo_fmt, D, o_, false));
       UAII_CUDA(launch_add_rmsnorm(x_, o_, b.ffn_norm, B, D, cfg_.rms_eps, n_, st), "rmsnorm(ffn)");
       UAII_TRY(be_->ffn(b.moe, n_, B, ff_, nullptr));
@@ -233,7 +304,8 @@ class Decoder {
     UAII_CUDA(launch_add_rmsnorm(x_, ff_, out_norm_, B, D, cfg_.rms_eps, n_, st), "rmsnorm(out)");
     UAII_TRY(be_->quant_matmul(n_, B, D, output_, output_fmt_, cfg_.vocab, logits_, false));
     UAII_CUDA(launch_argmax(logits_, B, cfg_.vocab, next_, st), "argmax");
-    be_->add_launches(3 + 5 * (uint64_t)cfg_.n_layers);  // embed, per block 2 norms + rope + 2 attention, norm, argmax
+    // embed, per block 2 norms + rope (+ 2 attention; a serving decoder's operators count their own), norm, argmax
+    be_->add_launches(3 + (serve_fmt_ ? 3 : 5) * (uint64_t)cfg_.n_layers);
     if (logits)
       UAII_CUDA(cudaMemcpyAsync(logits, logits_, sizeof(float) * (size_t)(B * cfg_.vocab), cudaMemcpyDefault, st),
                 "Memcpy(logits)");
@@ -262,6 +334,69 @@ class Decoder {
   }
 
  private:
+  Error make_cache(KvCache* c, int64_t batch, int64_t max_seq) {
+    const size_t rows = (size_t)(batch * cfg_.n_kv_heads) * (size_t)max_seq, hd = (size_t)cfg_.head_dim;
+    const size_t bytes = rows * hd * (serve_fmt_ == kKvF16 ? 2 : 1);
+    c->fmt = serve_fmt_;
+    c->hd = (int)hd;
+    c->batch = batch;
+    c->heads = cfg_.n_kv_heads;
+    c->max_seq = max_seq;
+    UAII_CUDA(cudaMalloc(&c->k, bytes), "Malloc(K cache)");
+    UAII_CUDA(cudaMalloc(&c->v, bytes), "Malloc(V cache)");
+    UAII_CUDA(cudaMemsetAsync(c->k, 0, bytes, be_->stream()), "Memset(K cache)");
+    UAII_CUDA(cudaMemsetAsync(c->v, 0, bytes, be_->stream()), "Memset(V cache)");
+    if (serve_fmt_ == kKvF16) return Error::success();
+    for (float** s : {&c->k_scale, &c->v_scale}) {
+      UAII_CUDA(cudaMalloc(s, rows * sizeof(float)), "Malloc(row scales)");
+      UAII_CUDA(cudaMemsetAsync(*s, 0, rows * sizeof(float), be_->stream()), "Memset(row scales)");
+    }
+    return Error::success();
+  }
+
+  // Positions [0, n) of a cache from f32 [batch, kv_heads, n, head_dim] (host or device).
+  Error put(const KvCache& c, const float* k, const float* v, int64_t n) {
+    const int64_t hd = cfg_.head_dim;
+    const size_t bytes = sizeof(float) * (size_t)(c.batch * c.heads * n * hd);
+    if (bytes == 0) return Error::success();
+    cudaStream_t st = be_->stream();
+    char* tmp = nullptr;
+    UAII_CUDA(cudaMalloc(&tmp, 2 * bytes + sizeof(int32_t) * (size_t)c.batch), "Malloc(kv staging)");
+    auto run = [&]() -> Error {
+      UAII_CUDA(cudaMemcpyAsync(tmp, k, bytes, cudaMemcpyDefault, st), "Memcpy(k)");
+      UAII_CUDA(cudaMemcpyAsync(tmp + bytes, v, bytes, cudaMemcpyDefault, st), "Memcpy(v)");
+      int32_t* zeros = reinterpret_cast<int32_t*>(tmp + 2 * bytes);
+      UAII_CUDA(cudaMemsetAsync(zeros, 0, sizeof(int32_t) * (size_t)c.batch, st), "Memset(positions)");
+      UAII_TRY(be_->kv_append(c, tmp, tmp + bytes, false, n, RowView{c.heads * n * hd, hd, n * hd}, zeros, nullptr));
+      return cuda_status(cudaStreamSynchronize(st), "StreamSynchronize");
+    };
+    const Error e = run();
+    if (!e.ok()) (void)cudaStreamSynchronize(st);
+    (void)cudaFree(tmp);
+    return e;
+  }
+
+  // RoPE, the append and the attention of layer l: qkv_ -> attn_.
+  Error serve_attention(int64_t l) {
+    const int64_t B = cfg_.batch, H = cfg_.n_heads, Hkv = cfg_.n_kv_heads, hd = cfg_.head_dim;
+    const int64_t row = q_dim_ + 2 * kv_dim_;
+    UAII_CUDA(launch_rope_rows(qkv_, B, H, Hkv, hd, freq_, pos_, prefix_len_, cfg_.rope_mode, own_pos_, own_len_, be_->stream()),
+              "rope");
+    const KvCache& c = own_[(size_t)l];
+    UAII_TRY(be_->kv_append(c, qkv_ + q_dim_, qkv_ + q_dim_ + kv_dim_, false, 1, RowView{row, row, hd}, own_pos_, nullptr));
+    PrefixAttnArgs a;
+    a.own = c;
+    a.prefix = prefix_[(size_t)l];
+    a.prefix_len = prefix_len_;
+    a.own_len = own_len_;
+    a.q = qkv_;
+    a.T = 1;
+    a.H = H;
+    a.qs = RowView{row, row, hd};
+    a.out = attn_;
+    return be_->prefix_attention(a);
+  }
+
   Error project_into(const void* w, int fmt, int64_t rows, int64_t col0) {
     // the packed-MatMul writes [B, rows] densely: project into o_ scratch, then place the columns
     const int64_t B = cfg_.batch;
@@ -302,6 +437,10 @@ class Decoder {
   };
   std::vector<KvMap> maps_;  // TMA maps of each layer's K and V caches
   float *x_ = nullptr, *n_ = nullptr, *o_ = nullptr, *ff_ = nullptr, *qkv_ = nullptr, *q_ = nullptr, *attn_ = nullptr;
+  int serve_fmt_ = 0;  // a serving decoder's cache format
+  int64_t prefix_max_ = 0, prefix_len_ = 0;
+  std::vector<KvCache> own_, prefix_;  // of each layer
+  int32_t *own_pos_ = nullptr, *own_len_ = nullptr;
   float *po_ = nullptr, *pm_ = nullptr, *pl_ = nullptr, *logits_ = nullptr;
   int32_t *tokens_ = nullptr, *next_ = nullptr;
   int* err_ = nullptr;
@@ -330,6 +469,45 @@ int uaii_moe_decoder_create(uaii_moe_backend* b, const uaii_moe_decoder_config* 
   }
   *out = d;
   return report_status(Error::success());
+}
+
+int uaii_moe_decoder_create_serving(uaii_moe_backend* b, const uaii_moe_decoder_config* cfg, int kv_fmt, int64_t prefix_max,
+                                    const uaii_moe_decoder_block* blocks, const float* output_norm, const void* token_embd,
+                                    int embd_fmt, const void* output, int output_fmt, uaii_moe_decoder** out) {
+  try {
+    if (!b || !cfg || !out) return report_status(Error::make(ErrorCode::InvalidArgument, "decoder create: null argument"));
+    *out = nullptr;
+    if (kv_fmt == 0)
+      return report_status(Error::make(ErrorCode::NotImplemented, "decoder: cache format must be F16, KV_I8 or KV_E4M3"));
+    auto d = std::make_unique<uaii_moe_decoder>();
+    const Error e = d->impl.create(&b->impl, *cfg, blocks, output_norm, token_embd, embd_fmt, output, output_fmt, kv_fmt,
+                                   prefix_max);
+    if (!e.ok()) return report_status(e);
+    *out = d.release();
+    return report_status(Error::success());
+  } catch (const std::exception&) {
+    return UAII_MOE_INTERNAL;
+  }
+}
+
+int uaii_moe_decoder_set_prefix(uaii_moe_decoder* d, int64_t layer, const float* k, const float* v, int64_t n_pos) {
+  try {
+    if (!d) return report_status(Error::make(ErrorCode::InvalidArgument, "null decoder"));
+    return report_status(d->impl.set_prefix(layer, k, v, n_pos));
+  } catch (const std::exception&) {
+    return UAII_MOE_INTERNAL;
+  }
+}
+
+int uaii_moe_decoder_step_sampled(uaii_moe_decoder* d, const int32_t* tokens, const float* temperature, const int32_t* top_k,
+                                  const float* top_p, const float* min_p, const float* u, int32_t* next, float* probs,
+                                  float* logits) {
+  try {
+    if (!d) return report_status(Error::make(ErrorCode::InvalidArgument, "null decoder"));
+    return report_status(d->impl.step_sampled(tokens, temperature, top_k, top_p, min_p, u, next, probs, logits));
+  } catch (const std::exception&) {
+    return UAII_MOE_INTERNAL;
+  }
 }
 
 void uaii_moe_decoder_destroy(uaii_moe_decoder* d) { delete d; }

@@ -142,6 +142,10 @@ def _load():
                                     c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
         "uaii_moe_decoder_create": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int,
                                             POINTER(c_void_p)]),
+        "uaii_moe_decoder_create_serving": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int,
+                                                    c_void_p, c_int, POINTER(c_void_p)]),
+        "uaii_moe_decoder_set_prefix": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64]),
+        "uaii_moe_decoder_step_sampled": (c_int, [c_void_p] * 10),
         "uaii_moe_decoder_destroy": (None, [c_void_p]),
         "uaii_moe_decoder_set_kv": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64]),
         "uaii_moe_decoder_fill_kv": (c_int, [c_void_p, c_int64, c_uint64]),
@@ -176,6 +180,7 @@ EXPORTED = ("uaii_moe_abi_version", "uaii_moe_last_error", "uaii_moe_backend_cre
             "uaii_moe_packed_nbytes", "uaii_moe_quantize_rows",
             "uaii_moe_fill_normal", "uaii_moe_kv_append", "uaii_moe_kv_read", "uaii_moe_prefix_attention",
             "uaii_moe_sample", "uaii_moe_decoder_create", "uaii_moe_decoder_destroy",
+            "uaii_moe_decoder_create_serving", "uaii_moe_decoder_set_prefix", "uaii_moe_decoder_step_sampled",
             "uaii_moe_decoder_set_kv", "uaii_moe_decoder_fill_kv", "uaii_moe_decoder_step",
             "uaii_moe_decoder_generate", "uaii_moe_decoder_position", "uaii_moe_fill_normal_device",
             "uaii_moe_quantize_rows_device")
@@ -590,11 +595,12 @@ class Decoder:
     """Batched greedy decode of a GGUF MoE transformer on the device (uaii_moe_decoder_*).
 
     blocks: list of dicts with attn_norm, wq, wk, wv, wo (+ *_fmt), ffn_norm and moe (a Layer);
-    every array is device memory (torch CUDA tensors), kept alive by this object."""
+    every array is device memory (torch CUDA tensors), kept alive by this object.  kv_fmt (F16, KV_I8 or KV_E4M3)
+    makes a serving decoder, whose sequences may share a prefix of up to prefix_max positions."""
 
     def __init__(self, backend: "Backend", n_layers, d_model, n_heads, n_kv_heads, vocab, batch, max_seq, blocks,
                  output_norm, token_embd, embd_fmt, output=None, output_fmt=0, head_dim=128, rope_theta=1e6,
-                 rms_eps=1e-5, rope_mode=0):
+                 rms_eps=1e-5, rope_mode=0, kv_fmt=None, prefix_max=0):
         self._keep = [blocks, output_norm, token_embd, output]
         cfg = DecoderConfig(n_layers, d_model, n_heads, n_kv_heads, head_dim, vocab, batch, max_seq, rope_theta,
                             rms_eps, rope_mode)
@@ -604,8 +610,15 @@ class Decoder:
                                   ptr(b["wv"]), b["wv_fmt"], ptr(b["wo"]), b["wo_fmt"], ptr(b["ffn_norm"]), b["moe"])
         self._cfg, self._arr = cfg, arr
         h = c_void_p()
-        _check(lib.uaii_moe_decoder_create(backend.handle, ctypes.byref(cfg), arr, ptr(output_norm), ptr(token_embd),
-                                           embd_fmt, ptr(output), output_fmt, ctypes.byref(h)))
+        if kv_fmt is None:
+            if prefix_max:
+                raise ValueError("a shared prefix needs a serving decoder (kv_fmt)")
+            _check(lib.uaii_moe_decoder_create(backend.handle, ctypes.byref(cfg), arr, ptr(output_norm), ptr(token_embd),
+                                               embd_fmt, ptr(output), output_fmt, ctypes.byref(h)))
+        else:
+            _check(lib.uaii_moe_decoder_create_serving(backend.handle, ctypes.byref(cfg), kv_fmt, prefix_max, arr,
+                                                       ptr(output_norm), ptr(token_embd), embd_fmt, ptr(output), output_fmt,
+                                                       ctypes.byref(h)))
         self._h = h
         self.batch, self.vocab = batch, vocab
 
@@ -630,6 +643,19 @@ class Decoder:
 
     def fill_kv(self, n_pos: int, seed: int = 0):
         _check(lib.uaii_moe_decoder_fill_kv(self._h, n_pos, seed))
+
+    def set_prefix(self, layer: int, k, v, n_pos: int):
+        """The shared prefix of a serving decoder: f32 K, V [n_kv_heads, n_pos, head_dim], rotated already."""
+        _check(lib.uaii_moe_decoder_set_prefix(self._h, layer, ptr(k), ptr(v), n_pos))
+
+    def step_sampled(self, tokens, temperature, top_k, top_p, min_p, u, next_tokens, probs=None, logits=None):
+        """One step whose next tokens are sampled (Backend.sample's settings: CUDA tensors [batch])."""
+        T, b = _torch(), self.batch
+        f, i = T.float32, T.int32
+        _check(lib.uaii_moe_decoder_step_sampled(
+            self._h, ptr(tokens), _typed(temperature, "temperature", f, b), _typed(top_k, "top_k", i, b),
+            _typed(top_p, "top_p", f, b), _typed(min_p, "min_p", f, b), _typed(u, "u", f, b),
+            _typed(next_tokens, "next_tokens", i, b), None if probs is None else _typed(probs, "probs", f, b), ptr(logits)))
 
     def step(self, tokens, logits=None, next_tokens=None):
         _check(lib.uaii_moe_decoder_step(self._h, ptr(tokens), ptr(logits), ptr(next_tokens)))
