@@ -331,6 +331,31 @@ __device__ __forceinline__ void zero_v(uint8_t* v, int from, int to, int thread,
   umma::fence_proxy_async_smem();
 }
 
+// V of positions that only some of an item's tokens see: infinities and NaNs (which an 8-bit integer is not) become
+// zeros, since 0 times either would reach the tokens that do not see them, and the joining kernel gives them to those
+// that do.  Whether there was one, for the whole warp.
+template <int F, int HD, int KEYS>
+__device__ __noinline__ bool hide_v(uint8_t* v, int from, int to, int lane) {
+  using Gm = Tile<F, HD, KEYS>;
+  constexpr int kPer = Gm::kPart / 16;
+  bool any = false;
+  for (int i = lane; i < (to - from) * kPer * Gm::kBoxes; i += 32) {
+    const int box = i / ((to - from) * kPer), j = i % ((to - from) * kPer);
+    uint4* at = reinterpret_cast<uint4*>(v + box * Gm::kBoxBytes + (from + j / kPer) * Gm::kPart + (j % kPer) * 16);
+    uint4 x = *at;
+    bool bad = false;
+    for (uint32_t* w : {&x.x, &x.y, &x.z, &x.w}) {
+      const uint32_t m = F == kKvF16 ? __vcmpeq2(*w & 0x7c007c00u, 0x7c007c00u) : __vcmpeq4(*w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+      bad |= m != 0;
+      *w &= ~m;
+    }
+    if (bad) *at = x;
+    any |= bad;
+  }
+  umma::fence_proxy_async_smem();
+  return __any_sync(0xffffffffu, any);
+}
+
 // ---------------------------------------------------------------- narrow
 
 // Two or four consecutive elements of a query row as f32 (vec: one load).
@@ -504,6 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     }
     st.clear();
     const int end = min(x.t1 * KEYS, x.limit);
+    bool hidden = false;
 #pragma unroll 1
     for (int key = x.t0 * KEYS; key < end; key += KEYS) {
       copy();
@@ -516,6 +542,8 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
         zero_v<F, HD, KEYS>(stage + Tl::kBytes, left, KEYS, lane, 32);
         __syncwarp();
       }
+      if (F != kKvI8 && key + KEYS > x.fewest && x.fewest < x.limit)
+        hidden |= hide_v<F, HD, KEYS>(stage + Tl::kBytes, max(0, x.fewest - key), min(left, KEYS), lane);
       const float* ks = scales + s * (2 * KEYS);
       auto frag = [&](int step, uint32_t (&f)[4]) {
 #pragma unroll
@@ -531,7 +559,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
       st.store(part + (g + 8 * r) * HD, r);
-      if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], st.l[r]);
+      if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], hidden ? -st.l[r] : st.l[r]);
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // no grid of this call ends before the one it followed

@@ -4,7 +4,7 @@
 // tile's products while the other's exponentials are made.
 //   rows split   the item's 256 rows are the two tiles, and every key tile serves both (f16 queries, many rows)
 //   keys split   the item's 128 rows are both, and each takes every other key tile (f32 queries, whose leading parts and
-//                rests are two operands added into one acseqsulator; or up to 128 rows)
+//                rests are two operands added into one accumulator; or up to 128 rows)
 // Per key tile of 64: copied bytes -> (four warps) f16 operands in shared memory, K as [key][dim], V transposed to
 // [dim][key] -> S = Q K^T, Q from tensor memory -> (a thread per row) 2^(S - m), weights packed into the tensor memory
 // that held S -> O += P V, P from tensor memory.  Q and P in tensor memory leave shared memory's bandwidth to K and V:
@@ -43,6 +43,7 @@ struct WideShared {
   alignas(16) float kf[kOps][kTile];   // K scale * softmax scale * log2(e)
   alignas(16) float vf[kOps][kTile];   // V scale * 2 / vtop: below 2
   float vtop[kOps];
+  alignas(4) uint8_t hidden[kOps][4];  // by the converting warps: V values that not all rows see were left out
   SeqTables seqs;
 };
 
@@ -142,11 +143,19 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
         }
       }
       // V transposed: 8-bit pieces hold 16 dimensions, whose even ones become rows 16 c .. 16 c + 7 and odd ones the next
-      // eight.  Nothing is stored past the item's last position: zeros, since 0 * NaN would not be 0.
+      // eight.  Nothing is stored past the item's last position: zeros, since 0 * NaN would not be 0.  Nor may an infinity
+      // or a NaN that only some of the item's tokens see meet the zero weights of the others: a zero instead, and the
+      // joining kernel gives it to those that see it.
       auto v_to = [&](int row) { return ov + row * 128 + (((2 * cw + (mi & 1)) ^ (row & 7)) << 4); };
+      const int all_see = x.fewest < x.limit ? x.fewest - (x.t0 + i) * kTile : left;
+      const bool end = F != kKvI8 && all_see < kTile;
+      bool hidden = false;
       auto keep = [&](uint32_t pair, int key) {
-        if (key + 1 < left) return pair;
-        return key < left ? pair & 0xffffu : 0u;
+        pair &= key + 1 < left ? ~0u : key < left ? 0xffffu : 0u;
+        uint32_t m = __vcmpeq2(pair & 0x7c007c00u, 0x7c007c00u);
+        m &= key >= all_see ? ~0u : key + 1 >= all_see ? ~0xffffu : 0u;
+        hidden |= m != 0;
+        return pair & ~m;
       };
 #pragma unroll
       for (int c = 0; c < kPieces; c += 2) {
@@ -154,7 +163,7 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
         ldsm4t(v, piece<F, HD, kTile>(rv, 16 * cw + 8 * (mi & 1) + r8, c + (mi >> 1)));
         const int lo = 16 * cw + 2 * tq, hi = lo + 8;
         if constexpr (F == kKvF16) {
-          if (left < kTile) {
+          if (end) {
             v[0] = keep(v[0], lo); v[1] = keep(v[1], hi);
             v[2] = keep(v[2], lo); v[3] = keep(v[3], hi);
           }
@@ -165,7 +174,7 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
             uint32_t e0, d0, e1, d1;
             unpack<F, true>(v[2 * j], e0, d0);
             unpack<F, true>(v[2 * j + 1], e1, d1);
-            if (F == kKvE4M3 && left < kTile) {
+            if (end) {
               e0 = keep(e0, lo); d0 = keep(d0, lo);
               e1 = keep(e1, hi); d1 = keep(d1, hi);
             }
@@ -196,9 +205,11 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
           if (lane == 0) sh.vtop[o] = vtop;
         }
       }
+      if constexpr (F != kKvI8) hidden = __any_sync(0xffffffffu, hidden);
       umma::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
+        if constexpr (F != kKvI8) sh.hidden[o][cw] = hidden;
         umma::mbar_arrive(&sh.raw_empty[s]);
         umma::mbar_arrive(&sh.op_full[o]);
       }
@@ -335,6 +346,13 @@ __device__ __forceinline__ int operand_dim(int pos) {
   return (pos & ~15) | ((pos & 6) << 1) | ((pos & 8) >> 2) | (pos & 1);
 }
 
+// y rounded towards zero, but to the smallest half of s's sign rather than to 0 unless s is 0.
+__device__ __forceinline__ __half toward_zero(float y, float s) {
+  const __half h = __float2half_rz(y);
+  return __hisnan(h) || (__half_as_ushort(h) & 0x7fff) || s == 0.f ? h : __ushort_as_half(s < 0.f ? 0x8001 : 1);
+}
+__device__ __forceinline__ __half toward_zero(float y) { return toward_zero(y, y); }
+
 // This thread's row of q (null: zeros) into tensor memory as operand `part` (1: the rests of a split); returns the power
 // of two by which a split row was multiplied.
 template <int F, int HD, bool SPLIT_Q, typename Q>
@@ -378,7 +396,15 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
       const int d = operand_dim<F>(2 * j);
       const float y0 = (float)v.e[d] * shrink, y1 = (float)v.e[d + 1] * shrink;
       __half2 e = __floats2half2_rn(y0, y1);
-      if (SPLIT_Q && part) {
+      if constexpr (SPLIT_Q && F == kKvF16) {
+        // K may hold infinities: both parts have the value's sign, and neither is 0 (their products would be NaN)
+        // unless the value is.  Rounded towards zero they still leave no more than 2^-22 of the largest.
+        e = __halves2half2(toward_zero(y0), toward_zero(y1));
+        if (part) {
+          const float2 z = __half22float2(e);
+          e = __halves2half2(toward_zero(y0 - z.x, y0), toward_zero(y1 - z.y, y1));
+        }
+      } else if (SPLIT_Q && part) {
         const float2 z = __half22float2(e);
         e = __floats2half2_rn(y0 - z.x, y1 - z.y);
       }
@@ -405,6 +431,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
     int lim;
     const Q* src = q_row<Q>(a, p, x, p.split_keys ? row : 128 * r + row, lim);
     float m = -INFINITY, l = 0.f, row_f = 1.f, vtop = 0x1p-100f;
+    uint32_t hidden = 0;
     if (n > 0) {
       if (p.split_keys) asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's products with q are done
       const float shrink = put_q<F, HD, SPLIT_Q, Q>(src, a.q_vec, r, tm + 128 + 64 * r);
@@ -482,6 +509,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
           if (slow) load();  // S is still in tensor memory
         }
         if (slow) {
+          if constexpr (F != kKvI8) hidden |= *reinterpret_cast<const uint32_t*>(sh.hidden[o]);
           float top = -INFINITY;
 #pragma unroll
           for (int j = 0; j < kHalf; ++j) {
@@ -529,7 +557,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
     count += n > 0 ? n : 0;
     const int64_t at = x.slot * 256 + 128 * r + row;
     float* part = p.part + at * HD;
-    *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m, l);
+    *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m, hidden ? -l : l);
     if (n > first) {
       umma::bounded_wait(&sh.o_done[r][1], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
       umma::tc_fence_after();

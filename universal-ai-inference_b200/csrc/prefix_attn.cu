@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
   for (int d = 16; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
   const float safe = mx == -INFINITY ? 0.f : mx;
   float l = 0.f, o[N] = {};
+  bool hidden = false;  // the sign of a piece's l: it left out infinities or NaNs of V
   auto add = [&](const Pieces& s) {
 #pragma unroll 4
     for (int k = wr; k < s.n; k += WARPS) {
@@ -120,7 +121,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
       if constexpr (N == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(s.part + r * HD + N * lane);
       else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(s.part + r * HD + N * lane);
       const float f = ex2(ml.x - safe);
-      l = fmaf(f, ml.y, l);
+      l = fmaf(f, fabsf(ml.y), l);
+      hidden |= signbit(ml.y);
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] = fmaf(f, y[i], o[i]);
     }
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
 #pragma unroll
     for (int i = 0; i < N; ++i) all[wr][N * lane + i] = o[i];
     if (lane == 0) all[wr][HD] = l;
-    __syncthreads();
+    hidden = __syncthreads_or(hidden);
     if (wr != 0) return;
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) {
@@ -142,6 +144,20 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
     }
   }
   if (!live) return;
+  if (hidden) {  // positions that the item's first token does not see and this one does
+    const int seen = own_length(a, b, false) - (int)a.T + 1, first = (t * po.G + g) / po.rt * po.rt / po.G;
+    const int64_t plane = ((int64_t)b * a.own.heads + kvh) * a.own.max_seq;
+    for (int pos = max(0, seen + first); pos < seen + t; ++pos) {
+      const int64_t at = (plane + pos) * HD + N * lane;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float v;
+        if (a.own.fmt == kKvF16) v = __half2float(static_cast<const __half*>(a.own.v)[at + i]);
+        else v = (static_cast<const uint8_t*>(a.own.v)[at + i] & 0x7f) == 0x7f ? NAN : 0.f;
+        if (!isfinite(v)) o[i] += v;
+      }
+    }
+  }
   Q y[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) y[i] = (Q)(l == 0.f ? 0.f : __fdiv_rn(o[i], l));
