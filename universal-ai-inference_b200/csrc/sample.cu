@@ -16,6 +16,7 @@
 // (about 30 instructions a logit, once each), a single row by the dozen cluster barriers on its way.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 #include "serve_kernels.hpp"
 
@@ -29,13 +30,14 @@ constexpr uint32_t kOne = 1u << 31;  // the weight of the largest logit
 __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const __half* p) { return __half2float(*p); }
 
-// A NaN counts as -inf, and both zeros are one.
-__device__ __forceinline__ float canonical(float x) { return x != x ? -INFINITY : x + 0.0f; }
+// A NaN counts as -inf (the maximum of a NaN and a number is the number), and both zeros are one.
+__device__ __forceinline__ float canonical(float x) { return fmaxf(x, -INFINITY) + 0.0f; }
 // Ordered bits of a canonical logit: larger keys for larger logits.
-__device__ __forceinline__ uint32_t key_of_logit(float x) {
-  const uint32_t b = __float_as_uint(canonical(x));
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(x);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ uint32_t key_of_logit(float x) { return key_of(canonical(x)); }
 __device__ __forceinline__ float logit_of_key(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
@@ -57,13 +59,17 @@ struct Heat {
     const float a = __fsub_rn(x, m);
     return expf(plain ? quotient(a, __fmul_rn(a, r)) : __fdiv_rn(a, h));
   }
-  // The weight; 0 without an exponential where that is below 2^-32 (e^-23) by far.
-  __device__ __forceinline__ uint32_t weight_of(float x) const {
-    const float a = __fsub_rn(x, m), q = __fmul_rn(a, r);
-    if (plain && q < -24.0f) return 0;
-    if (x == m) return kOne;
-    return weight(expf(plain ? quotient(a, q) : __fdiv_rn(a, h)));
+  // The weight.  In the plain range without a branch; below e^-24 it is 0, whatever the exponential of the product.
+  template <bool PLAIN>
+  __device__ __forceinline__ uint32_t weight_in(float x) const {
+    if constexpr (PLAIN) {
+      const float a = __fsub_rn(x, m), q = __fmul_rn(a, r);
+      const uint32_t y = weight(expf(quotient(a, q)));
+      return x == m ? kOne : q < -24.0f ? 0 : y;
+    }
+    return weight(exp_of(x));
   }
+  __device__ __forceinline__ uint32_t weight_of(float x) const { return plain ? weight_in<true>(x) : weight_in<false>(x); }
 };
 
 // One row's settings.
@@ -101,21 +107,20 @@ __device__ __forceinline__ uint64_t reach_of(float p, uint64_t mass) {  // at le
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 512, kList = 1024, kMaxCluster = 8;
 constexpr int kGroups = kThreads / (kBins / 2);         // threads that read the same bins, of different CTAs
-constexpr int kFixed = (2 + kGroups) * kBins * 8 + 3 * kList * 4;  // dynamic shared memory besides the weights
+constexpr int kFixed = (2 + kGroups) * kBins * 8 + 2 * kList * 4;  // dynamic shared memory besides the weights
 constexpr int kMaxSlice = (int)(kSampleMaxVocab / kMaxCluster);  // weights of a CTA
+static_assert(kList <= kGroups * kBins, "the lists of all CTAs take the place of the sums");
 static_assert(kFixed + 4 * kMaxSlice <= 225 * 1024, "a CTA's shared memory");
 
-// Leading bits of a weight: its exponent and four bits more (monotone; 0 for 0).
-__device__ __forceinline__ int bin_of(uint32_t w) {
-  if (w == 0) return 0;
-  const int e = 31 - __clz(w);
-  return e * 16 + (int)((w << (31 - e)) >> 27 & 15u);
-}
+// Leading bits of a weight above 0: its exponent and four bits more, as f32 has them.
+__device__ __forceinline__ int bin_of(uint32_t w) { return (int)(__float_as_uint(__uint2float_rz(w)) >> 19) - 127 * 16; }
 
-struct Found {        // a cut: weights above `w` are kept, and `need` of those that equal it
+struct Found {        // a cut: weights above `w` are kept, and `need` of the `equal` ones at it
   uint32_t w;
-  uint64_t above;     // count or mass above w
   uint64_t need, equal;
+  bool ranked;        // those whose logit is above `edge`, and the first `ties` with that logit; else it is to be found
+  uint32_t edge;
+  uint64_t ties;
 };
 
 struct RowShared {
@@ -131,16 +136,21 @@ enum Purpose { kTop, kMass, kSome, kHead, kTail };
 
 // What the CTAs of a cluster add up is read by each of them for itself, so that one cluster barrier is enough: bins and
 // lists come in two sets, used in turn, and a set is written again only after the barrier of the other's use.
+template <typename X>
 struct Row {
   cg::cluster_group cluster;
   RowShared& sh;
   uint32_t* w;          // this CTA's weights, in index order; zeros up to a multiple of four
-  uint2* bins;          // [2][kBins]: a bin's sum of low halves and of high halves (32-bit atomics are native)
+  uint32_t* bins;       // [2][2 kBins]: a bin's sums of low and of high halves (32-bit atomics are native)
   uint64_t* sums;       // [kGroups][kBins]
-  uint32_t* list;       // [2][kList] of this CTA, and [kList] of all
+  uint32_t* list;       // [2][kList] indices of this CTA's tokens
+  uint2* all;           // [kList] weights and keys of the tokens that all CTAs listed
+  const X* x;           // the row's logits
+  int slice;            // of which a CTA has so many
   int quads;            // fours of weights of this CTA
   int rank, ctas;
   int set;
+  Heat heat;
 
   template <typename F>
   __device__ __forceinline__ void each4(F&& f) const {  // f(index, weight) in fours, whole CTA
@@ -164,13 +174,16 @@ struct Row {
     for (int i = 0; i < ctas; ++i) t += sh.part[p][i];
     return t;
   }
-  __device__ __forceinline__ uint2* next_bins() {
+  __device__ __forceinline__ uint32_t* next_bins() {
     set ^= 1;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) bins[set * kBins + i] = make_uint2(0, 0);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) reinterpret_cast<uint2*>(bins + 2 * set * kBins)[i] = make_uint2(0, 0);
     if (threadIdx.x == 0) sh.listed[set] = 0;
     __syncthreads();
-    return bins + set * kBins;
+    return bins + 2 * set * kBins;
   }
+  // Where a bin's low sum lies (the high one beside it, at ^ 1): every other sixteen bins the other way round, so that
+  // low sums fall into all banks.
+  static __device__ __forceinline__ int low_at(int bin) { return 2 * bin + (bin >> 4 & 1); }
   // The bin, from the highest down, at which the cluster's bins reach `goal`: sh.bin and sh.above (plus `above`).  Remote
   // shared memory gave 4 to 5 bytes a cycle to an SM, so bins are read in 512-byte pieces and are no more than
   // 512: 1024 took 4 us more, 256 left longer lists to rank (381 against 341 us at 256 rows of 151936).
@@ -182,13 +195,14 @@ struct Row {
     for (int k = 0; k < kEach; ++k) {
       y[k] = make_uint4(0, 0, 0, 0);
       const int c = k * kGroups + group;
-      if (c < ctas) y[k] = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins + set * kBins, c))[at];
+      if (c < ctas) y[k] = reinterpret_cast<const uint4*>(cluster.map_shared_rank(bins + 2 * set * kBins, c))[at];
     }
     uint64_t two[2] = {};
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-      two[0] += y[k].x + ((uint64_t)y[k].y << 16);
-      two[1] += y[k].z + ((uint64_t)y[k].w << 16);
+      const bool turned = at & 8;
+      two[0] += (turned ? y[k].y : y[k].x) + ((uint64_t)(turned ? y[k].x : y[k].y) << 16);
+      two[1] += (turned ? y[k].w : y[k].z) + ((uint64_t)(turned ? y[k].z : y[k].w) << 16);
     }
     sums[group * kBins + 2 * at] = two[0];
     sums[group * kBins + 2 * at + 1] = two[1];
@@ -213,12 +227,13 @@ struct Row {
     __syncthreads();
   }
 
-  __device__ __forceinline__ void put(uint32_t x) {  // into this CTA's list
+  __device__ __forceinline__ void put(uint32_t i) {  // token i of this CTA into its list
     const uint32_t k = atomicAdd(&sh.listed[set], 1u);
-    if (k < kList) list[set * kList + k] = x;
+    if (k < kList) list[set * kList + k] = i;
   }
-  // Of the numbers that the CTAs have listed, the one at which the leading ones reach `goal`, `above` lying above them
-  // all.  False, with their count in f->equal, if they are more than a list holds.
+  // Of the tokens that the CTAs have listed, ranked by their logits (and so by weight), the cut at which the leading
+  // ones reach `goal`, `above` lying above them all.  False, with their count in f->equal, if they are more than a list
+  // holds.  Their logits are read again: they tell equal weights apart.
   template <bool MASS>
   __device__ bool rank_listed(uint64_t goal, uint64_t above, Found* f) {
     const int t = threadIdx.x;
@@ -230,7 +245,6 @@ struct Row {
     for (int c = 0; c < kMaxCluster; ++c) listed += count[c];
     f->equal = listed;
     if (listed > kList) return false;
-    uint32_t* all = list + 2 * kList;
     for (uint32_t i = t; i < listed; i += kThreads) {
       uint32_t j = i;
       int c = 0;
@@ -240,21 +254,26 @@ struct Row {
           j -= count[k];
           c = k + 1;
         }
-      all[i] = cluster.map_shared_rank(list + set * kList, c)[j];
+      const float y = canonical(logit(x + (int64_t)c * slice + cluster.map_shared_rank(list + set * kList, c)[j]));
+      all[i] = make_uint2(heat.weight_of(y), key_of_logit(y));
     }
     __syncthreads();
     for (uint32_t i = t; i < listed; i += kThreads) {
-      const uint32_t x = all[i];
+      const uint2 me = all[i];
       uint64_t over = above;
-      uint32_t equal = 0;
+      uint32_t same = 0, equal = 0, before = 0;  // of the same logit; of the same weight, and those with a larger logit
       for (uint32_t j = 0; j < listed; ++j) {
-        const uint32_t y = all[j];
-        over += y > x ? (MASS ? y : 1u) : 0u;
-        equal += y == x;
+        const uint2 y = all[j];
+        over += y.y > me.y ? (MASS ? y.x : 1u) : 0u;
+        same += y.y == me.y;
+        equal += y.x == me.x;
+        before += y.x == me.x && y.y > me.y;
       }
-      const uint64_t each = MASS ? x : 1;
-      if (over < goal && goal <= over + equal * each)  // (the same numbers write the same)
-        sh.found = Found{x, over, (goal - over + each - 1) / each, equal};
+      const uint64_t each = MASS ? me.x : 1;
+      if (over < goal && goal <= over + same * each) {  // (equal tokens write the same)
+        const uint64_t ties = (goal - over + each - 1) / each;
+        sh.found = Found{me.x, before + ties, equal, true, me.y, ties};
+      }
     }
     __syncthreads();
     *f = sh.found;
@@ -271,18 +290,23 @@ struct Row {
     int shift = -1;
     uint64_t above = 0;
     for (;;) {
-      uint2* mine = next_bins();
-      each4([&](int, uint4 v) {
-        if (max(max(v.x, v.y), max(v.z, v.w)) < lo) return;
-        const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+      uint32_t* mine = next_bins();
+      auto bin = [&](auto&& of) {
+        each4([&](int, uint4 v) {
+          if (max(max(v.x, v.y), max(v.z, v.w)) < lo) return;
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (x[j] >= lo && x[j] <= hi) {  // (50000 halves of 16 bits add up to less than 2^32)
-            uint2* to = &mine[shift < 0 ? bin_of(x[j]) : (int)((x[j] - lo) >> shift)];
-            atomicAdd(&to->x, MASS ? x[j] & 0xffffu : 1u);
-            if (MASS) atomicAdd(&to->y, x[j] >> 16);
+          for (int j = 0; j < 4; ++j) {
+            const int to = low_at(of(x[j]));
+            if (x[j] >= lo && x[j] <= hi) {  // (50000 halves of 16 bits add up to less than 2^32)
+              atomicAdd(mine + to, MASS ? x[j] & 0xffffu : 1u);
+              if (MASS) atomicAdd(mine + (to ^ 1), x[j] >> 16);
+            }
           }
-      });
+        });
+      };
+      if (shift < 0) bin([](uint32_t y) { return bin_of(y); });
+      else bin([&](uint32_t y) { return (int)((y - lo) >> shift); });
       cluster.sync();
       reach(goal, above);
       const int at = sh.bin;
@@ -299,16 +323,16 @@ struct Row {
       from = max(from, lo);
       to = min(to, hi);
       // the bin's weights
-      each4([&](int, uint4 v) {
+      each4([&](int i, uint4 v) {
         if (max(max(v.x, v.y), max(v.z, v.w)) < from) return;
         const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (x[j] >= from && x[j] <= to) put(x[j]);
+          if (x[j] >= from && x[j] <= to) put(i + j);
       });
       Found f;
       if (rank_listed<MASS>(goal, above, &f)) return f;
-      if (from == to) return Found{from, above, MASS ? (goal - above + from - 1) / from : goal - above, f.equal};
+      if (from == to) return Found{from, MASS ? (goal - above + from - 1) / from : goal - above, f.equal, false, 0, 0};
       lo = from;
       hi = to;
       const int bits = 32 - __clz(to - from);
@@ -331,18 +355,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t b = blockIdx.x / ctas, begin = (int64_t)rank * slice;
   const int n = (int)max(int64_t(0), min((int64_t)slice, V - begin));
-  uint2* bins = reinterpret_cast<uint2*>(dynamic);
-  uint64_t* sums = reinterpret_cast<uint64_t*>(bins + 2 * kBins);
+  uint32_t* bins = reinterpret_cast<uint32_t*>(dynamic);
+  uint64_t* sums = reinterpret_cast<uint64_t*>(bins + 4 * kBins);
+  uint2* all = reinterpret_cast<uint2*>(sums);  // the one in use while the other is not
   uint32_t* list = reinterpret_cast<uint32_t*>(sums + kGroups * kBins);
-  uint32_t* w = list + 3 * kList;
-  Row row{cluster, sh, w, bins, sums, list, (n + 3) / 4, rank, ctas, 0};
+  uint32_t* w = list + 2 * kList;
   const X* x = logits + b * ld + begin;
+  Row<X> row{cluster, sh, w, bins, sums, list, all, logits + b * ld, slice, (n + 3) / 4, rank, ctas, 0, {}};
   const Setting s = setting_of(b, temperature, top_k, top_p, min_p, u);
 
   // the logits, read once, and their largest
-  uint32_t top = 0;
+  float most = -INFINITY;
   constexpr int kVec = 16 / sizeof(X);
   const int whole = vec ? n / kVec * kVec : 0;
+#pragma unroll 4
   for (int i = t * kVec; i < whole; i += kThreads * kVec) {
     X v[kVec];
     *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(x + i));
@@ -350,17 +376,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       f[j] = canonical((float)v[j]);
-      top = max(top, key_of_logit(f[j]));
+      most = fmaxf(most, f[j]);
     }
 #pragma unroll
     for (int j = 0; j < kVec; j += 4) *reinterpret_cast<float4*>(w + i + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
   }
   for (int i = whole + t; i < n; i += kThreads) {
     const float f = canonical(logit(x + i));
-    top = max(top, key_of_logit(f));
+    most = fmaxf(most, f);
     w[i] = __float_as_uint(f);
   }
   if (n + t < 4 * row.quads) w[n + t] = 0xff800000u;  // -inf
+  uint32_t top = key_of(most);
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) sh.warp[warp] = top;
   __syncthreads();
@@ -379,16 +406,20 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   }
 
   // weights in place of the logits
-  const Heat heat{m, s.heat, __fdiv_rn(1.0f, s.heat), s.heat >= 0x1p-30f && s.heat <= 0x1p30f};
+  const Heat heat = row.heat = {m, s.heat, __fdiv_rn(1.0f, s.heat), s.heat >= 0x1p-30f && s.heat <= 0x1p30f};
   uint64_t mass = 0;
   uint32_t some = 0;
-  row.each4([&](int i, uint4 v) {
-    const uint4 y = {heat.weight_of(__uint_as_float(v.x)), heat.weight_of(__uint_as_float(v.y)),
-                     heat.weight_of(__uint_as_float(v.z)), heat.weight_of(__uint_as_float(v.w))};
-    *reinterpret_cast<uint4*>(w + i) = y;
-    mass += ((uint64_t)y.x + y.y) + ((uint64_t)y.z + y.w);
-    some += (y.x != 0) + (y.y != 0) + (y.z != 0) + (y.w != 0);
-  });
+  auto weigh = [&](auto plain) {
+    row.each4([&](int i, uint4 v) {
+      const uint4 y = {heat.template weight_in<plain.value>(__uint_as_float(v.x)), heat.template weight_in<plain.value>(__uint_as_float(v.y)),
+                       heat.template weight_in<plain.value>(__uint_as_float(v.z)), heat.template weight_in<plain.value>(__uint_as_float(v.w))};
+      *reinterpret_cast<uint4*>(w + i) = y;
+      mass += ((uint64_t)y.x + y.y) + ((uint64_t)y.z + y.w);
+      some += (y.x != 0) + (y.y != 0) + (y.z != 0) + (y.w != 0);
+    });
+  };
+  if (heat.plain) weigh(std::true_type{});
+  else weigh(std::false_type{});
   mass = row.block_sum(mass);
   some = (uint32_t)row.block_sum(some);
   row.tell(kMass, mass);
@@ -398,12 +429,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   const uint64_t positive = row.sum_of(kSome);
 
   // the cut: none (w 0), or weights above cut.w and `need` of the `equal` ones at it
-  Found cut{0, 0, 0, 0};
+  Found cut{};
   const bool by_count = s.k > 0 && s.k < V;
   if (s.k == 1) {
-    cut = Found{kOne, 0, 1, 2};  // whether there is another does not matter
+    cut = Found{kOne, 1, 2, true, top, 1};  // the first of the largest
   } else if (by_count && (uint64_t)s.k < positive) {
-    cut = row.find<false>((uint64_t)s.k, 0);
+    cut = row.template find<false>((uint64_t)s.k, 0);
   }
   if (!(s.p >= 1.0f) && s.k != 1) {
     uint64_t z = mass;
@@ -418,38 +449,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
     }
     const uint64_t goal = reach_of(s.p, z);
     // Weights below (z - goal) / V add up to less than z - goal: the goal is reached above them.
-    cut = row.find<true>(goal, (uint32_t)max((z - goal) / (uint64_t)V, (uint64_t)cut.w));
+    cut = row.template find<true>(goal, (uint32_t)max((z - goal) / (uint64_t)V, (uint64_t)cut.w));
   }
-  // of the weights at the cut: those whose logit is above `edge`, and the first `ties` with that logit
-  uint32_t edge = 0;
-  uint64_t ties = 0;
   const bool partial = cut.w != 0 && cut.need < cut.equal;
-  if (s.k == 1) {  // the first of the largest
-    edge = top;
-    ties = 1;
-  } else if (partial && cut.equal <= kList) {  // their logits, read again
-    (void)row.next_bins();
-    row.each4([&](int i, uint4 v) {
-      const uint32_t y[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (y[j] == cut.w) row.put(key_of_logit(logit(x + i + j)));
-    });
-    Found f;
-    (void)row.rank_listed<false>(cut.need, 0, &f);
-    edge = f.w;
-    ties = f.need;
-  } else if (partial) {  // eight bits of the keys at a time
+  uint32_t edge = cut.edge;
+  uint64_t ties = cut.ties;
+  if (partial && !cut.ranked) {  // more equal weights than a list holds: eight bits of their keys at a time
     uint64_t need = cut.need;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      uint2* mine = row.next_bins();
+      uint32_t* mine = row.next_bins();
       row.each4([&](int i, uint4 v) {
         const uint32_t y[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (y[j] != cut.w) continue;
           const uint32_t k = key_of_logit(logit(x + i + j));
-          if (shift == 24 || (k >> (shift + 8)) == (edge >> (shift + 8))) atomicAdd(&mine[(k >> shift) & 255].x, 1u);
+          if (shift == 24 || (k >> (shift + 8)) == (edge >> (shift + 8))) atomicAdd(mine + row.low_at((k >> shift) & 255), 1u);
         }
       });
       cluster.sync();
@@ -476,18 +491,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   // masses and ties of each warp's run of indices, four of them a lane
   const uint32_t low = max(cut.w, w_least);
   const int run = (row.quads + kWarps - 1) / kWarps, q0 = min(row.quads, run * warp), q1 = min(row.quads, q0 + run);
+  const bool cuts = cut.w != 0 || least > 0.f;
   uint64_t seg_mass = 0;
   uint32_t seg_ties = 0, seg_count = 0;
   for (int q = q0 + lane; q < q1; q += 32) {
     const uint4 v = reinterpret_cast<const uint4*>(w)[q];
-    if (max(max(v.x, v.y), max(v.z, v.w)) < low) continue;
+    // above both cuts a token is kept, at one of them it takes a look (without a cut none does: zeros have no mass)
+    bool look = false;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t y = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
-      const int f = side(4 * q + j, y);
-      seg_mass += f == 1 ? y : 0;
-      seg_count += f == 1;
-      seg_ties += f == 2;
+      seg_mass += y > low ? y : 0;
+      seg_count += y > low;
+      look |= y == low;
+    }
+    if (look && cuts) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t y = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+        if (y != low) continue;
+        const int f = side(4 * q + j, y);
+        seg_mass += f == 1 ? y : 0;
+        seg_count += f == 1;
+        seg_ties += f == 2;
+      }
     }
   }
   for (int o = 16; o > 0; o >>= 1) seg_mass += __shfl_xor_sync(0xffffffffu, seg_mass, o);
@@ -531,45 +558,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   }
   const uint64_t mine = sh.segment[warp] + (min(ties_before + sh.ties[warp], ties) - min(ties_before, ties)) * cut.w;
   if (before <= goal && goal < before + mine) {  // this warp's run holds the token
-    for (int q = q0; q < q1; q += 32) {
-      uint64_t add[4] = {}, sum = 0;
-      int f[4] = {}, edges = 0;
-      if (q + lane < q1) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[j] = side(4 * (q + lane) + j, w[4 * (q + lane) + j]);
-          edges += f[j] == 2;
-        }
-      }
-      int upto = edges;
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
-      }
-      uint64_t tie = ties_before + upto - edges;
+    // a lane's part of it: a few fours in a row
+    const int each = (q1 - q0 + 31) / 32, l0 = min(q1, q0 + each * lane), l1 = min(q1, l0 + each);
+    uint64_t sum = 0;
+    uint32_t edges = 0;
+    for (int q = l0; q < l1; ++q) {
+      const uint4 v = reinterpret_cast<const uint4*>(w)[q];
+      if (max(max(v.x, v.y), max(v.z, v.w)) < low) continue;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (f[j] == 1) add[j] = w[4 * (q + lane) + j];
-        if (f[j] == 2) add[j] = tie++ < ties ? cut.w : 0;
-        sum += add[j];
+        const uint32_t y = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+        const int f = side(4 * q + j, y);
+        sum += f == 1 ? y : 0;
+        edges += f == 2;
       }
-      uint64_t inc = sum;
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      uint64_t at = before + inc - sum;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (goal >= at && goal < at + add[j]) {
-          tokens[b] = (int32_t)(begin + 4 * (q + lane) + j);
-          if (probs) probs[b] = (float)((double)add[j] / (double)total);
+    }
+    uint64_t inc = edges;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    ties_before += inc - edges;
+    sum += (min(ties_before + edges, ties) - min(ties_before, ties)) * cut.w;
+    inc = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    before += inc - sum;
+    if (before <= goal && goal < before + sum) {
+      for (int q = 4 * l0; before <= goal; ++q) {
+        const int f = side(q, w[q]);
+        const uint64_t add = f == 1 ? w[q] : f == 2 && ties_before++ < ties ? cut.w : 0;
+        before += add;
+        if (before > goal) {
+          tokens[b] = (int32_t)(begin + q);
+          if (probs) probs[b] = (float)((double)add / (double)total);
         }
-        at += add[j];
       }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-      ties_before += __shfl_sync(0xffffffffu, upto, 31);
-      if (before > goal) break;
     }
   }
 }
