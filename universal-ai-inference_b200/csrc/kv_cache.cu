@@ -12,6 +12,7 @@
 // Both kernels are bound by the bytes they move: one pass, 16-byte accesses, nothing kept between rows.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "serve_kernels.hpp"
 
@@ -19,7 +20,7 @@ namespace uaii_b200 {
 namespace {
 
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
-constexpr int kRows = 2;  // rows of a thread, loaded together
+constexpr int kRows = 2, kReadRows = 4;  // rows of a thread, loaded together
 
 __device__ __forceinline__ void load8(const float* p, bool vec, float (&x)[8]) {
   if (vec) {
@@ -66,14 +67,19 @@ __device__ __forceinline__ float store_row8(const float (&x)[8], void* row, int 
     uint32_t w[2];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      uint32_t b[4];
+      float y[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = fine ? __fmul_rn(x[4 * p + i], inv) : 0.f;
-        if constexpr (F == kKvI8) b[i] = (uint32_t)(__float2int_rn(y) + 128);
-        else b[i] = __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+      for (int i = 0; i < 4; ++i) y[i] = fine ? __fmul_rn(x[4 * p + i], inv) : 0.f;
+      if constexpr (F == kKvI8) {  // added to 3 * 2^22 + 128, a number rounds to a whole one whose low byte is the code
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(__fadd_rn(y[i], 12583040.0f));
+        w[p] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+      } else {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+        w[p] = lo | (hi << 16);
       }
-      w[p] = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
     }
     if (row) reinterpret_cast<uint2*>(row)[lane8] = make_uint2(w[0], w[1]);
     return a >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fine ? __fdiv_rn(amax, top) : 0.f;
@@ -85,8 +91,9 @@ __device__ __forceinline__ float store_row8(const float (&x)[8], void* row, int 
 template <int F, int HD, typename X>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __restrict__ k, const X* __restrict__ v,
                                                         int T, RowView s, const int32_t* __restrict__ pos,
-                                                        const int32_t* __restrict__ n_new, bool vec, int* err) {
-  constexpr int kLanes = HD / 8, kGroups = 256 / kLanes;
+                                                        const int32_t* __restrict__ n_new, bool vec, int s_t, int s_h,
+                                                        int* err) {
+  constexpr int kLanes = HD / 8, kGroups = 256 / kLanes;  // (kGroups = s_t * heads + s_h)
   const int lane8 = threadIdx.x % kLanes, heads = (int)c.heads, b = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
   const X* from = (is_v ? v : k) + b * s.batch + 8 * lane8;
@@ -96,9 +103,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __re
   constexpr int kBytes = F == kKvF16 ? 2 * HD : HD;
   float x[kRows][8] = {};
   int64_t row[kRows];  // of the cache; -1: none
+  int r = blockIdx.x * kRows * kGroups + threadIdx.x / kLanes, t = r / heads, h = r - t * heads;
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const int r = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes, t = r / heads, h = r - t * heads;
+    if (i) {
+      r += kGroups;
+      h += s_h;
+      t += s_t;
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+    }
     const int64_t at = (int64_t)start + t;
     row[i] = -1;
     if (r >= rows) continue;
@@ -116,11 +132,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __re
   }
 }
 
+// Bytes 2 p and 2 p + 1 of w as values.
 template <int F>
-__device__ __forceinline__ float value_of(uint32_t byte, float scale) {
-  if constexpr (F == kKvI8) return __fmul_rn((float)((int)byte - 128), scale);
-  const __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
-  return __fmul_rn(__half2float(__half(h)), scale);
+__device__ __forceinline__ float2 values_of(uint32_t w, int p, float scale) {
+  float2 y;
+  if constexpr (F == kKvI8) {  // a byte behind 0x4b0000 is the float 2^23 + byte
+    y.x = __uint_as_float(__byte_perm(w, 0x4b000000u, p ? 0x7442 : 0x7440)) - 8388736.0f;
+    y.y = __uint_as_float(__byte_perm(w, 0x4b000000u, p ? 0x7443 : 0x7441)) - 8388736.0f;
+  } else {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * p) & 0xffffu), __NV_E4M3);
+    y = __half22float2(__half2(h));
+  }
+  return make_float2(__fmul_rn(y.x, scale), __fmul_rn(y.y, scale));
 }
 
 __device__ __forceinline__ void put8(float* p, const float (&x)[8]) {
@@ -134,49 +157,46 @@ __device__ __forceinline__ void put8(__half* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
 }
 
-// Positions of one (sequence, head) plane, K or V: grid (positions; plane; K or V).  A thread takes 16 values of a row,
-// kRows rows a block apart.
+// Positions of one (sequence, head) plane, K or V: grid (positions; plane; K or V).  A thread takes 8 values of a row (so
+// that a warp's 16-byte stores of f16 lie side by side), kReadRows rows a block apart, their loads under way together.
 template <int F, int HD, typename Y>
 __global__ void __launch_bounds__(256) kv_read_kernel(KvCache c, int64_t pos0, int n, Y* __restrict__ k_out, Y* __restrict__ v_out) {
-  constexpr int kLanes = HD / 16, kGroups = 256 / kLanes;
+  constexpr int kLanes = HD / 8, kGroups = 256 / kLanes;
   const int lane = threadIdx.x % kLanes;
   const bool is_v = blockIdx.z != 0;
   const int64_t plane = (int64_t)blockIdx.y * c.max_seq + pos0;
   const char* from = static_cast<const char*>(is_v ? c.v : c.k);
   const float* scales = is_v ? c.v_scale : c.k_scale;
-  Y* to = (is_v ? v_out : k_out) + (int64_t)blockIdx.y * n * HD + 16 * lane;
-  constexpr int kLoads = F == kKvF16 ? 2 : 1;  // of 16 bytes
-  uint4 w[kRows][kLoads];
-  float sc[kRows];
+  Y* to = (is_v ? v_out : k_out) + (int64_t)blockIdx.y * n * HD + 8 * lane;
+  using Word = std::conditional_t<F == kKvF16, uint4, uint2>;
+  Word w[kReadRows];
+  float sc[kReadRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int j = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes;
+  for (int i = 0; i < kReadRows; ++i) {
+    const int j = (blockIdx.x * kReadRows + i) * kGroups + threadIdx.x / kLanes;
     sc[i] = 0.f;
     if (j >= n) continue;
-    const uint4* src = reinterpret_cast<const uint4*>(from + (plane + j) * (HD * kLoads)) + lane * kLoads;
-#pragma unroll
-    for (int l = 0; l < kLoads; ++l) w[i][l] = __ldcs(src + l);
+    w[i] = __ldcs(reinterpret_cast<const Word*>(from + (plane + j) * (HD / 8 * (int)sizeof(Word))) + lane);
     if (F != kKvF16) sc[i] = __ldcs(scales + plane + j);
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int j = (blockIdx.x * kRows + i) * kGroups + threadIdx.x / kLanes;
+  for (int i = 0; i < kReadRows; ++i) {
+    const int j = (blockIdx.x * kReadRows + i) * kGroups + threadIdx.x / kLanes;
     if (j >= n) continue;
-    float x[2][8];
+    float x[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const uint4 q = w[i][F == kKvF16 ? k / 8 : 0];
+    for (int p = 0; p < 4; ++p) {
+      float2 y;
       if constexpr (F == kKvF16) {
-        const int e = k & 7;
-        const uint32_t u = e < 2 ? q.x : e < 4 ? q.y : e < 6 ? q.z : q.w;
-        x[k / 8][e] = __half2float(__ushort_as_half((unsigned short)(e & 1 ? u >> 16 : u & 0xffffu)));
+        const uint32_t u = p == 0 ? w[i].x : p == 1 ? w[i].y : p == 2 ? w[i].z : w[i].w;
+        y = __half22float2(__halves2half2(__ushort_as_half((unsigned short)(u & 0xffffu)), __ushort_as_half((unsigned short)(u >> 16))));
       } else {
-        const uint32_t u = k < 4 ? q.x : k < 8 ? q.y : k < 12 ? q.z : q.w;
-        x[k / 8][k & 7] = value_of<F>((u >> (8 * (k & 3))) & 255u, sc[i]);
+        y = values_of<F>(p < 2 ? w[i].x : w[i].y, p & 1, sc[i]);
       }
+      x[2 * p] = y.x;
+      x[2 * p + 1] = y.y;
     }
-    put8(to + (int64_t)j * HD, x[0]);
-    put8(to + (int64_t)j * HD + 8, x[1]);
+    put8(to + (int64_t)j * HD, x);
   }
 }
 
@@ -189,8 +209,9 @@ cudaError_t append_fmt(const KvCache& c, const X* k, const X* v, int64_t T, cons
   const size_t m = 16 / sizeof(X);  // 16-byte loads where every row starts on such a boundary
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 && s.batch % m == 0 &&
                    s.token % m == 0 && s.head % m == 0;
-  if (c.hd == 128) kv_append_kernel<F, 128, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, err);
-  else kv_append_kernel<F, 64, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, err);
+  const int groups = 256 / (c.hd / 8), s_t = groups / (int)c.heads, s_h = groups % (int)c.heads;
+  if (c.hd == 128) kv_append_kernel<F, 128, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, s_t, s_h, err);
+  else kv_append_kernel<F, 64, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, s_t, s_h, err);
   return cudaGetLastError();
 }
 
@@ -205,7 +226,7 @@ cudaError_t append_any(const KvCache& c, const void* k, const void* v, int64_t T
 
 template <int F, typename Y>
 cudaError_t read_fmt(const KvCache& c, int64_t pos0, int64_t n, Y* k, Y* v, cudaStream_t st) {
-  const int64_t per = kRows * (256 / (c.hd / 16)), blocks = (n + per - 1) / per;
+  const int64_t per = kReadRows * (256 / (c.hd / 8)), blocks = (n + per - 1) / per;
   if (c.batch * c.heads > 65535) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks, (unsigned)(c.batch * c.heads), 2);
   if (c.hd == 128) kv_read_kernel<F, 128, Y><<<grid, 256, 0, st>>>(c, pos0, (int)n, k, v);
