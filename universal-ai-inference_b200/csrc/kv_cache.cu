@@ -44,64 +44,79 @@ __device__ __forceinline__ void load8(const __half* p, bool vec, float (&x)[8]) 
   for (int i = 0; i < 8; ++i) x[i] = __half2float(h[i]);
 }
 
-// HD / 8 lanes hold a row, 8 consecutive values each, and store it at `row` unless that is null (every lane of the
+__device__ __forceinline__ float larger(float a, float b) {  // a NaN stays one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// HD / 16 lanes hold a row, of each half 8 values in a row, and store it at `row` unless that is null (every lane of the
 // warp takes part in the maxima); returns the row's scale (0 for f16, which has none).
 template <int F, int HD>
-__device__ __forceinline__ float store_row8(const float (&x)[8], void* row, int lane8) {
+__device__ __forceinline__ float store_row(const float (&x)[2][8], char* row, int lane) {
   if constexpr (F == kKvF16) {
-    __half h[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = __float2half_rn(x[i]);
-    if (row) reinterpret_cast<uint4*>(row)[lane8] = *reinterpret_cast<const uint4*>(h);
+    for (int d = 0; d < 2; ++d) {
+      __half h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = __float2half_rn(x[d][i]);
+      if (row) reinterpret_cast<uint4*>(row + d * HD)[lane] = *reinterpret_cast<const uint4*>(h);
+    }
     return 0.f;
   } else {
-    // |x| as bits: an infinity or a NaN compares above every finite value
-    uint32_t a = 0;
+    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int d = 0; d < 2; ++d)
 #pragma unroll
-    for (int o = HD / 16; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const float top = F == kKvI8 ? 127.f : 448.f, amax = __uint_as_float(a);
-    const bool fine = a < 0x7f800000u && amax >= kTiny;
-    const float inv = fine ? __fdiv_rn(top, amax) : 0.f;
-    uint32_t w[2];
+      for (int i = 0; i < 8; ++i) amax = larger(amax, fabsf(x[d][i]));
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      float y[4];
+    for (int o = HD / 32; o > 0; o >>= 1) amax = larger(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float top = F == kKvI8 ? 127.f : 448.f;
+    const bool fine = amax >= kTiny && amax < INFINITY;
+    const float inv = __fdiv_rn(top, amax);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = fine ? __fmul_rn(x[4 * p + i], inv) : 0.f;
-      if constexpr (F == kKvI8) {  // added to 3 * 2^22 + 128, a number rounds to a whole one whose low byte is the code
-        uint32_t u[4];
+    for (int d = 0; d < 2; ++d) {
+      uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(__fadd_rn(y[i], 12583040.0f));
-        w[p] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
-      } else {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-        w[p] = lo | (hi << 16);
+      for (int p = 0; p < 2; ++p) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = __fmul_rn(x[d][4 * p + i], inv);
+        if constexpr (F == kKvI8) {  // added to 3 * 2^22 + 128, a number rounds to a whole one whose low byte is the code
+          uint32_t u[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(__fadd_rn(y[i], 12583040.0f));
+          w[p] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+        } else {
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+          w[p] = lo | (hi << 16);
+        }
+        if (!fine) w[p] = F == kKvI8 ? 0x80808080u : 0u;
       }
+      if (row) reinterpret_cast<uint2*>(row + d * (HD / 2))[lane] = make_uint2(w[0], w[1]);
     }
-    if (row) reinterpret_cast<uint2*>(row)[lane8] = make_uint2(w[0], w[1]);
-    return a >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : fine ? __fdiv_rn(amax, top) : 0.f;
+    if (lane != 0) return 0.f;
+    return fine ? __fdiv_rn(amax, top) : amax < INFINITY ? 0.f : __uint_as_float(0x7fffffffu);
   }
 }
 
-// One group of HD / 8 lanes per row: grid (tokens x heads of a sequence, heads fastest; sequence; K or V), kRows groups
+// One group of HD / 16 lanes per row: grid (tokens x heads of a sequence, heads fastest; sequence; K or V), kRows groups
 // of heads x tokens a block apart for each thread, their loads under way together.
 template <int F, int HD, typename X>
 __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __restrict__ k, const X* __restrict__ v,
                                                         int T, RowView s, const int32_t* __restrict__ pos,
                                                         const int32_t* __restrict__ n_new, bool vec, int s_t, int s_h,
                                                         int* err) {
-  constexpr int kLanes = HD / 8, kGroups = 256 / kLanes;  // (kGroups = s_t * heads + s_h)
-  const int lane8 = threadIdx.x % kLanes, heads = (int)c.heads, b = blockIdx.y;
+  constexpr int kLanes = HD / 16, kGroups = 256 / kLanes;  // (kGroups = s_t * heads + s_h)
+  const int lane = threadIdx.x % kLanes, heads = (int)c.heads, b = blockIdx.y;
   const bool is_v = blockIdx.z != 0;
-  const X* from = (is_v ? v : k) + b * s.batch + 8 * lane8;
+  const X* from = (is_v ? v : k) + b * s.batch + 8 * lane;
   const int count = n_new ? min(n_new[b], T) : T, start = pos[b], rows = count * heads;
   char* out = static_cast<char*>(is_v ? c.v : c.k);
   float* scales = is_v ? c.v_scale : c.k_scale;
   constexpr int kBytes = F == kKvF16 ? 2 * HD : HD;
-  float x[kRows][8] = {};
+  float x[kRows][2][8] = {};
   int64_t row[kRows];  // of the cache; -1: none
   int r = blockIdx.x * kRows * kGroups + threadIdx.x / kLanes, t = r / heads, h = r - t * heads;
 #pragma unroll
@@ -119,16 +134,18 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvCache c, const X* __re
     row[i] = -1;
     if (r >= rows) continue;
     if (at < 0 || at >= c.max_seq) {
-      if (lane8 == 0) atomicExch(err, kErrKvPosition);
+      if (lane == 0) atomicExch(err, kErrKvPosition);
       continue;
     }
     row[i] = ((int64_t)b * heads + h) * c.max_seq + at;
-    load8(from + t * s.token + h * s.head, vec, x[i]);
+    const X* src = from + t * s.token + h * s.head;
+    load8(src, vec, x[i][0]);
+    load8(src + HD / 2, vec, x[i][1]);
   }
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const float sc = store_row8<F, HD>(x[i], row[i] >= 0 ? out + row[i] * kBytes : nullptr, lane8);
-    if (F != kKvF16 && row[i] >= 0 && lane8 == 0) scales[row[i]] = sc;
+    const float sc = store_row<F, HD>(x[i], row[i] >= 0 ? out + row[i] * kBytes : nullptr, lane);
+    if (F != kKvF16 && row[i] >= 0 && lane == 0) scales[row[i]] = sc;
   }
 }
 
@@ -203,13 +220,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvCache c, int64_t pos0, i
 template <int F, typename X>
 cudaError_t append_fmt(const KvCache& c, const X* k, const X* v, int64_t T, const RowView& s, const int32_t* pos,
                        const int32_t* n_new, int* err, cudaStream_t st) {
-  const int64_t per = kRows * (256 / (c.hd / 8)), blocks = (T * c.heads + per - 1) / per;
+  const int64_t per = kRows * (256 / (c.hd / 16)), blocks = (T * c.heads + per - 1) / per;
   if (blocks > 0x7fffffff || c.batch > 65535) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks, (unsigned)c.batch, 2);
   const size_t m = 16 / sizeof(X);  // 16-byte loads where every row starts on such a boundary
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 && s.batch % m == 0 &&
                    s.token % m == 0 && s.head % m == 0;
-  const int groups = 256 / (c.hd / 8), s_t = groups / (int)c.heads, s_h = groups % (int)c.heads;
+  const int groups = 256 / (c.hd / 16), s_t = groups / (int)c.heads, s_h = groups % (int)c.heads;
   if (c.hd == 128) kv_append_kernel<F, 128, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, s_t, s_h, err);
   else kv_append_kernel<F, 64, X><<<grid, 256, 0, st>>>(c, k, v, (int)T, s, pos, n_new, vec, s_t, s_h, err);
   return cudaGetLastError();
