@@ -210,16 +210,22 @@ def ptr(a) -> int | None:
 
 def _torch():
     """torch, which whoever holds a tensor has imported (this module does not need it)."""
-    import sys
-    return sys.modules["torch"]
+    global _T
+    if _T is None:
+        import sys
+        _T = sys.modules["torch"]
+    return _T
+
+
+_T = None
 
 
 def _dtype_code(t) -> int:
     """UAII_MOE_DTYPE_* of a torch tensor's element type (f32 or f16)."""
-    d = t.dtype
-    if d is _torch().float32:
+    d, T = t.dtype, _T or _torch()
+    if d is T.float32:
         return DTYPE_F32
-    if d is _torch().float16:
+    if d is T.float16:
         return DTYPE_F16
     raise TypeError(f"expected float32 or float16, got {d}")
 
@@ -244,6 +250,8 @@ def _whole(t, what, *shape):
 
 
 def _typed(t, what, dtype, *shape):
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype is not dtype:
         raise TypeError(f"{what}: expected {dtype}, got {t.dtype}")
     return _whole(t, what, *shape)
@@ -417,11 +425,12 @@ class Backend:
         same for both) at positions pos[i] + t, for t < n_new[i] (int32) where given."""
         b, t = k.shape[0], k.shape[1]
         sb, st, sh = _rows(k, cache.batch, t, cache.n_kv_heads, cache.head_dim)
-        if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype:
+        if v.shape != k.shape or v.stride() != k.stride() or v.dtype is not k.dtype:
             raise ValueError("k and v must have the same shape, strides and type")
+        i32 = (_T or _torch()).int32
         _check(lib.uaii_moe_kv_append(self._h, byref(cache), k.data_ptr(), v.data_ptr(), _dtype_code(k), t, sb, st, sh,
-                                      _typed(pos, "pos", _torch().int32, b),
-                                      None if n_new is None else _typed(n_new, "n_new", _torch().int32, b)))
+                                      _typed(pos, "pos", i32, b),
+                                      None if n_new is None else _typed(n_new, "n_new", i32, b)))
 
     def kv_read(self, cache: KVCache, pos0: int, n: int, k_out, v_out):
         """Positions [pos0, pos0 + n) into k_out, v_out [batch, n_kv_heads, n, head_dim] (f32 or f16)."""
