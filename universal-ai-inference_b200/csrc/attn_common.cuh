@@ -49,10 +49,12 @@ struct Plan {
   bool split_keys;         // wide: the two row tiles hold the same rows
   int unit;                // keys of a unit
   int prefix_nrt, own_nrt; // items per kv head (0: none)
-  int prefix_units;        // units of a prefix item
+  int lead;                // units without keys at the start of every item, for what a piece costs beside its keys
+  int prefix_units;        // units of a prefix item, the lead among them
   int prefix_items;
   int grid;                // CTAs (0: the kernel has no work)
   int workers;             // shares of the work: wide CTAs or narrow warps
+  int per_item;            // workers of each prefix item (0: the work is dealt out evenly)
   float* part;             // partial sums [slot][slot_rows][hd]
   float* ml;               // (maximum, denominator) of each partial row
 };
@@ -125,7 +127,7 @@ struct SeqTables {
   int32_t cum[kMaxScan + 1], len[kMaxScan], sum[kMaxScan / 32];
 };
 
-__device__ __forceinline__ int units_of(int len, int unit) { return (len + unit - 1) / unit; }
+__device__ __forceinline__ int units_of(int len, int unit, int lead) { return len ? (len + unit - 1) / unit + lead : 0; }
 
 // Inclusive sums of the units of 32 sequences, one a lane.
 __device__ __forceinline__ int scan32(int n) {
@@ -146,7 +148,7 @@ __device__ __forceinline__ Seqs sequences(const PrefixAttnArgs& a, const Plan& p
   const int lane = threadIdx.x & 31, B = (int)a.B;
   for (int c = threadIdx.x >> 5; 32 * c < B; c += blockDim.x >> 5) {
     const int b = 32 * c + lane, len = b < B ? own_length(a, b, blockIdx.x == 0) : 0;
-    const int n = scan32(b < B ? units_of(len, p.unit) : 0);
+    const int n = scan32(b < B ? units_of(len, p.unit, p.lead) : 0);
     if (b < B) {
       t.len[b] = len;
       t.cum[b + 1] = n;
@@ -196,14 +198,25 @@ __device__ __forceinline__ int share_of(int u, int total, int n) {
   return u < split ? u / (each + 1) : more + (u - split) / each;
 }
 
+// The same for a grid's workers: dealt evenly over all units, or over those of each prefix item (p.per_item).
+__device__ __forceinline__ int start_of(const Plan& p, int c, int total) {
+  if (p.per_item == 0) return share_start(c, total, p.workers);
+  return min(total, c / p.per_item * p.prefix_units + share_start(c % p.per_item, p.prefix_units, p.per_item));
+}
+__device__ __forceinline__ int worker_of(const Plan& p, int u, int total) {
+  if (p.per_item == 0) return share_of(u, total, p.workers);
+  const int item = u / p.prefix_units;
+  return item * p.per_item + share_of(u - item * p.prefix_units, p.prefix_units, p.per_item);
+}
+
 struct Walk {
   int u, end, b, worker;
   Walk() = default;
   __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const Seqs& q, int worker_) : b(0), worker(worker_) {
     const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
     const int total = prefix + (per ? q.cum[a.B] * per : 0);
-    u = share_start(worker, total, p.workers);
-    end = share_start(worker + 1, total, p.workers);
+    u = start_of(p, worker, total);
+    end = start_of(p, worker + 1, total);
     if (end > prefix) {  // the last sequence whose units start at or before the first own unit
       const int first = max(u - prefix, 0);
       int lo = 0, hi = (int)a.B - 1;
@@ -216,7 +229,12 @@ struct Walk {
     }
   }
   __device__ __forceinline__ bool next(Piece& x, const Plan& p, const PrefixAttnArgs& a, const Seqs& q) {
-    if (u >= end) return false;
+    while (u < end)
+      if (step(x, p, a, q)) return true;
+    return false;
+  }
+  // The next item's part; false if it has no keys.
+  __device__ __forceinline__ bool step(Piece& x, const Plan& p, const PrefixAttnArgs& a, const Seqs& q) {
     const int prefix = p.prefix_items * p.prefix_units;
     int in, units;
     if (u >= prefix) {
@@ -247,11 +265,11 @@ struct Walk {
       x.limit = x.fewest = (int)a.prefix_len;
     }
     const int n = min(units - in, end - u);
-    x.t0 = in;
-    x.t1 = in + n;
+    x.t0 = max(0, in - p.lead);
+    x.t1 = in + n - p.lead;
     x.slot += worker;
     u += n;
-    return true;
+    return x.t1 > 0;
   }
 };
 

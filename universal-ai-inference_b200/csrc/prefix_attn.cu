@@ -21,6 +21,8 @@
 //           exponentials are the work).
 // f32 queries are split in two f16 parts, and so are the probabilities: rows 0-7 of an MMA hold the leading parts and
 // rows 8-15 the rests ("folded"), which keeps f32 accuracy at no cost while an item has no more than 8 rows.
+#include <algorithm>
+
 #include "attn_narrow.cuh"
 #include "attn_wide.cuh"
 
@@ -29,13 +31,13 @@ namespace attn {
 namespace {
 
 // The tables of batches too large for a CTA's shared memory: cum [B + 1], then len [B].
-__global__ void __launch_bounds__(1024) sequences_kernel(const __grid_constant__ PrefixAttnArgs a, int unit, int32_t* cum) {
+__global__ void __launch_bounds__(1024) sequences_kernel(const __grid_constant__ PrefixAttnArgs a, int unit, int lead, int32_t* cum) {
   __shared__ int warp_sum[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   int before = 0;
   for (int64_t b0 = 0; b0 < a.B; b0 += 1024) {
     const int64_t b = b0 + t;
-    const int len = b < a.B ? own_length(a, b, true) : 0, n = scan32(b < a.B ? units_of(len, unit) : 0);
+    const int len = b < a.B ? own_length(a, b, true) : 0, n = scan32(b < a.B ? units_of(len, unit, lead) : 0);
     if (lane == 31) warp_sum[warp] = n;
     __syncthreads();
     const int s = warp_sum[lane], up_to = __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
@@ -78,7 +80,7 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
     u0 = (int)item * units;
   }
   if (units == 0) return q;
-  const int c0 = share_of(u0, total, p.workers), c1 = share_of(u0 + units - 1, total, p.workers);
+  const int c0 = worker_of(p, u0 + p.lead, total), c1 = worker_of(p, u0 + units - 1, total);
   q.part = p.part;
   q.ml = p.ml;
   q.first = (item + c0) * p.slot_rows + (rho - j * p.rt);
@@ -202,6 +204,8 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 int narrow_keys(const PrefixAttnArgs& a) { return a.own.fmt == kKvF16 && a.own.hd == 128 ? 16 : 32; }
 
+constexpr int kWideLead = 5, kNarrowLead = 2;
+
 // The grids of a call and the workspace.  Own items of more than 16 rows: one wide grid for them and the prefix.  Else a
 // grid for the prefix (wide above 16 rows) and a narrow one for the own items.
 struct Layout {
@@ -230,14 +234,28 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     p.unit = wide ? kTile : narrow_keys(a);
     p.own_nrt = own ? (own_rows + p.rt - 1) / p.rt : 0;
     p.prefix_nrt = prefix ? (prefix_rows + p.rt - 1) / p.rt : 0;
-    p.prefix_units = prefix ? (int)((a.prefix_len + p.unit - 1) / p.unit) : 0;
+    const int tiles = prefix ? (int)((a.prefix_len + p.unit - 1) / p.unit) : 0;
     p.prefix_items = (int)a.own.heads * p.prefix_nrt;
     const int64_t own_items = a.B * a.own.heads * p.own_nrt;
-    const int64_t most = (int64_t)p.prefix_items * p.prefix_units + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
-    l.most = most > l.most ? most : l.most;
+    const int64_t most = (int64_t)p.prefix_items * tiles + own_items * ((a.own.max_seq + p.unit - 1) / p.unit);
     const int each = wide ? 1 : kWarps, full = kSms * (wide ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
     p.grid = (int)(most < full * each ? (most + each - 1) / each : full);
     p.workers = p.grid * each;
+    // A piece costs about as much as kWideLead wide tiles more than its keys (sums out, other queries in: 58000 cycles
+    // for 7 tiles in two pieces, 41000 in one), or kNarrowLead narrow steps, so every item counts as that much longer.
+    // Where all items are alike, the same number of workers for each costs no second piece: taken unless the workers
+    // left over are worth more.
+    p.lead = wide ? kWideLead : kNarrowLead;
+    if (wide && !own && p.workers >= p.prefix_items) {
+      const int per = p.workers / p.prefix_items;
+      if ((tiles + per - 1) / per <= (most + p.workers - 1) / p.workers + kWideLead) {
+        p.per_item = per;
+        p.grid = p.workers = per * p.prefix_items;
+        p.lead = 0;
+      }
+    }
+    p.prefix_units = tiles ? tiles + p.lead : 0;
+    l.most = std::max(l.most, most + p.lead * (p.prefix_items + own_items));
     const int64_t slot_rows = (p.prefix_items + own_items + p.workers) * p.slot_rows;
     p.part = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * a.own.hd));
@@ -300,7 +318,7 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
   if (e != cudaSuccess) return e;
   // four warps a row where the rows alone would leave most of the GPU idle
   const int64_t rows = a.B * a.T * a.H;
-  const bool few = rows <= 4 * kSms;
+  const bool few = rows <= 16 * kSms;
   const auto kern = a.half ? (few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>)
                            : (few ? join_kernel<HD, float, 4> : join_kernel<HD, float, 1>);
   const int32_t* sums = cum;
@@ -328,7 +346,7 @@ cudaError_t launch_prefix_attn(PrefixAttnArgs a, void* ws, int* launches, cudaSt
   const int32_t* given = nullptr;
   *launches = 2 + (l.prefix.grid > 0);
   if (a.B > kMaxScan) {
-    sequences_kernel<<<1, 1024, 0, st>>>(a, l.own.unit, cum);
+    sequences_kernel<<<1, 1024, 0, st>>>(a, l.own.unit, l.own.lead, cum);
     given = cum;
     ++*launches;
   }
