@@ -39,6 +39,20 @@ struct Maps {
   CUtensorMap pk, pv, ok, ov;
 };
 
+// Division by a number that the host knows: n / d = floor(n m / 2^(31 + s)) for 0 <= n < 2^31, with 2^s >= d and
+// m = ceil(2^(31 + s) / d) < 2^32 (m d exceeds 2^(31 + s) by less than d <= 2^s, n times that is below 2^(31 + s)).
+// The plain operator took a worker's walk to its next piece 3500 cycles, most of it six divisions one after the other.
+struct Div {
+  uint32_t m = 0;
+  int s = 0;  // 0: d = 1
+  Div() = default;
+  explicit Div(int d) {
+    while ((int64_t(1) << s) < d) ++s;
+    m = (uint32_t)(((uint64_t(1) << (31 + s)) + (uint64_t)d - 1) / (uint64_t)d);
+  }
+};
+__device__ __forceinline__ int operator/(int n, const Div& d) { return d.s ? (int)(__umulhi((uint32_t)n, d.m) >> (d.s - 1)) : n; }
+
 // The items of one kernel: prefix items first, then own ones (either may be missing).
 struct Plan {
   int G;                   // query heads per kv head
@@ -54,6 +68,7 @@ struct Plan {
   int prefix_items;
   int grid;                // CTAs (0: the kernel has no work)
   int workers;             // shares of the work: wide CTAs or narrow warps
+  Div by_G, by_rt, by_own_rows, by_own_nrt, by_prefix_nrt, by_prefix_units, by_workers, by_per_item;
   int per_item;            // workers of each prefix item (0: the work is dealt out evenly)
   float* part;             // partial sums [slot][slot_rows][hd]
   float* ml;               // (maximum, denominator) of each partial row
@@ -188,25 +203,26 @@ struct Piece {
 };
 
 // The first unit of worker c: the first total % n workers take one unit more than the others.
-__device__ __forceinline__ int share_start(int c, int total, int n) {
-  const int each = total / n;
+__device__ __forceinline__ int share_start(int c, int total, int n, int each) {  // each = total / n
   return c * each + min(c, total - each * n);
 }
 // The worker that holds unit u < total.
-__device__ __forceinline__ int share_of(int u, int total, int n) {
-  const int each = total / n, more = total - each * n, split = more * (each + 1);
+__device__ __forceinline__ int share_of(int u, int total, int n, int each) {
+  const int more = total - each * n, split = more * (each + 1);
   return u < split ? u / (each + 1) : more + (u - split) / each;
 }
 
 // The same for a grid's workers: dealt evenly over all units, or over those of each prefix item (p.per_item).
 __device__ __forceinline__ int start_of(const Plan& p, int c, int total) {
-  if (p.per_item == 0) return share_start(c, total, p.workers);
-  return min(total, c / p.per_item * p.prefix_units + share_start(c % p.per_item, p.prefix_units, p.per_item));
+  if (p.per_item == 0) return share_start(c, total, p.workers, total / p.by_workers);
+  const int item = c / p.by_per_item;
+  return min(total, item * p.prefix_units + share_start(c - item * p.per_item, p.prefix_units, p.per_item,
+                                                        p.prefix_units / p.by_per_item));
 }
 __device__ __forceinline__ int worker_of(const Plan& p, int u, int total) {
-  if (p.per_item == 0) return share_of(u, total, p.workers);
-  const int item = u / p.prefix_units;
-  return item * p.per_item + share_of(u - item * p.prefix_units, p.prefix_units, p.per_item);
+  if (p.per_item == 0) return share_of(u, total, p.workers, total / p.by_workers);
+  const int item = u / p.by_prefix_units;
+  return item * p.per_item + share_of(u - item * p.prefix_units, p.prefix_units, p.per_item, p.prefix_units / p.by_per_item);
 }
 
 struct Walk {
@@ -245,21 +261,21 @@ struct Walk {
       in = rest - j * units;
       x.slot = p.prefix_items + (int64_t)b * per + j;
       x.own = 1;
-      x.kvh = j / p.own_nrt;
-      x.rt = j % p.own_nrt;
+      x.kvh = j / p.by_own_nrt;
+      x.rt = j - x.kvh * p.own_nrt;
       x.seq = b;
       x.z = b * (int)a.own.heads + x.kvh;
-      const int first = x.rt * p.rt / p.G, last = (min((x.rt + 1) * p.rt, p.own_rows) - 1) / p.G;  // tokens
+      const int first = x.rt * p.rt / p.by_G, last = (min((x.rt + 1) * p.rt, p.own_rows) - 1) / p.by_G;  // tokens
       const int seen = q.len[b] - (int)a.T + 1;
       x.limit = seen + last;
       x.fewest = seen + first;
     } else {
       units = p.prefix_units;
-      x.slot = u / units;
+      x.slot = u / p.by_prefix_units;
       in = u - (int)x.slot * units;
       x.own = 0;
-      x.kvh = (int)x.slot / p.prefix_nrt;
-      x.rt = (int)x.slot % p.prefix_nrt;
+      x.kvh = (int)x.slot / p.by_prefix_nrt;
+      x.rt = (int)x.slot - x.kvh * p.prefix_nrt;
       x.seq = 0;
       x.z = x.kvh;
       x.limit = x.fewest = (int)a.prefix_len;
@@ -294,11 +310,10 @@ __device__ __forceinline__ const Q* q_row(const PrefixAttnArgs& a, const Plan& p
     lim = 0;
     return nullptr;
   }
-  const int64_t b = x.own ? x.seq : rho / p.own_rows;
-  const int in = x.own ? rho : rho % p.own_rows;
-  const int t = in / p.G, g = in % p.G;
-  lim = x.own ? x.fewest + t - x.rt * p.rt / p.G : x.limit;
-  return static_cast<const Q*>(a.q) + b * a.qs.batch + t * a.qs.token + ((int64_t)x.kvh * p.G + g) * a.qs.head;
+  const int b = x.own ? x.seq : rho / p.by_own_rows, in = x.own ? rho : rho - b * p.own_rows;
+  const int t = in / p.by_G, g = in - t * p.G;
+  lim = x.own ? x.fewest + t - x.rt * p.rt / p.by_G : x.limit;
+  return static_cast<const Q*>(a.q) + (int64_t)b * a.qs.batch + t * a.qs.token + ((int64_t)x.kvh * p.G + g) * a.qs.head;
 }
 
 // A power of two that brings the largest of a folded row into [1, 2): its exponent leaves through the score factor, so

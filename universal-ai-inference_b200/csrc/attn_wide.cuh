@@ -386,10 +386,15 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
     }
     shrink = row_shrink(mx);
   }
+  constexpr bool kAhead = sizeof(Q) == 2;  // (f32 rows do not fit twice)
+  Block all[kAhead ? HD / 64 : 1];
+  if constexpr (kAhead)
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) load(h, all[h]);
 #pragma unroll
   for (int h = 0; h < HD / 64; ++h) {
-    Block v;
-    load(h, v);
+    Block& v = all[kAhead ? h : 0];
+    if constexpr (!kAhead) load(h, v);
     uint32_t c[32];
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
@@ -414,6 +419,13 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
   }
   umma::tmem_st_wait();
   return shrink;
+}
+
+// 32 bytes, a whole sector: a thread's row lies apart from its neighbours'.
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
 }
 
 template <int F, int HD, bool SPLIT_Q, typename Q>
@@ -571,11 +583,12 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
 #pragma unroll
         for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(u[j]) * up;
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < 32; j += 8) {
           // 8-bit pieces: even dimensions of 16 lie before the odd ones
-          const int e = (j & 16) + ((j & 15) >> 1);
-          reinterpret_cast<float4*>(part + 32 * c + j)[0] =
-              F == kKvF16 ? make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]) : make_float4(y[e], y[e + 8], y[e + 1], y[e + 9]);
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = F == kKvF16 ? y[j + i] : y[(j & 16) + ((j & 15) >> 1) + (i >> 1) + 8 * (i & 1)];
+          store8(part + 32 * c + j, z);
         }
       }
     } else {

@@ -65,7 +65,7 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
                                             int kvh) {
   Pieces q{};
   if (!OWN && p.prefix_items == 0) return q;
-  const int j = rho / p.rt, per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
+  const int j = rho / p.by_rt, per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
   const int total = prefix + (per ? cum[a.B] * per : 0);
   int64_t item;
   int u0, units;
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
   const int rows = (int)(a.B * a.T * a.H), row = (int)blockIdx.x * kRows + warp / WARPS;
   const bool live = row < rows;
   const int bt = live ? row / (int)a.H : 0, h = live ? row - bt * (int)a.H : 0, b = bt / (int)a.T, t = bt - b * (int)a.T;
-  const int kvh = h / po.G, g = h - kvh * po.G;
+  const int kvh = h / po.by_G, g = h - kvh * po.G;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the pieces are there from here on
   const Pieces qp = pieces_of<false>(a, px, cum, b, bt * po.G + g, kvh), qo = pieces_of<true>(a, po, cum, b, t * po.G + g, kvh);
   // the row's reference, a piece a lane
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Prefi
   }
   if (!live) return;
   if (hidden) {  // positions that the item's first token does not see and this one does
-    const int seen = own_length(a, b, false) - (int)a.T + 1, first = (t * po.G + g) / po.rt * po.rt / po.G;
+    const int seen = own_length(a, b, false) - (int)a.T + 1, first = (t * po.G + g) / po.by_rt * po.rt / po.by_G;
     const int64_t plane = ((int64_t)b * a.own.heads + kvh) * a.own.max_seq;
     for (int pos = max(0, seen + first); pos < seen + t; ++pos) {
       const int64_t at = (plane + pos) * HD + N * lane;
@@ -256,6 +256,14 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     }
     p.prefix_units = tiles ? tiles + p.lead : 0;
     l.most = std::max(l.most, most + p.lead * (p.prefix_items + own_items));
+    p.by_G = Div(G);
+    p.by_rt = Div(p.rt);
+    p.by_own_rows = Div(own_rows);
+    p.by_own_nrt = Div(std::max(1, p.own_nrt));
+    p.by_prefix_nrt = Div(std::max(1, p.prefix_nrt));
+    p.by_prefix_units = Div(std::max(1, p.prefix_units));
+    p.by_workers = Div(std::max(1, p.workers));
+    p.by_per_item = Div(std::max(1, p.per_item));
     const int64_t slot_rows = (p.prefix_items + own_items + p.workers) * p.slot_rows;
     p.part = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * a.own.hd));
