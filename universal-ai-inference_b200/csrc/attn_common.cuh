@@ -68,8 +68,7 @@ struct Plan {
   int prefix_items;
   int grid;                // CTAs (0: the kernel has no work)
   int workers;             // shares of the work: wide CTAs or narrow warps
-  Div by_G, by_rt, by_own_rows, by_own_nrt, by_prefix_nrt, by_prefix_units, by_workers, by_per_item;
-  int per_item;            // workers of each prefix item (0: the work is dealt out evenly)
+  Div by_G, by_rt, by_own_rows, by_own_nrt, by_prefix_nrt, by_prefix_units, by_workers;
   float* part;             // partial sums [slot][slot_rows][hd]
   float* ml;               // (maximum, denominator) of each partial row
 };
@@ -212,27 +211,15 @@ __device__ __forceinline__ int share_of(int u, int total, int n, int each) {
   return u < split ? u / (each + 1) : more + (u - split) / each;
 }
 
-// The same for a grid's workers: dealt evenly over all units, or over those of each prefix item (p.per_item).
-__device__ __forceinline__ int start_of(const Plan& p, int c, int total) {
-  if (p.per_item == 0) return share_start(c, total, p.workers, total / p.by_workers);
-  const int item = c / p.by_per_item;
-  return min(total, item * p.prefix_units + share_start(c - item * p.per_item, p.prefix_units, p.per_item,
-                                                        p.prefix_units / p.by_per_item));
-}
-__device__ __forceinline__ int worker_of(const Plan& p, int u, int total) {
-  if (p.per_item == 0) return share_of(u, total, p.workers, total / p.by_workers);
-  const int item = u / p.by_prefix_units;
-  return item * p.per_item + share_of(u - item * p.prefix_units, p.prefix_units, p.per_item, p.prefix_units / p.by_per_item);
-}
-
 struct Walk {
   int u, end, b, worker;
   Walk() = default;
   __device__ Walk(const Plan& p, const PrefixAttnArgs& a, const Seqs& q, int worker_) : b(0), worker(worker_) {
     const int prefix = p.prefix_items * p.prefix_units, per = (int)a.own.heads * p.own_nrt;
     const int total = prefix + (per ? q.cum[a.B] * per : 0);
-    u = start_of(p, worker, total);
-    end = start_of(p, worker + 1, total);
+    const int each = total / p.by_workers;
+    u = share_start(worker, total, p.workers, each);
+    end = share_start(worker + 1, total, p.workers, each);
     if (end > prefix) {  // the last sequence whose units start at or before the first own unit
       const int first = max(u - prefix, 0);
       int lo = 0, hi = (int)a.B - 1;

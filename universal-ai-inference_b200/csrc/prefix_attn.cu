@@ -80,7 +80,8 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
     u0 = (int)item * units;
   }
   if (units == 0) return q;
-  const int c0 = worker_of(p, u0 + p.lead, total), c1 = worker_of(p, u0 + units - 1, total);
+  const int each = total / p.by_workers;
+  const int c0 = share_of(u0 + p.lead, total, p.workers, each), c1 = share_of(u0 + units - 1, total, p.workers, each);
   q.part = p.part;
   q.ml = p.ml;
   q.first = (item + c0) * p.slot_rows + (rho - j * p.rt);
@@ -204,7 +205,7 @@ size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 
 int narrow_keys(const PrefixAttnArgs& a) { return a.own.fmt == kKvF16 && a.own.hd == 128 ? 16 : 32; }
 
-constexpr int kWideLead = 5, kNarrowLead = 2;
+constexpr int kWideLead = 7, kNarrowLead = 2;
 
 // The grids of a call and the workspace.  Own items of more than 16 rows: one wide grid for them and the prefix.  Else a
 // grid for the prefix (wide above 16 rows) and a narrow one for the own items.
@@ -241,19 +242,11 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     const int each = wide ? 1 : kWarps, full = kSms * (wide ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
     p.grid = (int)(most < full * each ? (most + each - 1) / each : full);
     p.workers = p.grid * each;
-    // A piece costs about as much as kWideLead wide tiles more than its keys (sums out, other queries in: 58000 cycles
-    // for 7 tiles in two pieces, 41000 in one), or kNarrowLead narrow steps, so every item counts as that much longer.
-    // Where all items are alike, the same number of workers for each costs no second piece: taken unless the workers
-    // left over are worth more.
+    // A piece costs more than its keys (sums out, other queries in: 58000 cycles for 7 wide tiles in two pieces, 41000
+    // in one), so every item counts as kWideLead tiles or kNarrowLead steps longer.  64 rows behind 8192 positions, 24 x 4
+    // tokens behind 4101: 62.3 and 66.8 us without, 51.6 and 43.1 with 3 tiles, 49.2 and 41.5 with 7; 32 rows of 4096
+    // own positions: 64.1, 62.2, 61.5 and 60.0 us with 0, 1, 2 and 4 steps, 64 rows behind 8192 62.2, 58.2, 57.5, 58.7.
     p.lead = wide ? kWideLead : kNarrowLead;
-    if (wide && !own && p.workers >= p.prefix_items) {
-      const int per = p.workers / p.prefix_items;
-      if ((tiles + per - 1) / per <= (most + p.workers - 1) / p.workers + kWideLead) {
-        p.per_item = per;
-        p.grid = p.workers = per * p.prefix_items;
-        p.lead = 0;
-      }
-    }
     p.prefix_units = tiles ? tiles + p.lead : 0;
     l.most = std::max(l.most, most + p.lead * (p.prefix_items + own_items));
     p.by_G = Div(G);
@@ -263,7 +256,6 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     p.by_prefix_nrt = Div(std::max(1, p.prefix_nrt));
     p.by_prefix_units = Div(std::max(1, p.prefix_units));
     p.by_workers = Div(std::max(1, p.workers));
-    p.by_per_item = Div(std::max(1, p.per_item));
     const int64_t slot_rows = (p.prefix_items + own_items + p.workers) * p.slot_rows;
     p.part = reinterpret_cast<float*>(ws + used);
     used += up256(sizeof(float) * (size_t)(slot_rows * a.own.hd));
