@@ -8,15 +8,16 @@
 // none is zero.  Running maximum, sums and outputs are f32.
 //
 // Work.  An item is a tile of query rows that read the same keys: (kv head, rows of the whole batch) over the
-// prefix, (sequence, kv head, rows) over own positions.  Its keys come in units; the units of all items, laid end to
-// end, are dealt out evenly to the workers (CTAs or warps), so a share starts and ends inside items.  Every piece of an item leaves
-// its unnormalised sums, row maxima and denominators in the workspace (slot = item + worker, unique because each next
-// piece raises one of the two), and a last kernel joins the pieces of each row in a fixed order.
+// prefix, (sequence, kv head, rows) over own positions.  Its keys come in units, a few more of them in front of each
+// item for what a piece costs besides; the units of all items, laid end to end, are dealt out evenly to the workers (CTAs
+// or warps), so a share starts and ends inside items.  Every piece of an item leaves its unnormalised sums, row maxima and
+// denominators in the workspace (slot = item + worker, unique because each next piece raises one of the two), and a last
+// kernel joins the pieces of each row in a fixed order.
 //
 // Two tilings, one kernel each.  Bytes become exact f16 operands (the row scales act on scores and probabilities);
 // accumulators are f32.
-//   narrow  (attn_narrow.cuh) 8 or 16 rows; every warp takes other keys of the piece, from copies of its own (few rows: the keys are
-//           the work, and the kernel is bound by the cache's bytes).
+//   narrow  (attn_narrow.cuh) 8 or 16 rows; every warp takes other keys, from copies of its own (few rows: the keys are
+//           the work, and the kernel is near the cache's bytes).
 //   wide    (attn_wide.cuh) 128 or 256 rows on tcgen05, operands made once for all rows (many rows: the products and the
 //           exponentials are the work).
 // f32 queries are split in two f16 parts, and so are the probabilities: rows 0-7 of an MMA hold the leading parts and
@@ -93,7 +94,9 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
 }
 
 // out = sum over a row's pieces of 2^(m - M) o / sum of 2^(m - M) l.  WARPS warps per row; the pieces are taken in the
-// order of the workers, prefix first, a warp every WARPS-th.  px, po: the plans of the kernels that took the prefix and
+// order of the workers, prefix first, a warp every WARPS-th.  Bound by latency (lengths, then maxima, then sums: 4 to 8 us
+// whatever the rows); inside the narrow kernel, by the worker that comes last, it cost more (67 against 63 us at 64 rows
+// behind 8192 positions).  px, po: the plans of the kernels that took the prefix and
 // the own items.
 template <int HD, typename Q, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan px,
@@ -316,7 +319,7 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
   if (l.prefix.grid) e = l.prefix_wide ? wide(l.prefix) : narrow(l.prefix, false);
   if (e == cudaSuccess) e = l.own_wide ? wide(l.own) : narrow(l.own, l.prefix.grid > 0);
   if (e != cudaSuccess) return e;
-  // four warps a row where the rows alone would leave most of the GPU idle
+  // four warps a row up to what the GPU holds at once (2048 rows 54.4 against 55.6 us with one; 4096 rows 130 against 124)
   const int64_t rows = a.B * a.T * a.H;
   const bool few = rows <= 16 * kSms;
   const auto kern = a.half ? (few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>)

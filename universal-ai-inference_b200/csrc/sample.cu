@@ -11,9 +11,12 @@
 // rises, so the kept set is all weights above a cut, and of the weights that equal it the first few by logit and index.
 //
 // A cluster of up to eight CTAs holds a row: every logit is read once and its weight kept in shared memory.  The cut is
-// found with one histogram over the weights' leading bits and a ranking of the few weights of one bin; counts, sums and
-// bins of the CTAs meet through distributed shared memory.  A large batch is bound by the exponentials and divisions
-// (about 30 instructions a logit, once each), a single row by the dozen cluster barriers on its way.
+// found with one histogram over the weights' leading bits and a ranking, by logit, of the few tokens of one bin; counts,
+// sums and bins of the CTAs meet through distributed shared memory.
+// 256 rows of 151936 f16 logits take 270 us (77 MB read once, which alone would be 12 us): 127 instructions a logit at
+// 0.55 of the issue rate, with two CTAs an SM; of a CTA's 60000 cycles 10000 go to reading, 7000 to weights, 8000 to the
+// histogram's atomics, 7000 to ranking, 6000 to the kept mass and 15000 to seven cluster barriers.  A single row takes
+// 20 us, 13.5 of which the caller's side of the call.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>
