@@ -155,3 +155,52 @@ def test_serving_refusals(um, backend):
                 call()
     finally:
         dec.close()
+
+
+def test_rope_pairs_of_halves(um, backend):
+    """rope_mode 2 (halves of a head are the pairs) turns q and k as the plain decoder does."""
+    W, kv = _weights(um)
+    plain = _decoder(um, backend, W, S0 + STEPS, rope_mode=2)
+    serving = _decoder(um, backend, W, S0 + STEPS, rope_mode=2, kv_fmt=um.F16)
+    try:
+        for dec in (plain, serving):
+            for l, (k, v) in enumerate(kv):
+                dec.set_kv(l, k, v, S0)
+        for s, tok in enumerate(_tokens(3)):
+            a, b = _logits(plain, tok), _logits(serving, tok)
+            assert np.abs(a - b).max() <= 2e-3 * np.abs(a).max(), s
+    finally:
+        plain.close()
+        serving.close()
+
+
+def test_generate_equals_stepping(um, backend):
+    W, kv = _weights(um)
+    tok = _tokens(7)[0]
+    a, b = (_decoder(um, backend, W, S0 + STEPS, kv_fmt=um.KV_E4M3) for _ in range(2))
+    try:
+        for dec in (a, b):
+            for l, (k, v) in enumerate(kv):
+                dec.set_kv(l, k, v, S0)
+        out = np.empty((STEPS, B), np.int32)
+        a.generate(tok, STEPS, out)
+        for s in range(STEPS):
+            nxt = np.empty(B, np.int32)
+            b.step(tok, None, nxt)
+            assert np.array_equal(nxt, out[s]), s
+            tok = nxt
+    finally:
+        a.close()
+        b.close()
+
+
+def test_refused_settings_leave_the_position(um, backend):
+    W, _ = _weights(um)
+    dec = _decoder(um, backend, W, 4, kv_fmt=um.F16)
+    f, i = torch.zeros(B, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    try:
+        with pytest.raises(um.UaiiMoeError) as e:
+            dec.step_sampled(i, f.cpu(), i, f, f, f, i)
+        assert e.value.status == um.INVALID_ARGUMENT and dec.position == 0
+    finally:
+        dec.close()
