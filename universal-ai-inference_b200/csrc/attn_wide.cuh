@@ -391,34 +391,42 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
     }
     shrink = row_shrink(mx);
   }
-  constexpr bool kAhead = sizeof(Q) == 2;  // (f32 rows do not fit twice)
-  Block all[kAhead ? HD / 64 : 1];
-  if constexpr (kAhead)
+  Block all[SPLIT_Q ? 1 : HD / 64];  // (f32 rows are too long to hold whole)
+  if constexpr (!SPLIT_Q)
 #pragma unroll
     for (int h = 0; h < HD / 64; ++h) load(h, all[h]);
 #pragma unroll
   for (int h = 0; h < HD / 64; ++h) {
-    Block& v = all[kAhead ? h : 0];
-    if constexpr (!kAhead) load(h, v);
+    Block& v = all[SPLIT_Q ? 0 : h];
+    if constexpr (SPLIT_Q) load(h, v);
     uint32_t c[32];
+    if constexpr (!SPLIT_Q) {  // pairs as they are
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int d = operand_dim<F>(2 * j);
-      const float y0 = (float)v.e[d] * shrink, y1 = (float)v.e[d + 1] * shrink;
-      __half2 e = __floats2half2_rn(y0, y1);
-      if constexpr (SPLIT_Q && F == kKvF16) {
-        // K may hold infinities: both parts have the value's sign, and neither is 0 (their products would be NaN)
-        // unless the value is.  Rounded towards zero they still leave no more than 2^-22 of the largest.
-        e = __halves2half2(toward_zero(y0), toward_zero(y1));
-        if (part) {
-          const float2 z = __half22float2(e);
-          e = __halves2half2(toward_zero(y0 - z.x, y0), toward_zero(y1 - z.y, y1));
-        }
-      } else if (SPLIT_Q && part) {
-        const float2 z = __half22float2(e);
-        e = __floats2half2_rn(y0 - z.x, y1 - z.y);
+      for (int j = 0; j < 32; ++j) {
+        const int d = operand_dim<F>(2 * j) / 2;
+        const uint4 x = v.u[d >> 2];
+        c[j] = (d & 3) == 0 ? x.x : (d & 3) == 1 ? x.y : (d & 3) == 2 ? x.z : x.w;
       }
-      c[j] = half2_bits(e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int d = operand_dim<F>(2 * j);
+        const float y0 = (float)v.e[d] * shrink, y1 = (float)v.e[d + 1] * shrink;
+        __half2 e = __floats2half2_rn(y0, y1);
+        if constexpr (F == kKvF16) {
+          // K may hold infinities: both parts have the value's sign, and neither is 0 (their products would be NaN)
+          // unless the value is.  Rounded towards zero they still leave no more than 2^-22 of the largest.
+          e = __halves2half2(toward_zero(y0), toward_zero(y1));
+          if (part) {
+            const float2 z = __half22float2(e);
+            e = __halves2half2(toward_zero(y0 - z.x, y0), toward_zero(y1 - z.y, y1));
+          }
+        } else if (part) {
+          const float2 z = __half22float2(e);
+          e = __floats2half2_rn(y0 - z.x, y1 - z.y);
+        }
+        c[j] = half2_bits(e);
+      }
     }
     umma::tmem_st32(taddr + 32 * h, c);
   }
