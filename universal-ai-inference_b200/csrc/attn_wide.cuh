@@ -224,6 +224,10 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
 
 // ---------------------------------------------------------------- products
 
+// The tensor cores cut sums off where they should round (a loss of 1.5e-8 of an f32 sum at each of its additions, 8 a
+// key tile of f32 queries: 5e-6 in 46 tiles), so f32 sums are taken out after this many tiles and added up in f32.
+constexpr int kDrain = 5;
+
 // One warp per row tile r: the scores of a half, then, when its weights are there, O += P V; when those products are
 // done, the half of the next key tile takes P's place.  The whole warp stays together and one lane issues: the descriptors
 // then live in uniform registers.
@@ -246,12 +250,13 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
   auto scores = [&](int o, int h) {  // 32 rows (4 KB) of K; 32 bytes a step, 64 dimensions a swizzled block
     const uint64_t k = operand(o) + (uint64_t)(h * (32 * 128) >> 4);
     if (umma::elect_one()) {
+      // the rests first: every addition cuts the running sum off, and theirs is small
 #pragma unroll
-      for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
+      for (int part = SPLIT_Q; part >= 0; --part)
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks)
           umma::mma_f16_ts(ts + 32 * h, q + 64 * part + 8 * ks, k + (uint64_t)(((ks >> 2) * (kTile * 128) + (ks & 3) * 32) >> 4),
-                           kIdS, part | ks);
+                           kIdS, part != SPLIT_Q || ks);
       umma::mma_commit(&sh.s_full[r][h]);
     }
     __syncwarp();
@@ -259,6 +264,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
   while (w.next(x, p, a, seqs)) {
     const int n = tiles_of(x), first = p.split_keys ? r : 0, step = p.split_keys ? 2 : 1;
     if (n <= 0) continue;
+    int summed = 0;
     wait(&sh.q_full, pieces++ & 1);
     if (first < n) {
       const int o = (count + first) % Wd::kOps;
@@ -266,7 +272,8 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
       scores(o, 0);
       scores(o, 1);
     }
-    for (int i = first; i < n; i += step, ++mine) {
+    for (int i = first; i < n; i += step, ++mine, ++summed) {
+      if (SPLIT_Q && summed == kDrain) summed = 0;  // (the sums are taken out, by then)
       const int o = (count + i) % Wd::kOps, on = (count + i + step) % Wd::kOps;
       const uint64_t v = operand(o) + (Wd::kOpK >> 4);
 #pragma unroll
@@ -277,7 +284,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
           for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
-              umma::mma_f16_ts(to, ts + 32 * h + 16 * part + 8 * ks, v + 2 * (2 * h + ks), kIdO, i != first || h || part || ks);
+              umma::mma_f16_ts(to, ts + 32 * h + 16 * part + 8 * ks, v + 2 * (2 * h + ks), kIdO, summed || h || part || ks);
           umma::mma_commit(&sh.o_done[r][h]);
           if (h) umma::mma_commit(&sh.op_empty[o]);
         }
@@ -351,12 +358,10 @@ __device__ __forceinline__ int operand_dim(int pos) {
   return (pos & ~15) | ((pos & 6) << 1) | ((pos & 8) >> 2) | (pos & 1);
 }
 
-// y rounded towards zero, but to the smallest half of s's sign rather than to 0 unless s is 0.
-__device__ __forceinline__ __half toward_zero(float y, float s) {
-  const __half h = __float2half_rz(y);
+// h, but the smallest half of s's sign rather than 0 unless s is 0.
+__device__ __forceinline__ __half but_zero(__half h, float s) {
   return __hisnan(h) || (__half_as_ushort(h) & 0x7fff) || s == 0.f ? h : __ushort_as_half(s < 0.f ? 0x8001 : 1);
 }
-__device__ __forceinline__ __half toward_zero(float y) { return toward_zero(y, y); }
 
 // This thread's row of q (null: zeros) into tensor memory as operand `part` (1: the rests of a split); returns the power
 // of two by which a split row was multiplied.
@@ -415,11 +420,11 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
         __half2 e = __floats2half2_rn(y0, y1);
         if constexpr (F == kKvF16) {
           // K may hold infinities: both parts have the value's sign, and neither is 0 (their products would be NaN)
-          // unless the value is.  Rounded towards zero they still leave no more than 2^-22 of the largest.
-          e = __halves2half2(toward_zero(y0), toward_zero(y1));
+          // unless the value is.  With the leading part rounded towards zero the rest leaves 2^-22 of the largest.
+          e = __halves2half2(but_zero(__float2half_rz(y0), y0), but_zero(__float2half_rz(y1), y1));
           if (part) {
             const float2 z = __half22float2(e);
-            e = __halves2half2(toward_zero(y0 - z.x, y0), toward_zero(y1 - z.y, y1));
+            e = __halves2half2(but_zero(__float2half_rn(y0 - z.x), y0), but_zero(__float2half_rn(y1 - z.y), y1));
           }
         } else if (part) {
           const float2 z = __half22float2(e);
@@ -457,6 +462,47 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
     const Q* src = q_row<Q>(a, p, x, p.split_keys ? row : 128 * r + row, lim);
     float m = -INFINITY, l = 0.f, row_f = 1.f, vtop = 0x1p-100f;
     uint32_t hidden = 0;
+    const int64_t at_row = x.slot * 256 + 128 * r + row;
+    float* part = p.part + at_row * HD;
+    int summed = 0;           // key tiles in the sums that tensor memory holds
+    float drained_m = 0.f;    // the reference of the sums taken out before
+    bool drained = false;
+    // The sums so far to the workspace, added to those taken out before.
+    auto drain = [&]() {
+      umma::bounded_wait(&sh.o_done[r][1], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
+      umma::tc_fence_after();
+      const float up = F == kKvF16 ? 1.f : 0.5f * vtop, old = drained_m == m ? 1.f : ex2(drained_m - m);
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t u[32];
+        tmem_ld32(to + 32 * c, u);
+        umma::tmem_ld_wait();
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(u[j]) * up;
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          // 8-bit pieces: even dimensions of 16 lie before the odd ones
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] = F == kKvF16 ? y[j + i] : y[(j & 16) + ((j & 15) >> 1) + (i >> 1) + 8 * (i & 1)];
+          if (SPLIT_Q && drained) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(part + 32 * c + j + i);
+              z[i] = fmaf(v.x, old, z[i]);
+              z[i + 1] = fmaf(v.y, old, z[i + 1]);
+              z[i + 2] = fmaf(v.z, old, z[i + 2]);
+              z[i + 3] = fmaf(v.w, old, z[i + 3]);
+            }
+          }
+          store8(part + 32 * c + j, z);
+        }
+      }
+      umma::tc_fence_before();
+      drained = true;
+      drained_m = m;
+    };
     if (n > 0) {
       if (p.split_keys) asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's products with q are done
       const float shrink = put_q<F, HD, SPLIT_Q, Q>(src, a.q_vec, r, tm + 128 + 64 * r);
@@ -465,7 +511,11 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
       __syncwarp();
       if (lane == 0) umma::mbar_arrive(&sh.q_full);
     }
-    for (int i = first; i < n; i += step, ++mine) {
+    for (int i = first; i < n; i += step, ++mine, ++summed) {
+      if (SPLIT_Q && summed == kDrain) {
+        drain();
+        summed = 0;
+      }
       const int at = count + i, o = at % Wide<F, HD>::kOps;
       umma::bounded_wait(&sh.op_full[o], (at / Wide<F, HD>::kOps) & 1, &sh.abort, a.err, kErrKvCopy);  // the column factors
 #pragma unroll 1
@@ -550,7 +600,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
             shrink_o *= c;
             m = t;
           }
-          if ((h || i != first) && __any_sync(0xffffffffu, shrink_o != 1.f)) {
+          if ((h || summed) && __any_sync(0xffffffffu, shrink_o != 1.f)) {
             // the products made so far, up to those of the half before, rest
             umma::bounded_wait(&sh.o_done[r][h ^ 1], (h ? mine : mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
             umma::tc_fence_after();
@@ -580,30 +630,9 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
       }
     }
     count += n > 0 ? n : 0;
-    const int64_t at = x.slot * 256 + 128 * r + row;
-    float* part = p.part + at * HD;
-    *reinterpret_cast<float2*>(p.ml + 2 * at) = make_float2(m, hidden ? -l : l);
+    *reinterpret_cast<float2*>(p.ml + 2 * at_row) = make_float2(m, hidden ? -l : l);
     if (n > first) {
-      umma::bounded_wait(&sh.o_done[r][1], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
-      umma::tc_fence_after();
-      const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        uint32_t u[32];
-        tmem_ld32(to + 32 * c, u);
-        umma::tmem_ld_wait();
-        float y[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(u[j]) * up;
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          // 8-bit pieces: even dimensions of 16 lie before the odd ones
-          float z[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] = F == kKvF16 ? y[j + i] : y[(j & 16) + ((j & 15) >> 1) + (i >> 1) + 8 * (i & 1)];
-          store8(part + 32 * c + j, z);
-        }
-      }
+      drain();
     } else {
 #pragma unroll 4
       for (int j = 0; j < HD; j += 4) reinterpret_cast<float4*>(part + j)[0] = make_float4(0.f, 0.f, 0.f, 0.f);

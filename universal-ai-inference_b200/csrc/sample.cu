@@ -234,9 +234,10 @@ struct Row {
     const uint32_t k = atomicAdd(&sh.listed[set], 1u);
     if (k < kList) list[set * kList + k] = i;
   }
-  // Of the tokens that the CTAs have listed, ranked by their logits (and so by weight), the cut at which the leading
-  // ones reach `goal`, `above` lying above them all.  False, with their count in f->equal, if they are more than a list
-  // holds.  Their logits are read again: they tell equal weights apart.
+  // Of the tokens that the CTAs have listed, ranked by weight and then by logit (read again: should the exponential not
+  // rise with its argument to the last bit, the ranking is still the one that the cut is applied by), the cut at which
+  // the leading ones reach `goal`, `above` lying above them all.  False, with their count in f->equal, if they are more
+  // than a list holds.
   template <bool MASS>
   __device__ bool rank_listed(uint64_t goal, uint64_t above, Found* f) {
     const int t = threadIdx.x;
@@ -267,10 +268,11 @@ struct Row {
       uint32_t same = 0, equal = 0, before = 0;  // of the same logit; of the same weight, and those with a larger logit
       for (uint32_t j = 0; j < listed; ++j) {
         const uint2 y = all[j];
-        over += y.y > me.y ? (MASS ? y.x : 1u) : 0u;
+        const bool level = y.x == me.x, higher = level && y.y > me.y;
+        over += y.x > me.x || higher ? (MASS ? y.x : 1u) : 0u;
         same += y.y == me.y;
-        equal += y.x == me.x;
-        before += y.x == me.x && y.y > me.y;
+        equal += level;
+        before += higher;
       }
       const uint64_t each = MASS ? me.x : 1;
       if (over < goal && goal <= over + same * each) {  // (equal tokens write the same)
