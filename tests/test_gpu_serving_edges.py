@@ -194,3 +194,32 @@ def test_sizes_that_are_refused(um, backend):
     refused(um.INVALID_ARGUMENT, "cache sizes", backend.kv_append, many, x, x, pos)
     refused(um.INVALID_ARGUMENT, "cache sizes", backend.prefix_attention, x, many, pos, x)
     backend.synchronize()
+
+
+@pytest.mark.parametrize("fmt,hd", [("e4m3", 128), ("f16", 64)])
+def test_attention_long_f32_sums_do_not_shrink(um, backend, fmt, hd):
+    """Many rows over thousands of keys: an accumulator that is cut off at each addition loses 2^-24 of itself on average,
+    so 40 additions to a sum that grows from nothing lose 40 / 2 * 2^-24 of it, 1.2e-6; scores (8 additions, up to 4
+    in magnitude) and the roundings of the reference's rows add as much again.  Bar on the whole result: 2.5e-6."""
+    rng = np.random.default_rng(9)
+    b, h, g, t, p_len, own_len = 64, 8, 7, 4, 7741, 70
+    prefix = Cache(um, fmt, 1, h, p_len, hd, rng)
+    own = Cache(um, fmt, b, h, own_len, hd, rng)
+    q = torch.randn((b, t, h * g, hd), device="cuda")
+    out = torch.empty_like(q)
+    lens = dev(np.full(b, own_len, np.int32))
+    backend.prefix_attention(q, own.view, lens, out, prefix=prefix.view, prefix_len=p_len)
+    backend.synchronize()
+    sees = torch.arange(own_len, device="cuda")[None, :] <= own_len - t + torch.arange(t, device="cuda")[:, None]
+    off = whole = 0.0
+    (pk, ok), (pv, ov) = ((dev(prefix.values(n)), dev(own.values(n))) for n in "kv")
+    for kh in range(h):
+        for i in range(b):
+            k, v = torch.cat([pk[0, kh], ok[i, kh]]), torch.cat([pv[0, kh], ov[i, kh]])
+            x = q[i, :, kh * g:(kh + 1) * g].double()
+            s = torch.einsum("tgd,nd->tgn", x, k) / hd ** 0.5
+            s[:, :, p_len:].masked_fill_(~sees[:, None, :], float("-inf"))
+            want = torch.softmax(s, -1) @ v
+            off += float((out[i, :, kh * g:(kh + 1) * g].double() - want).square().sum())
+            whole += float(want.square().sum())
+    assert (off / whole) ** 0.5 <= 2.5e-6

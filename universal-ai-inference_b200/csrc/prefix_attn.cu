@@ -247,7 +247,8 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     p.workers = p.grid * each;
     // A piece costs more than its keys (sums out, other queries in: 58000 cycles for 7 wide tiles in two pieces, 41000
     // in one), so every item counts as kWideLead tiles or kNarrowLead steps longer.  64 rows behind 8192 positions, 24 x 4
-    // tokens behind 4101: 62.3 and 66.8 us without, 51.6 and 43.1 with 3 tiles, 49.2 and 41.5 with 7; 32 rows of 4096
+    // tokens behind 4101: 62.3 and 66.8 us without, 51.6 and 43.1 with 3 tiles, 49.2 and 41.5 with 7 (45 with f32 sums
+    // taken out); 32 rows of 4096
     // own positions: 64.1, 62.2, 61.5 and 60.0 us with 0, 1, 2 and 4 steps, 64 rows behind 8192 62.2, 58.2, 57.5, 58.7.
     p.lead = wide ? kWideLead : kNarrowLead;
     p.prefix_units = tiles ? tiles + p.lead : 0;
