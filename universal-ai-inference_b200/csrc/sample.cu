@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   extern __shared__ uint4 dynamic[];
   __shared__ RowShared sh;
   cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();  // this CTA has started: the others may write to its shared memory once all have
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t b = blockIdx.x / ctas, begin = (int64_t)rank * slice;
   const int n = (int)max(int64_t(0), min((int64_t)slice, V - begin));
@@ -397,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const X* __restrict
   if (lane == 0) sh.warp[warp] = top;
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) top = max(top, (uint32_t)sh.warp[i]);
+  cluster.barrier_wait();  // (the reading hid it)
   row.tell(kTop, top);
   cluster.sync();
   for (int i = 0; i < ctas; ++i) top = max(top, (uint32_t)sh.part[kTop][i]);
