@@ -1,4 +1,5 @@
-"""Serving operators where blocks, warps and calls meet one another: sampling rows whose blocks have little to read.
+"""Serving operators where blocks, warps and calls meet one another: sampling rows whose blocks have little to read, and
+faults that one lane clears for the others.
 
 Sampled tokens are held to the definition's exactly (whole-number weights).
 """
@@ -9,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_serving import dev, sample  # noqa: E402
+from test_gpu_serving import Cache, dev, sample  # noqa: E402
 
 
 @pytest.mark.parametrize("half", [False, True])
@@ -30,3 +31,23 @@ def test_sample_rows_of_many_short_blocks(um, backend, half, b, v):
     tok, prob, kept = sample(um, backend, xd, 1.0, min_p=0.9, u=u)  # the next logit is far below 9
     assert np.array_equal(tok, np.where(u < 0.5, np.minimum(at, two), np.maximum(at, two)))
     assert (kept == 2).all() and (prob == 0.5).all()
+
+
+@pytest.mark.parametrize("fmt,half,hd,g,t", [("f16", False, 128, 2, 4), ("f16", True, 64, 2, 8), ("e4m3", False, 64, 1, 7),
+                                             ("e4m3", True, 128, 4, 4), ("f16", True, 128, 4, 2)])
+def test_attention_faults_in_every_position_that_some_tokens_do_not_see(um, backend, fmt, half, hd, g, t):
+    """NaNs in V of every position that only later tokens see, in all dimensions and many sequences: whichever lane of a
+    warp clears a byte, no other lane reads it as it was.  The first tokens' results are as without them, bit for bit."""
+    rng = np.random.default_rng(t)
+    b = 96
+    lens = np.array([t + (i * 7) % 90 for i in range(b)], np.int32)
+    own = Cache(um, fmt, b, 2, int(lens.max()) + 1, hd, rng)
+    q = torch.randn((b, t, 2 * g, hd), device="cuda").to(torch.float16 if half else torch.float32)
+    clean, out = torch.empty_like(q), torch.empty_like(q)
+    backend.prefix_attention(q, own.view, dev(lens), clean)
+    for i, n in enumerate(lens):
+        own.t["v"][0][i, :, n - t + 1:] = float("nan") if fmt == "f16" else 0xff
+    for _ in range(3):
+        backend.prefix_attention(q, own.view, dev(lens), out)
+        backend.synchronize()
+        assert torch.equal(out[:, 0], clean[:, 0]) and out[:, 1:].isnan().all()

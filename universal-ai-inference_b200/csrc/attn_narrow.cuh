@@ -356,6 +356,7 @@ __device__ __noinline__ bool hide_v(uint8_t* v, int from, int to, int lane) {
     any |= bad;
   }
   umma::fence_proxy_async_smem();
+  __syncwarp();  // other lanes read these bytes next (a vote orders no memory)
   return __any_sync(0xffffffffu, any);
 }
 
