@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from test_gpu_serving import Cache, dev, sample  # noqa: E402
+from test_gpu_serving import FMTS, Cache, check_attention, dev, sample  # noqa: E402
 
 
 @pytest.mark.parametrize("half", [False, True])
@@ -51,3 +51,12 @@ def test_attention_faults_in_every_position_that_some_tokens_do_not_see(um, back
         backend.prefix_attention(q, own.view, dev(lens), out)
         backend.synchronize()
         assert torch.equal(out[:, 0], clean[:, 0]) and out[:, 1:].isnan().all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("half", [False, True])
+def test_attention_many_items_of_one_tile(um, backend, fmt, half):
+    """Items of many rows whose keys are one tile (or none): one of the two warps that issue products has nothing to issue
+    between the pieces, and keeps step with them."""
+    lens = [(i * 23) % 65 for i in range(300)]
+    check_attention(um, backend, fmt, half, 128, 3, 8, 3, lens, 0)

@@ -41,7 +41,7 @@ struct WideShared {
   static constexpr int kRawStages = Wide<F, HD>::kRawStages;
   static constexpr int kOps = Wide<F, HD>::kOps;
   uint64_t raw_full[kRawStages], raw_empty[kRawStages], op_full[kOps], op_empty[kOps];
-  uint64_t q_full, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
+  uint64_t q_full, q_seen, s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
   uint32_t tmem;
   int abort;
   alignas(16) float raw_scale[kRawStages][2][kTile];
@@ -266,6 +266,8 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
     if (n <= 0) continue;
     int summed = 0;
     wait(&sh.q_full, pieces++ & 1);
+    if (umma::elect_one()) umma::mbar_arrive(&sh.q_seen);
+    __syncwarp();
     if (first < n) {
       const int o = (count + first) % Wd::kOps;
       wait(&sh.op_full[o], ((count + first) / Wd::kOps) & 1);
@@ -456,6 +458,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
   Piece x;
   int count = 0;            // key tiles of the CTA
   uint32_t mine = 0;        // key tiles of this warpgroup
+  int pieces = 0;           // with keys
   while (w.next(x, p, a, seqs)) {
     const int n = tiles_of(x), step = p.split_keys ? 2 : 1, first = p.split_keys ? r : 0;
     int lim;
@@ -504,6 +507,9 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
       drained_m = m;
     };
     if (n > 0) {
+      // Both issuing warps have seen the piece before's queries: with one tile and split keys the second has nothing to
+      // issue, and nothing else would keep the barrier's phase from passing it by.
+      if (pieces++) umma::bounded_wait(&sh.q_seen, pieces & 1, &sh.abort, a.err, kErrKvCopy);
       if (p.split_keys) asm volatile("bar.sync 1, 256;" ::: "memory");  // the other half's products with q are done
       const float shrink = put_q<F, HD, SPLIT_Q, Q>(src, a.q_vec, r, tm + 128 + 64 * r);
       if constexpr (SPLIT_Q) row_f = 1.f / shrink;
@@ -671,6 +677,7 @@ __global__ void __launch_bounds__(Wide<F, HD>::kThreads, 1)
       }
     }
     umma::mbar_init(&sh.q_full, 8);
+    umma::mbar_init(&sh.q_seen, 2);
     sh.abort = 0;
     umma::fence_barrier_init();
   }
