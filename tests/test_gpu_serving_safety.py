@@ -60,3 +60,27 @@ def test_attention_many_items_of_one_tile(um, backend, fmt, half):
     between the pieces, and keeps step with them."""
     lens = [(i * 23) % 65 for i in range(300)]
     check_attention(um, backend, fmt, half, 128, 3, 8, 3, lens, 0)
+
+
+@pytest.mark.parametrize("g,t,p_len", [(4, 1, 0), (4, 1, 100), (8, 4, 100)])
+def test_attention_calls_in_a_row_with_other_lengths(um, backend, g, t, p_len):
+    """Calls queued back to back share the workspace: each joins the pieces that its own lengths give."""
+    rng = np.random.default_rng(g)
+    b, h, hd = 40, 2, 64
+    own, prefix = Cache(um, "i8", b, h, 400, hd, rng), Cache(um, "i8", 1, h, 128, hd, rng)
+    q = torch.randn((b, t, h * g, hd), device="cuda")
+    lens = [dev(x.astype(np.int32)) for x in (np.full(b, 400), np.arange(b) * 3 % 7, rng.integers(0, 400, b),
+                                             np.where(np.arange(b) % 2, 399, 0))]
+    kw = dict(prefix=prefix.view, prefix_len=p_len) if p_len else {}
+    alone = []
+    for n in lens:
+        out = torch.empty_like(q)
+        backend.prefix_attention(q, own.view, n, out, **kw)
+        backend.synchronize()
+        alone.append(out)
+    order = [0, 1, 0, 2, 3, 1, 2, 0, 3] * 20
+    outs = [torch.empty_like(q) for _ in order]
+    for i, out in zip(order, outs):
+        backend.prefix_attention(q, own.view, lens[i], out, **kw)
+    backend.synchronize()
+    assert all(torch.equal(out, alone[i]) for i, out in zip(order, outs))

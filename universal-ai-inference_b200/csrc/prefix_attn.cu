@@ -62,8 +62,7 @@ struct Pieces {
 };
 
 template <bool OWN>
-__device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan& p, const int32_t* __restrict__ cum, int b, int rho,
-                                            int kvh) {
+__device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan& p, const int32_t* cum, int b, int rho, int kvh) {
   Pieces q{};
   if (!OWN && p.prefix_items == 0) return q;
   const int j = rho / p.by_rt, per = (int)a.own.heads * p.own_nrt, prefix = p.prefix_items * p.prefix_units;
@@ -97,10 +96,11 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
 // order of the workers, prefix first, a warp every WARPS-th.  Bound by latency (lengths, then maxima, then sums: 4 to 8 us
 // whatever the rows); inside the narrow kernel, by the worker that comes last, it cost more (67 against 63 us at 64 rows
 // behind 8192 positions).  px, po: the plans of the kernels that took the prefix and
-// the own items.
+// the own items.  cum is not __restrict__: it is written while this grid waits, and a load of data declared unchanging may
+// be moved in front of the wait.
 template <int HD, typename Q, int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ Plan px,
-                                                   const __grid_constant__ Plan po, const int32_t* __restrict__ cum) {
+                                                   const __grid_constant__ Plan po, const int32_t* cum) {
   constexpr int N = HD / 32, kRows = 4 / WARPS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wr = warp % WARPS;
   const int rows = (int)(a.B * a.T * a.H), row = (int)blockIdx.x * kRows + warp / WARPS;
