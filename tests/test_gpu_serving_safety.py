@@ -84,3 +84,21 @@ def test_attention_calls_in_a_row_with_other_lengths(um, backend, g, t, p_len):
         backend.prefix_attention(q, own.view, lens[i], out, **kw)
     backend.synchronize()
     assert all(torch.equal(out, alone[i]) for i, out in zip(order, outs))
+
+
+def test_sample_refuses_misaligned_arrays(um, backend):
+    """Addresses that are no multiple of an element's size are refused on the host, one argument at a time."""
+    b, v = 2, 8
+    x = torch.zeros((b, v), device="cuda")
+    f, i = torch.zeros(b + 1, device="cuda"), torch.zeros(b + 1, dtype=torch.int32, device="cuda")
+    good = [f, i, f, f, f, i.clone(), f.clone(), i.clone()]  # temperature, top_k, top_p, min_p, u, tokens, probs, kept
+    for at in range(len(good)):
+        for shift in (1, 2, 3):
+            ptrs = [a.data_ptr() + (shift if k == at else 0) for k, a in enumerate(good)]
+            st = um.lib.uaii_moe_sample(backend._h, x.data_ptr(), um.DTYPE_F32, b, v, v, *ptrs)
+            assert st == um.INVALID_ARGUMENT and b"misaligned" in um.lib.uaii_moe_last_error(), (at, shift)
+    st = um.lib.uaii_moe_sample(backend._h, x.data_ptr() + 2, um.DTYPE_F32, b, v, v, *[a.data_ptr() for a in good])
+    assert st == um.INVALID_ARGUMENT
+    st = um.lib.uaii_moe_sample(backend._h, x.data_ptr(), um.DTYPE_F32, b, v, v, *[a.data_ptr() for a in good])
+    assert st == um.OK
+    backend.synchronize()

@@ -297,6 +297,9 @@ bool is_device_ptr(const void* p) noexcept;
 bool layer_args_from_c(const struct uaii_moe_layer* l, LayerArgs* out);
 // The C ABI's cache description, checked (`op` opens the messages).
 Error kv_cache_from_c(const char* op, const struct uaii_moe_kv_cache* s, KvCache* out);
+// sample's per-row arrays: device memory, aligned to their elements (probs and kept may be null).
+Error check_sample_arrays(const char* op, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                          const float* u, const int32_t* tokens, const float* probs, const int32_t* kept);
 // Record `e` as this thread's last error (uaii_moe_last_error) and return its status code.
 int report_status(const Error& e);
 Error cuda_status(cudaError_t st, const char* what);

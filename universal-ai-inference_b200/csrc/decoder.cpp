@@ -256,12 +256,8 @@ class Decoder {
                      const float* min_p, const float* u, int32_t* next, float* probs, float* logits) {
     if (cfg_.vocab > kSampleMaxVocab)
       return Error::make(ErrorCode::NotImplemented, "decoder step_sampled: vocab above " + std::to_string(kSampleMaxVocab));
-    bool device = !probs || is_device_ptr(probs);  // refused before the step, which would leave a position behind
-    for (const void* p : {(const void*)temperature, (const void*)top_k, (const void*)top_p, (const void*)min_p,
-                          (const void*)u, (const void*)next})
-      device = device && is_device_ptr(p);
-    if (!device)
-      return Error::make(ErrorCode::InvalidArgument, "decoder step_sampled: settings and next must be device memory");
+    // refused before the step, which would leave a position behind
+    UAII_TRY(check_sample_arrays("decoder step_sampled", temperature, top_k, top_p, min_p, u, next, probs, nullptr));
     UAII_TRY(step(tokens, logits, nullptr));
     return be_->sample(logits_, false, cfg_.batch, cfg_.vocab, cfg_.vocab, temperature, top_k, top_p, min_p, u, next, probs,
                        nullptr);

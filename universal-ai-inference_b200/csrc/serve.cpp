@@ -58,6 +58,21 @@ Error kv_cache_from_c(const char* op, const uaii_moe_kv_cache* s, KvCache* out) 
   return Error::success();
 }
 
+Error check_sample_arrays(const char* op, const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                          const float* u, const int32_t* tokens, const float* probs, const int32_t* kept) {
+  const void* needed[] = {temperature, top_k, top_p, min_p, u, tokens};
+  const void* optional[] = {probs, kept};
+  for (const void* p : needed) {
+    if (!is_device_ptr(p)) return invalid(std::string(op) + ": arguments must be device memory");
+    if (!aligned(p, 4)) return invalid(std::string(op) + ": misaligned argument");
+  }
+  for (const void* p : optional) {
+    if (p && !is_device_ptr(p)) return invalid(std::string(op) + ": arguments must be device memory");
+    if (!aligned(p, 4)) return invalid(std::string(op) + ": misaligned argument");
+  }
+  return Error::success();
+}
+
 Error MoeCudaBackend::kv_append(const KvCache& c, const void* k, const void* v, bool half, int64_t T, const RowView& s,
                                 const int32_t* pos, const int32_t* n_new) {
   std::lock_guard<std::mutex> lk(mu_);
@@ -132,12 +147,8 @@ Error MoeCudaBackend::sample(const void* logits, bool half, int64_t B, int64_t V
     return Error::make(ErrorCode::NotImplemented, "sample: vocab above " + std::to_string(kSampleMaxVocab));
   if (ld < V) return invalid("sample: rows overlap (ld < vocab)");
   if (B == 0) return Error::success();
-  for (const void* p : {logits, static_cast<const void*>(temperature), static_cast<const void*>(top_k),
-                        static_cast<const void*>(top_p), static_cast<const void*>(min_p), static_cast<const void*>(u),
-                        static_cast<const void*>(tokens)})
-    if (!is_device_ptr(p)) return invalid("sample: arguments must be device memory");
-  if ((probs && !is_device_ptr(probs)) || (kept && !is_device_ptr(kept)))
-    return invalid("sample: arguments must be device memory");
+  if (!is_device_ptr(logits)) return invalid("sample: arguments must be device memory");
+  UAII_TRY(check_sample_arrays("sample", temperature, top_k, top_p, min_p, u, tokens, probs, kept));
   if (!aligned(logits, half ? 2 : 4)) return invalid("sample: misaligned logits");
   UAII_CUDA(cudaSetDevice(device_), "SetDevice");
   UAII_CUDA(launch_sample(logits, half, B, V, ld, temperature, top_k, top_p, min_p, u, tokens, probs, kept, stream_),
