@@ -102,3 +102,38 @@ def test_sample_refuses_misaligned_arrays(um, backend):
     st = um.lib.uaii_moe_sample(backend._h, x.data_ptr(), um.DTYPE_F32, b, v, v, *[a.data_ptr() for a in good])
     assert st == um.OK
     backend.synchronize()
+
+
+def test_sample_from_several_threads_with_other_vocabularies(um):
+    """Backends sample in threads of their own, rows of the largest vocabulary and short ones: no call's launch depends on
+    the shared memory that another one asks for."""
+    import threading
+
+    errors, start = [], threading.Barrier(4)
+
+    def work(v, b, n):
+        be = um.Backend(0)
+        try:
+            x = torch.zeros((b, v), device="cuda")
+            f, i = torch.ones(b, device="cuda"), torch.zeros(b, dtype=torch.int32, device="cuda")
+            torch.cuda.synchronize()
+            tok, zero, u = torch.empty(b, dtype=torch.int32, device="cuda"), f * 0, f * 0.5
+            args = (be._h, x.data_ptr(), um.DTYPE_F32, b, v, v, f.data_ptr(), i.data_ptr(), f.data_ptr(), zero.data_ptr(),
+                    u.data_ptr(), tok.data_ptr(), None, None)
+            start.wait()
+            for _ in range(n):
+                st = um.lib.uaii_moe_sample(*args)
+                assert st == um.OK, um.lib.uaii_moe_last_error()
+            be.synchronize()
+            assert (tok == v // 2).all()
+        except Exception as e:  # noqa: BLE001 (reported by the test)
+            errors.append((v, repr(e)))
+        finally:
+            be.close()
+
+    threads = [threading.Thread(target=work, args=a) for a in ((400000, 1, 20000), (600, 1, 20000), (60000, 1, 20000), (20, 1, 20000))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors

@@ -621,7 +621,8 @@ cudaError_t launch_sample(const void* logits, bool half, int64_t B, int64_t V, i
   const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && ld * (int64_t)esz % 16 == 0;
   const int smem = kFixed + (int)slice * 4;
   auto run = [&](auto kern, const auto* x) -> cudaError_t {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // the limit of the kernel, not this call's: another backend's thread may be between its own two calls
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFixed + 4 * kMaxSlice);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(B * ctas));
