@@ -1,0 +1,182 @@
+"""Attention where rows, scores and lengths are far from alike: V rows of very unequal size, keys that weigh nothing, long
+walks of one warp.
+
+Reference: the definition in 64 bits over the stored rows.  With p_j the probabilities and e_j the bound of a score's error,
+2^-18 * scale * sum_d |q_d k_jd| (f32 sums of 16-element products: at most 16 roundings of 2^-23 of the summed magnitudes,
+and a split of q to 2^-22), a result may be off by
+    sum_j p_j e_j |v_j|  +  (sum_j p_j e_j) sum_j p_j |v_j|          the scores' errors, in weights and denominator
+  + ((n / 16 + 64) 2^-23 + 2^-20) sum_j p_j |v_j|                    sums over n positions; exponentials and scales
+  + n 2^-32 max_j (p_j max_d |v_jd|)                                 weights that f16's smallest step cuts: at most 2^-25
+                                                                     each, where the largest product of a weight and a
+                                                                     row's scale is 2^7 or more
+f16 results add a rounding of p and of the result: 2^-11 (sum_j p_j |v_j| + |result|) + 2^-25.
+"""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_serving import FMTS, code, dev, encode, values  # noqa: E402
+
+
+class Rows:
+    """A cache of given rows: k, v [batch, heads, positions, head_dim]."""
+
+    def __init__(self, um, fmt, k, v):
+        self.val, t = {}, {}
+        for n, x in (("k", k), ("v", v)):
+            c, s = (x.astype(np.float16), None) if fmt == "f16" else encode(x, fmt)
+            self.val[n] = dev(values(c, s, fmt))
+            t[n], t[n + "s"] = dev(c), None if s is None else dev(s)
+        self.t = t
+        self.view = um.kv_cache(code(um, fmt), t["k"], t["v"], t["ks"], t["vs"])
+
+
+def definition(q, own, lens, prefix=None, p_len=0, scale=None):
+    """(result, tolerance for f32 results, sum p |v|), all in 64 bits on the device; q [B, T, H, d]."""
+    b, t, hq, d = q.shape
+    h = own.val["k"].shape[1]
+    g = hq // h
+    scale = scale or d ** -0.5
+    q = q.double().view(b, t, h, g, d)
+    out, tol, mag = (torch.zeros_like(q) for _ in range(3))
+    for i in range(b):
+        for kh in range(h):
+            k, v = own.val["k"][i, kh, :lens[i]], own.val["v"][i, kh, :lens[i]]
+            if p_len:
+                k = torch.cat([prefix.val["k"][0, kh, :p_len], k])
+                v = torch.cat([prefix.val["v"][0, kh, :p_len], v])
+            n = len(k)
+            if n == 0:
+                continue
+            x = q[i, :, kh]
+            sees = torch.arange(n, device="cuda") < p_len + torch.arange(t, device="cuda")[:, None] + lens[i] - t + 1
+            sees |= torch.arange(n, device="cuda") < p_len
+            s = (scale * x @ k.T).masked_fill(~sees[:, None], float("-inf"))
+            p = torch.softmax(s, -1).nan_to_num(0.0)
+            e = p * (2.0 ** -18 * scale * x.abs() @ k.abs().T)
+            w, peak = p @ v.abs(), (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+            out[i, :, kh], mag[i, :, kh] = p @ v, w
+            tol[i, :, kh] = (e @ v.abs() + e.sum(-1, keepdim=True) * w + ((n / 16 + 64) * 2.0 ** -23 + 2.0 ** -20) * w
+                             + n * 2.0 ** -32 * peak)
+    return tuple(x.view(b, t, hq, d) for x in (out, tol, mag))
+
+
+def check(um, backend, q, own, lens, prefix=None, p_len=0, scale=0.0):
+    out = torch.full_like(q, 9.0)
+    backend.prefix_attention(q, own.view, dev(np.array(lens, np.int32)), out, prefix=prefix.view if prefix else None,
+                             prefix_len=p_len, scale=scale)
+    backend.synchronize()
+    want, tol, mag = definition(q, own, lens, prefix, p_len, scale)
+    if q.dtype is torch.float16:
+        tol = tol + 2.0 ** -11 * (mag + want.abs()) + 2.0 ** -25
+        over = want.abs() - tol >= 65520.0  # beyond the type: an infinity (and near its end, either)
+        assert (out[over] == torch.copysign(torch.full_like(want[over], float("inf")), want[over])).all()
+        edge = want.abs() + tol >= 65520.0
+        out, want, tol = (torch.where(edge, torch.zeros_like(x), x) for x in (out, want, tol))
+    off = (out.double() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3].tolist(), float((off / tol).nan_to_num(1e30).max()),
+                           float((off.amax() / want.abs().amax())))
+
+
+def queries(b, t, hq, d, half, rng, lead=4.0):
+    """Random queries whose dimension 0 is `lead`: a key's dimension 0 then moves all their scores alike."""
+    q = rng.standard_normal((b, t, hq, d))
+    q[..., 0] = lead
+    return dev(q.astype(np.float16 if half else np.float32))
+
+
+def random_rows(rng, *shape):
+    k, v = (rng.standard_normal(shape).astype(np.float32) for _ in range(2))
+    k[..., 0] = 0
+    return k, v
+
+
+SHAPES = [(4, 1), (4, 4), (7, 4)]  # query heads of a kv head, tokens: items of 4, 16 and 28 rows
+
+
+# ---------------------------------------------------------------- V rows of unequal size
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", SHAPES)
+@pytest.mark.parametrize("ratio", [1e3, 1e6, 1e9, 1e12])
+@pytest.mark.parametrize("nats", [4.0, 18.0, 100.0])
+def test_a_large_v_row_of_little_weight(um, backend, fmt, half, g, t, ratio, nats):
+    """One V row is `ratio` times larger than the others, its key `nats` below them: whatever it weighs, the others keep
+    their bits (in the own positions at three places, and in the prefix)."""
+    rng = np.random.default_rng(int(nats) + g + t)
+    b, h, d, n, p_len = 3, 2, 128, 200, 140
+    k, v = random_rows(rng, b, h, n, d)
+    pk, pv = random_rows(rng, 1, h, p_len, d)
+    for x, y, at in ((k[0], v[0], 0), (k[1], v[1], n // 2), (k[2], v[2], n - t - 1), (pk[0], pv[0], 70)):
+        x[:, at] = 0
+        x[:, at, 0] = -nats * d ** 0.5 / 4.0
+        y[:, at] *= ratio
+    own, prefix = Rows(um, fmt, k, v), Rows(um, fmt, pk, pv)
+    q = queries(b, t, g * h, d, half, rng)
+    check(um, backend, q, own, [n] * b)
+    check(um, backend, q, own, [n, n, n - 70], prefix, 70)   # (the prefix's large row is its first unseen one)
+    check(um, backend, q, own, [n, 60, n - 70], prefix, p_len)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", SHAPES)
+def test_a_large_v_row_that_earlier_tokens_do_not_see(um, backend, fmt, half, g, t):
+    """The last token's V row is 1e8 times larger: the tokens before it, which do not see it, keep their bits."""
+    rng = np.random.default_rng(g)
+    b, h, d, n = 2, 2, 64, 90
+    k, v = random_rows(rng, b, h, n, d)
+    v[:, :, -1] *= 1e8
+    check(um, backend, queries(b, t, g * h, d, half, rng), Rows(um, fmt, k, v), [n, n])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", SHAPES)
+@pytest.mark.parametrize("v_up", [-24, 24])
+@pytest.mark.parametrize("k_up", [-120.0, 0.0, 120.0])
+def test_v_rows_that_grow_or_shrink_along_the_sequence(um, backend, fmt, half, g, t, v_up, k_up):
+    """V's size changes by 2^v_up from the first position to the last, the scores by k_up nats: the largest product of both
+    moves along the sequence, with and against the largest score."""
+    rng = np.random.default_rng(g + t)
+    b, h, d, n = 2, 1, 64, 420
+    k, v = random_rows(rng, b, h, n, d)
+    along = np.linspace(0, 1, n)
+    v *= 2.0 ** (v_up * along)[:, None].astype(np.float32)
+    k = (0.5 * k).astype(np.float32)
+    k[..., 0] = k_up * along * d ** 0.5 / 4.0
+    check(um, backend, queries(b, t, g * h, d, half, rng), Rows(um, fmt, k, v), [n, n - 130])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", SHAPES)
+@pytest.mark.parametrize("nats", [12.0, 40.0])
+def test_a_heavy_position_whose_v_is_zero(um, backend, fmt, half, g, t, nats):
+    """Nearly all weight lies on a position whose V row is zero: the result is the others' small share, to its own bits."""
+    rng = np.random.default_rng(g)
+    b, h, d, n = 2, 2, 128, 150
+    k, v = random_rows(rng, b, h, n, d)
+    k[0, :, 0, 0] = k[1, :, 77, 0] = nats * d ** 0.5 / 4.0
+    v[0, :, 0] = v[1, :, 77] = 0
+    check(um, backend, queries(b, t, g * h, d, half, rng), Rows(um, fmt, k, v), [n, n])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", SHAPES)
+@pytest.mark.parametrize("size", [1e-20, 1e-3, 1e15])
+def test_v_of_any_size(um, backend, fmt, half, g, t, size):
+    """All V rows tiny or huge (f16 results: within their type)."""
+    rng = np.random.default_rng(g)
+    b, h, d, n = 2, 2, 64, 150
+    k, v = random_rows(rng, b, h, n, d)
+    if half and size > 1:
+        size = 1e4
+    check(um, backend, queries(b, t, g * h, d, half, rng), Rows(um, fmt, k, (v * size).astype(np.float32)), [n, n - 7])

@@ -18,10 +18,17 @@ constexpr int kWarps = 4;        // narrow: warps of a CTA
 constexpr int kNarrowCtas = 3;   // narrow: CTAs per SM (wide: one)
 constexpr int kMaxScan = 512;    // sequences whose unit counts a CTA sums itself
 constexpr float kLog2e = 1.4426950408889634f;
-// Probabilities are 2^(s - m + 8) (in sums and denominators alike), and m follows the running maximum only when that
-// rises by more than 6: the sums are then seldom rescaled, weights stay below 2^14 (2^15 with V's scale, a fraction
-// below 2), and f16 keeps 11 bits of each down to 2^-22 of the largest.
-constexpr float kLift = 8.0f, kSlack = 6.0f;
+// A position's weight is 2^(s - m + 8) in the denominator, and that times V's row scale (1 in an f16 cache) where it meets
+// V's bytes.  Only the second becomes f16, so a row's reference m is a whole number at or above the largest product 2^s vs
+// so far, not the largest score: a V row much larger than the others does not push them out of f16's range unless its
+// product outweighs theirs.  (A reference made from the scales alone lost 2e-4 of a result beside a row 10^6 times
+// larger whose own weight was 0, and all of it beside one 10^12 times larger.)  m moves only when a product has come to
+// be near f16's end: the sums are then seldom rescaled, and f16 keeps 11 bits of a product down to 2^-22 of the largest.
+// The denominator is f32 and may lie far from 1; V rows of scale 0, whose products ask for no reference, are held within
+// it by kOver.
+constexpr float kLift = 8.0f, kSlack = 6.0f, kOver = 96.0f;
+constexpr float kMostProduct = 15.f, kMostWeight = 110.f;  // binary orders
+constexpr float kLeastScale = 0x1p-96f;
 
 // A stored row, and a copied tile of KEYS rows of K or V: boxes of at most 128 bytes a row (the swizzle span).
 template <int F, int HD, int KEYS>
@@ -70,7 +77,7 @@ struct Plan {
   int workers;             // shares of the work: wide CTAs or narrow warps
   Div by_G, by_rt, by_own_rows, by_own_nrt, by_prefix_nrt, by_prefix_units, by_workers;
   float* part;             // partial sums [slot][slot_rows][hd]
-  float* ml;               // (maximum, denominator) of each partial row
+  float* ml;               // (reference, denominator) of each partial row
 };
 
 __device__ __forceinline__ int own_length(const PrefixAttnArgs& a, int64_t b, bool report) {
@@ -102,6 +109,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// log2 of a V scale's size, to a tenth: an f32's bits as a number (straight lines between powers of two, never above it;
+// 0 counts as 2^-127).
+__device__ __forceinline__ float log2_scale(float vs) {
+  return fmaf((float)(__float_as_int(vs) & 0x7fffffff), 0x1p-23f, -127.f);
+}
+// The reference after positions with this largest score and largest product: whole numbers, so that neither the factors nor
+// the differences to them round.
+__device__ __forceinline__ float next_reference(float m, float top, float product) {
+  return fmaxf(fmaxf(m, ceilf(product)), ceilf(top) - kOver);
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 

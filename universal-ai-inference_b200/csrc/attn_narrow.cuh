@@ -30,12 +30,11 @@ struct Rows {
   // The two parts of a weight resolve 2^-24, f16's smallest step.  Smaller weights are added in passes of their own,
   // 20 binary orders at a time, raised to [2^-6, 2^14): only very uneven scores (22 e-foldings) need them.
   static constexpr bool kFar = FOLD;
-  static constexpr float kNear = -24.f;
+  static constexpr float kNear = 0x1p-24f;
   float o[HD / 8][4];
-  float m[kPer], l[kPer];
-  float f[kPer];         // score factor: scale * log2(e), and the power of two taken out of a folded row of q
-  int lim[kPer];         // positions the row sees
-  float vtop;                // a power of two above every V scale so far (8-bit formats)
+  float m[kPer], l[kPer];  // the reference (attn_common.cuh), the denominator
+  float f[kPer];           // score factor: scale * log2(e), and the power of two taken out of a folded row of q
+  int lim[kPer];           // positions the row sees
 
   // Leading part and rest.  Where an f16 cache holds an infinity, the rest is 0 * inf.
   static __device__ __forceinline__ float join(float lead, float rest) {
@@ -44,61 +43,53 @@ struct Rows {
   }
 
   __device__ __forceinline__ void clear() {
-    {
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
+    for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
 #pragma unroll
-      for (int r = 0; r < kPer; ++r) {
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-      }
+    for (int r = 0; r < kPer; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
     }
-    vtop = 0x1p-100f;
   }
 
-  // Keys [key, key + 8 NT) of the tile at k_base / v_base, which starts at position pos0 and of
-  // which some row sees the first `left`; masked says that some row may not see all of them.  a(ks, frag) gives
-  // the query operands.
+  // Keys [key, key + 8 NT) of the tile at k_base / v_base, which starts at position pos0; masked says that some row may not
+  // see all of them.  a(ks, frag) gives the query operands.
   template <int NT, bool masked, typename A>
-  __device__ __forceinline__ void step(uint32_t k_base, uint32_t v_base, const float* ks, const float* vs, int key,
-                                       int left, int pos0, A&& a) {
+  __device__ __forceinline__ void step(uint32_t k_base, uint32_t v_base, const float* ks, const float* vs, int key, int pos0, A&& a) {
     const int lane = threadIdx.x & 31, tq = lane & 3, mi = lane >> 3, r8 = lane & 7;
     float s[NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.f;
     // scores: four 16-byte pieces of eight keys at a time
 #pragma unroll
     for (int c = 0; c < kPieces; c += 4) {
       constexpr int kSteps = F == kKvF16 ? 2 : 4;
       uint32_t q[kSteps][4];
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j)
-        a((F == kKvF16 ? c / 2 : c) + j, q[j]);
+      for (int j = 0; j < kSteps; ++j) a((F == kKvF16 ? c / 2 : c) + j, q[j]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         uint32_t w[4];
         ldsm4(w, piece<F, HD, KEYS>(k_base, key + 8 * n + r8, c + mi));
         if constexpr (F == kKvF16) {
-          {
-            mma16816(s[n], q[0], w[0], w[1]);
-            mma16816(s[n], q[1], w[2], w[3]);
-          }
+          mma16816(s[n], q[0], w[0], w[1]);
+          mma16816(s[n], q[1], w[2], w[3]);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t b0, b1;
             unpack<F, false>(w[j], b0, b1);
-        mma16816(s[n], q[j], b0, b1);
+            mma16816(s[n], q[j], b0, b1);
           }
         }
       }
     }
-    // columns 2 tq, 2 tq + 1 of each eight keys: K scales, and V scales as fractions of a power of two
-    float kf[NT][2], vf[NT][2];
+    // columns 2 tq, 2 tq + 1 of each eight keys: K and V scales
+    float kf[NT][2], vf[NT][2], large = 0.f;  // log2 of this lane's largest V scale
     if constexpr (F != kKvF16) {
       float most = 0.f;
 #pragma unroll
@@ -107,109 +98,110 @@ struct Rows {
         const float2 y = *reinterpret_cast<const float2*>(vs + key + 8 * n + 2 * tq);
         kf[n][0] = x.x; kf[n][1] = x.y;
         vf[n][0] = y.x; vf[n][1] = y.y;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (masked && key + 8 * n + 2 * tq + i >= left) vf[n][i] = 0.f;  // nothing is stored there
-          most = fmaxf(most, vf[n][i]);                                    // (a NaN shows in its products, not here)
-        }
+        most = fmaxf(most, fmaxf(fabsf(y.x), fabsf(y.y)));  // (a NaN shows in its products, not here)
       }
-      if (__any_sync(0xffffffffu, most >= vtop)) raise_v(most);
-      const float inv = __uint_as_float(0x7f800000u - __float_as_uint(vtop));  // 2 / vtop
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        vf[n][0] *= inv;
-        vf[n][1] *= inv;
-      }
+      large = log2_scale(most);
     }
-    // exponents against the reference; a lane checks its own, the row's maximum is only made when one is too large
-    bool grew = false;
-    float x[kPer][NT][2];
-    auto exponents = [&]() {
 #pragma unroll
-        for (int r = 0; r < kPer; ++r) {
-          const float off = kLift - (m[r] == -INFINITY ? 0.f : m[r]);
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              x[r][n][i] = fmaf(s[n][2 * r + i], F == kKvF16 ? f[r] : kf[n][i] * f[r], off);
-        }
-    };
+      for (int i = 0; i < 2; ++i)
+        if constexpr (FOLD) s[n][i] = join(s[n][i], s[n][2 + i]);
     auto seen = [&](int r, int n, int i) { return !masked || pos0 + key + 8 * n + 2 * tq + i < lim[r]; };
+    auto factor = [&](int r, int n, int i) {
+      if constexpr (F == kKvF16) return f[r];
+      else return kf[n][i] * f[r];
+    };
+    // exponents against the reference as it is; a lane checks its own, and a row's maxima are only made when a product may
+    // be too large
+    float x[kPer][NT][2];
+    bool over = false;
+    auto exponents = [&](int r) {
+      const float off = kLift - (m[r] == -INFINITY ? 0.f : m[r]);
+      float most = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if constexpr (FOLD) s[n][i] = join(s[n][i], s[n][2 + i]);
-    exponents();
-    float mx[kPer];
+        for (int i = 0; i < 2; ++i) {
+          x[r][n][i] = fmaf(s[n][2 * r + i], factor(r, n, i), off);
+          if (seen(r, n, i)) most = fmaxf(most, x[r][n][i]);
+        }
+      over |= most + large > kMostProduct || most > kMostWeight || (m[r] == -INFINITY && most > -INFINITY);
+    };
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) exponents(r);
+    if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
-        mx[r] = -INFINITY;
+        float top = -INFINITY, product = -INFINITY;  // the largest score, the largest product
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            if (seen(r, n, i)) mx[r] = fmaxf(mx[r], x[r][n][i]);
-        grew |= mx[r] > (m[r] == -INFINITY ? -INFINITY : kLift + kSlack);
-      }
-    if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-        for (int r = 0; r < kPer; ++r) {
-          float y = mx[r];
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 1));
-          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 2));
-          y += (m[r] == -INFINITY ? 0.f : m[r]) - kLift;
-          // whole numbers, so that neither the factors nor the differences to them round
-          const float to = fmaxf(m[r], ceilf(y));
-          const float c = to > m[r] ? ex2(m[r] - to) : 1.f;
-          m[r] = to;
-          l[r] *= c;
-#pragma unroll
-          for (int n = 0; n < HD / 8; ++n) {
-            o[n][2 * r] *= c;
-            o[n][2 * r + 1] *= c;
-            if constexpr (FOLD) {
-              o[n][2] *= c;
-              o[n][3] *= c;
+            if (seen(r, n, i)) {
+              const float y = s[n][2 * r + i] * factor(r, n, i);
+              top = fmaxf(top, y);
+              if constexpr (F != kKvF16) product = fmaxf(product, y + log2_scale(vf[n][i]));
             }
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          if constexpr (F != kKvF16) product = fmaxf(product, __shfl_xor_sync(0xffffffffu, product, d));
+        }
+        const float to = next_reference(m[r], top, F == kKvF16 ? top : product);
+        const float c = to > m[r] ? ex2(m[r] - to) : 1.f;
+        m[r] = to;
+        l[r] *= c;
+#pragma unroll
+        for (int n = 0; n < HD / 8; ++n) {
+          o[n][2 * r] *= c;
+          o[n][2 * r + 1] *= c;
+          if constexpr (FOLD) {
+            o[n][2] *= c;
+            o[n][3] *= c;
           }
         }
-      exponents();
+        exponents(r);
+      }
     }
-    float low = 0.f;  // the smallest exponent
-#pragma unroll
-      for (int r = 0; r < kPer; ++r)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (kFar && seen(r, n, i)) low = fminf(low, x[r][n][i]);
-    const bool far = kFar && __any_sync(0xffffffffu, low < kNear);
+    // a seen position's weight times its V scale
+    auto weight = [&](int r, int n, int i, float& e) {
+      e = ex2(x[r][n][i]);
+      if constexpr (F == kKvF16) return e;
+      else return e * vf[n][i];
+    };
+    float low = 1.f;  // the smallest
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
       uint32_t p[4];
-      weigh(x, vf, n, seen, [&](int r, float y, float e) {
+      operand(n, [&](int r, int n, int i) {
+        if (!seen(r, n, i)) return 0.f;
+        float e;
+        const float w = weight(r, n, i, e);
         l[r] += e;
-        return far && y < kNear ? 0.f : e;
+        if (kFar) low = fminf(low, w);
+        return kFar && w < kNear ? 0.f : w;
       }, p);
       products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) { mma16816(o[c], p, b0, b1); });
     }
     if constexpr (kFar) {
-      if (far) {
+      if (__any_sync(0xffffffffu, low < kNear)) {
 #pragma unroll 1
-        for (float top = kNear, up = 38.f; top > -130.f; top -= 20.f, up += 20.f) {
-          const float down = ex2(-up);
+        for (float top = kNear, up = 0x1p38f, down = 0x1p-38f; top > 0x1p-110f; top *= 0x1p-20f, up *= 0x1p20f, down *= 0x1p-20f) {
 #pragma unroll
           for (int n = 0; n < NT; n += 2) {
             uint32_t p[4];
-            weigh(x, vf, n, seen, [&](int, float y, float) { return y >= top - 20.f && y < top ? ex2(y + up) : 0.f; }, p);
+            operand(n, [&](int r, int n, int i) {
+              float e;
+              const float w = weight(r, n, i, e);
+              return seen(r, n, i) && w >= top * 0x1p-20f && w < top ? w * up : 0.f;
+            }, p);
             if (__any_sync(0xffffffffu, (p[0] | p[2]) != 0))
               products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) {
-                float x[4] = {};
-                mma16816(x, p, b0, b1);
+                float y[4] = {};
+                mma16816(y, p, b0, b1);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[c][i] = fmaf(x[i], down, o[c][i]);
+                for (int i = 0; i < 4; ++i) o[c][i] = fmaf(y[i], down, o[c][i]);
               });
           }
         }
@@ -217,50 +209,24 @@ struct Rows {
     }
   }
 
-  // A V scale of vtop or more: the next power of two above the largest, and the sums so far brought to it.
-  static __device__ __noinline__ float next_vtop(float vtop, float most) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const uint32_t e = min((__float_as_uint(most) & 0x7f800000u) + (1u << 23), 252u << 23);
-    return fmaxf(vtop, __uint_as_float(e));
-  }
-  __device__ __forceinline__ void raise_v(float most) {
-    const float to = next_vtop(vtop, most), c = vtop / to;
+  // Weights of 16 keys as an operand: weight(r, n, i).
+  template <typename W>
+  __device__ __forceinline__ void operand(int n, W&& weight, uint32_t (&p)[4]) {
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] *= c;
-    vtop = to;
-  }
-
-  // Weights of 16 keys as an operand; take(r, exponent, 2^exponent) gives a seen position's weight before V's scale.
-  template <int NT, typename S, typename W>
-  __device__ __forceinline__ void weigh(const float (&x)[kPer][NT][2], const float (&vf)[NT][2], int n, S&& seen,
-                                        W&& take, uint32_t (&p)[4]) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int r = 0; r < kPer; ++r) {
-          float w[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float y = x[r][n + h][i];
-            w[i] = 0.f;
-            if (seen(r, n + h, i)) {
-              w[i] = take(r, y, ex2(y));
-              if constexpr (F != kKvF16) w[i] *= vf[n + h][i];
-            }
-          }
-          const __half2 lead = __floats2half2_rn(w[0], w[1]);
-          p[2 * h + r] = half2_bits(lead);
-          if constexpr (FOLD) {
-            const float2 z = __half22float2(lead);
-            p[2 * h + 1] = half2_bits(__floats2half2_rn(w[0] - z.x, w[1] - z.y));
-          }
+      for (int r = 0; r < kPer; ++r) {
+        const float x = weight(r, n + h, 0), y = weight(r, n + h, 1);
+        const __half2 lead = __floats2half2_rn(x, y);
+        p[2 * h + r] = half2_bits(lead);
+        if constexpr (FOLD) {
+          const float2 z = __half22float2(lead);
+          p[2 * h + 1] = half2_bits(__floats2half2_rn(x - z.x, y - z.y));
         }
+      }
   }
 
-  // The V operands of 16 keys: use(c, b0, b1) for every output tile c and row tile t.
+  // The V operands of 16 keys: use(c, b0, b1) for every output tile c.
   template <typename U>
   __device__ __forceinline__ void products(uint32_t v_base, int key, U&& use) {
     const int lane = threadIdx.x & 31, mi = lane >> 3, r8 = lane & 7;
@@ -269,41 +235,33 @@ struct Rows {
       uint32_t w[4];
       ldsm4t(w, piece<F, HD, KEYS>(v_base, key + 8 * (mi & 1) + r8, c + (mi >> 1)));
       if constexpr (F == kKvF16) {
-        {
-          use(c, w[0], w[1]);
-          use(c + 1, w[2], w[3]);
-        }
+        use(c, w[0], w[1]);
+        use(c + 1, w[2], w[3]);
       } else {  // a piece holds 16 dimensions: its even ones are tile 2 c, its odd ones tile 2 c + 1
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t e0, e1, d0, d1;
           unpack<F, true>(w[2 * j], e0, d0);
           unpack<F, true>(w[2 * j + 1], e1, d1);
-          {
-            use(2 * (c + j), e0, e1);
-            use(2 * (c + j) + 1, d0, d1);
-          }
+          use(2 * (c + j), e0, e1);
+          use(2 * (c + j) + 1, d0, d1);
         }
       }
     }
   }
 
-  // The row sums with V's power of two put back; l summed over the lanes of a row.
+  // l summed over the lanes of a row; leading parts and rests together.
   __device__ __forceinline__ void finish() {
-    const float up = F == kKvF16 ? 1.f : 0.5f * vtop;
 #pragma unroll
-      for (int r = 0; r < kPer; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    for (int r = 0; r < kPer; ++r) {
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
 #pragma unroll
-        for (int n = 0; n < HD / 8; ++n)
+      for (int n = 0; n < HD / 8; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& x = o[n][2 * r + i];
-            if constexpr (FOLD) x = join(x, o[n][2 + i]);
-            x *= up;
-          }
-      }
+        for (int i = 0; i < 2; ++i)
+          if constexpr (FOLD) o[n][i] = join(o[n][i], o[n][2 + i]);
+    }
   }
 
   // Row r to dst[HD].
@@ -553,8 +511,8 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = qa[step][i];
       };
-      if (key + KEYS > x.fewest) st.template step<KEYS / 8, true>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, left, key, frag);
-      else st.template step<KEYS / 8, false>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, left, key, frag);
+      if (key + KEYS > x.fewest) st.template step<KEYS / 8, true>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, key, frag);
+      else st.template step<KEYS / 8, false>(k_base, k_base + Tl::kBytes, ks, ks + KEYS, 0, key, frag);
       __syncwarp();
       ++done;
     }

@@ -46,8 +46,9 @@ struct WideShared {
   int abort;
   alignas(16) float raw_scale[kRawStages][2][kTile];
   alignas(16) float kf[kOps][kTile];   // K scale * softmax scale * log2(e)
-  alignas(16) float vf[kOps][kTile];   // V scale * 2 / vtop: below 2
-  float vtop[kOps];
+  alignas(16) float vf[kOps][kTile];   // V scale
+  alignas(16) float vlog[kOps][kTile]; // its log2_scale
+  float vmost[kOps];                   // the largest of a tile, at least kLeastScale
   alignas(4) uint8_t hidden[kOps][4];  // by the converting warps: V values that not all rows see were left out
   SeqTables seqs;
 };
@@ -119,7 +120,6 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
   Piece x;
   int count = 0;
   while (w.next(x, p, a, seqs)) {
-    float vtop = 0x1p-100f;
     for (int i = 0, n = tiles_of(x); i < n; ++i, ++count) {
       const int s = count % Wd::kRawStages, o = count % Wd::kOps, left = x.limit - (x.t0 + i) * kTile;
       umma::bounded_wait(&sh.raw_full[s], (count / Wd::kRawStages) & 1, &sh.abort, a.err, kErrKvCopy);
@@ -189,25 +189,18 @@ __device__ void wide_convert(const PrefixAttnArgs& a, const Plan& p, const Seqs&
       }
       if constexpr (F != kKvF16) {
         if (cw == 0) {  // the tile's column factors
-          float kx[2], vx[2], most = 0.f;
+          float most = kLeastScale;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            kx[j] = sh.raw_scale[s][0][32 * j + lane];
-            vx[j] = 32 * j + lane < left ? sh.raw_scale[s][1][32 * j + lane] : 0.f;
-            most = fmaxf(most, vx[j]);  // (a NaN shows in its products, not here)
+            const int k = 32 * j + lane;
+            const float vx = k < left ? sh.raw_scale[s][1][k] : 0.f;  // nothing is stored past the last position
+            sh.kf[o][k] = sh.raw_scale[s][0][k] * base;
+            sh.vf[o][k] = vx;
+            sh.vlog[o][k] = log2_scale(vx);
+            most = fmaxf(most, fabsf(vx));  // (a NaN shows in its products, not here)
           }
-          if (__any_sync(0xffffffffu, most >= vtop)) {
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            vtop = fmaxf(vtop, __uint_as_float(min((__float_as_uint(most) & 0x7f800000u) + (1u << 23), 252u << 23)));
-          }
-          const float inv = __uint_as_float(0x7f800000u - __float_as_uint(vtop));  // 2 / vtop
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            sh.kf[o][32 * j + lane] = kx[j] * base;
-            sh.vf[o][32 * j + lane] = vx[j] * inv;
-          }
-          if (lane == 0) sh.vtop[o] = vtop;
+          const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+          if (lane == 0) sh.vmost[o] = __uint_as_float(top);
         }
       }
       if constexpr (F != kKvI8) hidden = __any_sync(0xffffffffu, hidden);
@@ -348,9 +341,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 constexpr int kHalf = kTile / 2;  // keys of a half
 
-// The largest sum of a half's weights for which every weight, with a V scale below 2, is an f16.  (At or below the
-// reference weights are at most 2^8 and their sum 2^13.)
-constexpr float kMostSum = 23000.f;
+// The largest sum of a half's weights, times the tile's largest V scale, for which every product is surely an f16.  (At or
+// below the reference products are at most 2^8.)
+constexpr float kMostSum = 46000.f;
 
 // Operand position -> dimension: K's words hold four consecutive dimensions of a byte row, which lie in two chunks of an
 // operand row.  Even positions keep their neighbour.
@@ -463,7 +456,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
     const int n = tiles_of(x), step = p.split_keys ? 2 : 1, first = p.split_keys ? r : 0;
     int lim;
     const Q* src = q_row<Q>(a, p, x, p.split_keys ? row : 128 * r + row, lim);
-    float m = -INFINITY, l = 0.f, row_f = 1.f, vtop = 0x1p-100f;
+    float m = -INFINITY, l = 0.f, row_f = 1.f;
     uint32_t hidden = 0;
     const int64_t at_row = x.slot * 256 + 128 * r + row;
     float* part = p.part + at_row * HD;
@@ -474,21 +467,18 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
     auto drain = [&]() {
       umma::bounded_wait(&sh.o_done[r][1], (mine - 1) & 1, &sh.abort, a.err, kErrKvCopy);
       umma::tc_fence_after();
-      const float up = F == kKvF16 ? 1.f : 0.5f * vtop, old = drained_m == m ? 1.f : ex2(drained_m - m);
+      const float old = drained_m == m ? 1.f : ex2(drained_m - m);
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t u[32];
         tmem_ld32(to + 32 * c, u);
         umma::tmem_ld_wait();
-        float y[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(u[j]) * up;
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
           // 8-bit pieces: even dimensions of 16 lie before the odd ones
           float z[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) z[i] = F == kKvF16 ? y[j + i] : y[(j & 16) + ((j & 15) >> 1) + (i >> 1) + 8 * (i & 1)];
+          for (int i = 0; i < 8; ++i) z[i] = __uint_as_float(u[F == kKvF16 ? j + i : (j & 16) + ((j & 15) >> 1) + (i >> 1) + 8 * (i & 1)]);
           if (SPLIT_Q && drained) {
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
@@ -581,30 +571,29 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
           }
           return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         };
-        float sum = 0.f, vtop_now = vtop;
-        if constexpr (F != kKvF16) vtop_now = sh.vtop[o];
-        bool slow = __any_sync(0xffffffffu, masked || m == -INFINITY || vtop_now != vtop);
+        float sum = 0.f, vmost = 1.f;
+        if constexpr (F != kKvF16) vmost = sh.vmost[o];
+        bool slow = __any_sync(0xffffffffu, masked || m == -INFINITY);
         if (!slow) {
           sum = weights(std::false_type{});
-          slow = __any_sync(0xffffffffu, !(sum <= kMostSum));
+          slow = __any_sync(0xffffffffu, !(sum * vmost <= kMostSum));
           if (slow) load();  // S is still in tensor memory
         }
         if (slow) {
           if constexpr (F != kKvI8) hidden |= *reinterpret_cast<const uint32_t*>(sh.hidden[o]);
-          float top = -INFINITY;
+          float top = -INFINITY, product = -INFINITY, shrink_o = 1.f;
 #pragma unroll
           for (int j = 0; j < kHalf; ++j) {
-            float f = base;
-            if constexpr (F != kKvF16) f = kf[j];
-            if (j < seen) top = fmaxf(top, s[j] * (f * row_f));
+            if (j >= seen) continue;
+            const float y = s[j] * ((F == kKvF16 ? base : kf[j]) * row_f);
+            top = fmaxf(top, y);
+            if constexpr (F != kKvF16) product = fmaxf(product, y + sh.vlog[o][kHalf * h + j]);
           }
-          float shrink_o = vtop / vtop_now;
-          vtop = vtop_now;
-          if (top > m + (m == -INFINITY ? 0.f : kSlack)) {  // whole numbers: neither factors nor differences round
-            const float t = ceilf(top), c = ex2(m - t);
-            l *= c;
-            shrink_o *= c;
-            m = t;
+          const float next = next_reference(m, top, F == kKvF16 ? top : product);
+          if (next > m + (m == -INFINITY ? 0.f : kSlack)) {
+            shrink_o = ex2(m - next);
+            l *= shrink_o;
+            m = next;
           }
           if ((h || summed) && __any_sync(0xffffffffu, shrink_o != 1.f)) {
             // the products made so far, up to those of the half before, rest

@@ -10,7 +10,7 @@
 // Work.  An item is a tile of query rows that read the same keys: (kv head, rows of the whole batch) over the
 // prefix, (sequence, kv head, rows) over own positions.  Its keys come in units, a few more of them in front of each
 // item for what a piece costs besides; the units of all items, laid end to end, are dealt out evenly to the workers (CTAs
-// or warps), so a share starts and ends inside items.  Every piece of an item leaves its unnormalised sums, row maxima and
+// or warps), so a share starts and ends inside items.  Every piece of an item leaves its unnormalised sums, references and
 // denominators in the workspace (slot = item + worker, unique because each next piece raises one of the two), and a last
 // kernel joins the pieces of each row in a fixed order.
 //
