@@ -180,3 +180,32 @@ def test_v_of_any_size(um, backend, fmt, half, g, t, size):
     if half and size > 1:
         size = 1e4
     check(um, backend, queries(b, t, g * h, d, half, rng), Rows(um, fmt, k, (v * size).astype(np.float32)), [n, n - 7])
+
+
+# ---------------------------------------------------------------- keys that weigh nothing
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("g,t", [(4, 1), (3, 4), (7, 4)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lead", [1e-9, -3e-8, 1e-12, 0.7])
+def test_infinite_keys_against_small_query_values(um, backend, half, g, t, d, lead):
+    """Keys masked by an infinity in one dimension, where the queries hold a value that may be far below the row's largest:
+    the masked positions lose their weight and nothing else changes."""
+    rng = np.random.default_rng(g + d)
+    b, h, n = 2, 2, 130
+    k, v = random_rows(rng, b, h, n, d)
+    hidden = rng.random(n) < 0.4
+    hidden[-t:] = False  # (every token sees the same finite keys but its own last ones)
+    if half:
+        lead = np.copysign(max(abs(lead), 6e-8), lead)  # f16's smallest
+    k[:, :, hidden, 0] = np.copysign(np.inf, -lead)
+    q = queries(b, t, g * h, d, half, rng, lead=lead)
+    own, left = Rows(um, "f16", k, v), Rows(um, "f16", k[:, :, ~hidden], v[:, :, ~hidden])
+    out = torch.full_like(q, 9.0)
+    backend.prefix_attention(q, own.view, dev(np.array([n] * b, np.int32)), out)
+    backend.synchronize()
+    want, tol, mag = definition(q, left, [int((~hidden).sum())] * b)
+    if half:
+        tol = tol + 2.0 ** -11 * (mag + want.abs()) + 2.0 ** -25
+    assert ((out.double() - want).abs() <= tol).all()

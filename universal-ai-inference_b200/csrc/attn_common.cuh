@@ -122,6 +122,11 @@ __device__ __forceinline__ float next_reference(float m, float top, float produc
 }
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
+// h, but the smallest half of s's sign rather than 0 unless s is 0.
+__device__ __forceinline__ __half but_zero(__half h, float s) {
+  return __hisnan(h) || (__half_as_ushort(h) & 0x7fff) || s == 0.f ? h : __ushort_as_half(s < 0.f ? 0x8001 : 1);
+}
+
 // Two pairs of stored bytes -> two f16 pairs.  i8: a byte u behind 0x64 is the half 1024 + u, less 1152 = u - 128.
 // SEL: bytes (0, 1) and (2, 3) for K, whose pairs run along a row; (0, 2) and (1, 3) for V, whose transposed words
 // hold two dimensions of two positions.

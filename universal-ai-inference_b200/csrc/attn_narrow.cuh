@@ -481,7 +481,10 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
       for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const __half2 lead = __floats2half2_rn(v[ks][2 * h], v[ks][2 * h + 1]);
+          __half2 lead = __floats2half2_rn(v[ks][2 * h], v[ks][2 * h + 1]);
+          // K may hold infinities, whose products with a leading part of 0 would be NaN (and with the rest are not looked at)
+          if constexpr (FOLD && sizeof(Q) == 4 && F == kKvF16)
+            lead = __halves2half2(but_zero(__low2half(lead), v[ks][2 * h]), but_zero(__high2half(lead), v[ks][2 * h + 1]));
           qa[ks][2 * h + r] = half2_bits(lead);
           if constexpr (FOLD) {
             const float2 z = __half22float2(lead);

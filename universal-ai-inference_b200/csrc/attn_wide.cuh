@@ -353,11 +353,6 @@ __device__ __forceinline__ int operand_dim(int pos) {
   return (pos & ~15) | ((pos & 6) << 1) | ((pos & 8) >> 2) | (pos & 1);
 }
 
-// h, but the smallest half of s's sign rather than 0 unless s is 0.
-__device__ __forceinline__ __half but_zero(__half h, float s) {
-  return __hisnan(h) || (__half_as_ushort(h) & 0x7fff) || s == 0.f ? h : __ushort_as_half(s < 0.f ? 0x8001 : 1);
-}
-
 // This thread's row of q (null: zeros) into tensor memory as operand `part` (1: the rests of a split); returns the power
 // of two by which a split row was multiplied.
 template <int F, int HD, bool SPLIT_Q, typename Q>
@@ -419,7 +414,10 @@ __device__ __forceinline__ float put_q(const Q* src, bool vec, int part, uint32_
           e = __halves2half2(but_zero(__float2half_rz(y0), y0), but_zero(__float2half_rz(y1), y1));
           if (part) {
             const float2 z = __half22float2(e);
-            e = __halves2half2(but_zero(__float2half_rn(y0 - z.x), y0), but_zero(__float2half_rn(y1 - z.y), y1));
+            auto rest = [](float y, float z) {  // (a leading part that is larger than its value was made of 0)
+              return but_zero(__float2half_rn(fabsf(z) > fabsf(y) ? 0.f : y - z), y);
+            };
+            e = __halves2half2(rest(y0, z.x), rest(y1, z.y));
           }
         } else if (part) {
           const float2 z = __half22float2(e);
