@@ -30,24 +30,48 @@ class Rows:
             c, s = (x.astype(np.float16), None) if fmt == "f16" else encode(x, fmt)
             self.val[n] = dev(values(c, s, fmt))
             t[n], t[n + "s"] = dev(c), None if s is None else dev(s)
-        self.t = t
         self.view = um.kv_cache(code(um, fmt), t["k"], t["v"], t["ks"], t["vs"])
+
+    def rows(self, n, i, kh, end):
+        return self.val[n][i, kh, :end]
+
+
+class DeviceRows:
+    """The same of rows made on the device, where they may be many."""
+
+    def __init__(self, um, fmt, k, v):
+        self.fmt, self.t = fmt, {}
+        for n, x in (("k", k), ("v", v)):
+            if fmt == "f16":
+                self.t[n] = x.half(), None
+                continue
+            scale = x.abs().amax(-1) / (127 if fmt == "i8" else 448)
+            y = x / scale[..., None]
+            self.t[n] = ((y.round() + 128).to(torch.uint8) if fmt == "i8" else y.to(torch.float8_e4m3fn).view(torch.uint8)), scale
+        self.view = um.kv_cache(code(um, fmt), *(self.t[n][j] for j in (0, 1) for n in "kv"))
+
+    def rows(self, n, i, kh, end):
+        c, s = self.t[n]
+        c = c[i, kh, :end]
+        if self.fmt == "f16":
+            return c.double()
+        c = c.double() - 128 if self.fmt == "i8" else c.view(torch.float8_e4m3fn).double()
+        return c * s[i, kh, :end, None].double()
 
 
 def definition(q, own, lens, prefix=None, p_len=0, scale=None):
     """(result, tolerance for f32 results, sum p |v|), all in 64 bits on the device; q [B, T, H, d]."""
     b, t, hq, d = q.shape
-    h = own.val["k"].shape[1]
+    h = own.view.n_kv_heads
     g = hq // h
     scale = scale or d ** -0.5
     q = q.double().view(b, t, h, g, d)
     out, tol, mag = (torch.zeros_like(q) for _ in range(3))
     for i in range(b):
         for kh in range(h):
-            k, v = own.val["k"][i, kh, :lens[i]], own.val["v"][i, kh, :lens[i]]
+            k, v = own.rows("k", i, kh, lens[i]), own.rows("v", i, kh, lens[i])
             if p_len:
-                k = torch.cat([prefix.val["k"][0, kh, :p_len], k])
-                v = torch.cat([prefix.val["v"][0, kh, :p_len], v])
+                k, v = torch.cat([prefix.rows("k", 0, kh, p_len), k]), torch.cat([prefix.rows("v", 0, kh, p_len), v])
             n = len(k)
             if n == 0:
                 continue
@@ -209,3 +233,77 @@ def test_infinite_keys_against_small_query_values(um, backend, half, g, t, d, le
     if half:
         tol = tol + 2.0 ** -11 * (mag + want.abs()) + 2.0 ** -25
     assert ((out.double() - want).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------- long walks
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("half,g,t", [(False, 4, 1), (True, 4, 1), (True, 4, 4)])
+def test_many_steps_of_one_warp(um, backend, fmt, d, half, g, t):
+    """Thousands of positions of many sequences, so that a warp walks some thirty to seventy steps of one item: copies reuse
+    their places, references rise while sums are not zero, small weights follow large ones.  By turns, sequences are plain,
+    their scores rise by 60 nats along the positions, their V grows 2^12-fold, and both at once with V falling."""
+    gen = torch.Generator(device="cuda").manual_seed(d + g + t)
+    b, h, n = 64, 8, 3900
+    k, v = (torch.randn((b, h, n, d), generator=gen, device="cuda") for _ in range(2))
+    along, kind = torch.linspace(0, 1, n, device="cuda"), torch.arange(b, device="cuda") % 4
+    k[..., 0] = 60 * d ** 0.5 / 4.0 * along * (kind % 2 == 1)[:, None, None]
+    turn = torch.where(kind == 2, 1.0, torch.where(kind == 3, -1.0, 0.0))[:, None, None]
+    v *= torch.exp2(12 * turn * (along - 0.5))[..., None]
+    own = DeviceRows(um, fmt, k, v)
+    del k, v
+    q = torch.randn((b, t, g * h, d), generator=gen, device="cuda")
+    q[..., 0] = 4.0
+    check(um, backend, q.half() if half else q, own, [n - 61 * (i % 7) for i in range(b)])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("half", [False, True])
+def test_many_tiles_of_one_block(um, backend, fmt, half):
+    """Items of 160 rows over a prefix of thousands of positions: a block walks some tens of tiles of one item, with scores
+    that rise and V that grows, then falls."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    b, h, g, d, n = 40, 8, 4, 128, 31000
+    k, v = (torch.randn((1, h, n, d), generator=gen, device="cuda") for _ in range(2))
+    along = torch.linspace(0, 1, n, device="cuda")
+    k[..., 0] = 40 * d ** 0.5 / 4.0 * along * (torch.arange(h, device="cuda") % 2)[:, None]
+    v *= torch.exp2(12 * (1 - (2 * along - 1).abs()))[:, None]
+    prefix = DeviceRows(um, fmt, k, v)
+    own = DeviceRows(um, fmt, *(torch.randn((b, h, 30, d), generator=gen, device="cuda") for _ in range(2)))
+    q = torch.randn((b, 1, g * h, d), generator=gen, device="cuda")
+    q[..., 0] = 4.0
+    check(um, backend, q.half() if half else q, own, [i % 31 for i in range(b)], prefix, n)
+
+
+@pytest.mark.parametrize("fmt,d", [("i8", 64), ("e4m3", 128), ("f16", 64), ("f16", 128)])
+def test_long_f32_sums_of_few_rows_do_not_shrink(um, backend, fmt, d):
+    """Few rows over tens of thousands of positions, hundreds of steps of one warp: an accumulator that is cut off at each
+    addition loses 2^-24 of itself on average, so 32 additions to a sum that grows from nothing lose 32 / 2 * 2^-24 of it,
+    1e-6; scores (8 additions) and the roundings of the rows as much again.  Bar on the whole result: 2.5e-6."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    b, h, g, n = 96, 4 if fmt == "f16" else 8, 2, 24000
+    k = torch.empty((b, h, n, d), dtype=torch.float16 if fmt == "f16" else torch.uint8, device="cuda")
+    own = DeviceRows.__new__(DeviceRows)
+    own.fmt, own.t = fmt, {}
+    for name in "kv":
+        if fmt == "f16":
+            own.t[name] = torch.randn(k.shape, generator=gen, dtype=torch.float16, device="cuda"), None
+        else:  # any bytes are rows; e4m3's two NaNs are not
+            c = torch.randint(1, 126, k.shape, generator=gen, dtype=torch.uint8, device="cuda")
+            c += 128 * torch.randint(0, 2, k.shape, generator=gen, dtype=torch.uint8, device="cuda")
+            own.t[name] = c, (0.015 if fmt == "i8" else 0.01) * (0.5 + torch.rand((b, h, n), generator=gen, device="cuda"))
+    own.view = um.kv_cache(code(um, fmt), *(own.t[x][j] for j in (0, 1) for x in "kv"))
+    q = torch.randn((b, 1, g * h, d), generator=gen, device="cuda")
+    out = torch.empty_like(q)
+    backend.prefix_attention(q, own.view, dev(np.full(b, n, np.int32)), out)
+    backend.synchronize()
+    off = whole = 0.0
+    for i in range(b):
+        for kh in range(h):
+            x = q[i, 0, kh * g:(kh + 1) * g].double()
+            want = torch.softmax(x @ own.rows("k", i, kh, n).T / d ** 0.5, -1) @ own.rows("v", i, kh, n)
+            off += float((out[i, 0, kh * g:(kh + 1) * g].double() - want).square().sum())
+            whole += float(want.square().sum())
+    assert (off / whole) ** 0.5 <= 2.5e-6, (off / whole) ** 0.5

@@ -23,7 +23,7 @@ struct Narrow {
 
 // ---------------------------------------------------------------- one warp's running softmax
 
-template <int F, int HD, bool FOLD, int KEYS>
+template <int F, int HD, bool FOLD, int KEYS, bool F32>
 struct Rows {
   static constexpr int kPer = FOLD ? 1 : 2;  // logical rows of a lane in one MMA tile
   static constexpr int kPieces = HD * Tile<F, HD, KEYS>::kEsz / 16;  // 16-byte pieces of a row
@@ -35,6 +35,11 @@ struct Rows {
   float m[kPer], l[kPer];  // the reference (attn_common.cuh), the denominator
   float f[kPer];           // score factor: scale * log2(e), and the power of two taken out of a folded row of q
   int lim[kPer];           // positions the row sees
+  // The tensor cores cut sums off where they should round (half of f32's last place at each addition, 1e-5 of a sum after
+  // the 1500 of a warp's 750 steps), so f32 sums are taken out after 32 additions and added up in f32.
+  static constexpr bool kTake = FOLD && F32;
+  static constexpr int kTakeSteps = 32 / (KEYS / 16);
+  float taken_m;           // their reference
 
   // Leading part and rest.  Where an f16 cache holds an infinity, the rest is 0 * inf.
   static __device__ __forceinline__ float join(float lead, float rest) {
@@ -250,33 +255,48 @@ struct Rows {
     }
   }
 
-  // l summed over the lanes of a row; leading parts and rests together.
-  __device__ __forceinline__ void finish() {
-#pragma unroll
-    for (int r = 0; r < kPer; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-#pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if constexpr (FOLD) o[n][i] = join(o[n][i], o[n][2 + i]);
-    }
-  }
-
-  // Row r to dst[HD].
-  __device__ __forceinline__ void store(float* dst, int r) const {
+  // Row r's sums to dst[HD], added to those taken out before (`more`); the next ones start from nothing.
+  __device__ __forceinline__ void take_out(float* dst, int r, bool more) {
     const int tq = threadIdx.x & 3;
+    const float old = taken_m == m[r] ? 1.f : ex2(taken_m - m[r]);
+    auto out = [&](int n, int i) {
+      float y = o[n][2 * r + i];
+      if constexpr (FOLD) y = join(y, o[n][2 + i]);
+      o[n][2 * r + i] = 0.f;
+      if constexpr (FOLD) o[n][2 + i] = 0.f;
+      return y;
+    };
     if constexpr (F == kKvF16) {
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n)
-        *reinterpret_cast<float2*>(dst + 8 * n + 2 * tq) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+      for (int n = 0; n < HD / 8; ++n) {
+        float2* at = reinterpret_cast<float2*>(dst + 8 * n + 2 * tq);
+        float2 y = make_float2(out(n, 0), out(n, 1));
+        if (kTake && more) {
+          const float2 z = *at;
+          y = make_float2(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y));
+        }
+        *at = y;
+      }
     } else {
 #pragma unroll
-      for (int n = 0; n < HD / 8; n += 2)
-        *reinterpret_cast<float4*>(dst + 8 * n + 4 * tq) =
-            make_float4(o[n][2 * r], o[n + 1][2 * r], o[n][2 * r + 1], o[n + 1][2 * r + 1]);
+      for (int n = 0; n < HD / 8; n += 2) {
+        float4* at = reinterpret_cast<float4*>(dst + 8 * n + 4 * tq);
+        float4 y = make_float4(out(n, 0), out(n + 1, 0), out(n, 1), out(n + 1, 1));
+        if (kTake && more) {
+          const float4 z = *at;
+          y = make_float4(fmaf(z.x, old, y.x), fmaf(z.y, old, y.y), fmaf(z.z, old, y.z), fmaf(z.w, old, y.w));
+        }
+        *at = y;
+      }
     }
+    taken_m = m[r];
+  }
+
+  // Row r's denominator, summed over its lanes.
+  __device__ __forceinline__ float denominator(int r) const {
+    float y = l[r];
+    y += __shfl_xor_sync(0xffffffffu, y, 1);
+    return y + __shfl_xor_sync(0xffffffffu, y, 2);
   }
 };
 
@@ -439,7 +459,7 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
   };
   for (int i = 0; i < N::kStages - 1; ++i) copy();
 
-  Rows<F, HD, FOLD, KEYS> st;
+  Rows<F, HD, FOLD, KEYS, sizeof(Q) == 4> st;
   const float base = a.scale * kLog2e;
   Piece x;
   while (w.next(x, p, a, cum)) {
@@ -494,9 +514,16 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
     }
     st.clear();
     const int end = min(x.t1 * KEYS, x.limit);
-    bool hidden = false;
+    float* part = p.part + x.slot * (RT * HD);
+    bool hidden = false, taken = false;
+    int steps = 0;
 #pragma unroll 1
     for (int key = x.t0 * KEYS; key < end; key += KEYS) {
+      if (st.kTake && steps++ == st.kTakeSteps) {
+        st.take_out(part + g * HD, 0, taken);
+        taken = true;
+        steps = 1;
+      }
       copy();
       const int s = done % N::kStages;
       umma::bounded_wait(&sh.full[warp][s], (done / N::kStages) & 1, &sh.abort, a.err, kErrKvCopy);
@@ -519,12 +546,11 @@ __global__ void __launch_bounds__(32 * kWarps, kNarrowCtas)
       __syncwarp();
       ++done;
     }
-    st.finish();
-    float* part = p.part + x.slot * (RT * HD);
 #pragma unroll
     for (int r = 0; r < kPer; ++r) {
-      st.store(part + (g + 8 * r) * HD, r);
-      if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], hidden ? -st.l[r] : st.l[r]);
+      st.take_out(part + (g + 8 * r) * HD, r, taken);
+      const float l = st.denominator(r);
+      if (tq == 0) *reinterpret_cast<float2*>(p.ml + 2 * (x.slot * RT + g + 8 * r)) = make_float2(st.m[r], hidden ? -l : l);
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // no grid of this call ends before the one it followed
