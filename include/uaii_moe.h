@@ -561,7 +561,8 @@ UAII_MOE_API int uaii_moe_decoder_create_serving(uaii_moe_backend* b, const uaii
                                                  const float* output_norm, const void* token_embd, int embd_fmt,
                                                  const void* output, int output_fmt, uaii_moe_decoder** out);
 /* The shared prefix of layer `layer`: f32 k, v [n_kv_heads, n_pos, head_dim] (host or device), rotated to positions
- * 0 .. n_pos - 1 already.  The sequences' own positions follow it; give every layer the same n_pos. */
+ * 0 .. n_pos - 1 already.  The sequences' own positions follow it; a step is refused (UAII_MOE_INVALID_ARGUMENT) while
+ * the layers' n_pos differ. */
 UAII_MOE_API int uaii_moe_decoder_set_prefix(uaii_moe_decoder* d, int64_t layer, const float* k, const float* v,
                                              int64_t n_pos);
 /* One step whose next tokens are drawn by uaii_moe_sample from the step's logits: temperature, top_k, top_p, min_p, u,

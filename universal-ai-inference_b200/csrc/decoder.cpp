@@ -140,6 +140,7 @@ class Decoder {
     if (serve_fmt_) {
       own_.assign((size_t)L, KvCache{});
       prefix_.assign((size_t)L, KvCache{});
+      prefix_lens_.assign((size_t)L, 0);
       for (int64_t l = 0; l < L; ++l) {
         UAII_TRY(make_cache(&own_[(size_t)l], B, c.max_seq));
         if (prefix_max_) UAII_TRY(make_cache(&prefix_[(size_t)l], 1, prefix_max_));
@@ -247,7 +248,7 @@ class Decoder {
       return Error::make(ErrorCode::InvalidArgument, "decoder set_prefix: layer or position count out of range");
     UAII_CUDA(cudaSetDevice(be_->device()), "SetDevice");
     UAII_TRY(put(prefix_[(size_t)layer], k, v, n));
-    prefix_len_ = n;
+    prefix_lens_[(size_t)layer] = n;
     return Error::success();
   }
 
@@ -268,6 +269,9 @@ class Decoder {
   Error step(const int32_t* tokens, float* logits, int32_t* next) {
     if (!tokens) return Error::make(ErrorCode::InvalidArgument, "decoder step: null tokens");
     if (pos_ >= cfg_.max_seq) return Error::make(ErrorCode::InvalidArgument, "decoder step: the cache is full");
+    for (int64_t n : prefix_lens_)
+      if (n != prefix_lens_[0])
+        return Error::make(ErrorCode::InvalidArgument, "decoder step: the layers hold prefixes of different lengths");
     UAII_CUDA(cudaSetDevice(be_->device()), "SetDevice");
     cudaStream_t st = be_->stream();
     const int64_t B = cfg_.batch, D = cfg_.d_model, H = cfg_.n_heads, Hkv = cfg_.n_kv_heads, hd = cfg_.head_dim;
@@ -376,14 +380,14 @@ class Decoder {
   Error serve_attention(int64_t l) {
     const int64_t B = cfg_.batch, H = cfg_.n_heads, Hkv = cfg_.n_kv_heads, hd = cfg_.head_dim;
     const int64_t row = q_dim_ + 2 * kv_dim_;
-    UAII_CUDA(launch_rope_rows(qkv_, B, H, Hkv, hd, freq_, pos_, prefix_len_, cfg_.rope_mode, own_pos_, own_len_, be_->stream()),
+    UAII_CUDA(launch_rope_rows(qkv_, B, H, Hkv, hd, freq_, pos_, prefix_lens_[0], cfg_.rope_mode, own_pos_, own_len_, be_->stream()),
               "rope");
     const KvCache& c = own_[(size_t)l];
     UAII_TRY(be_->kv_append(c, qkv_ + q_dim_, qkv_ + q_dim_ + kv_dim_, false, 1, RowView{row, row, hd}, own_pos_, nullptr));
     PrefixAttnArgs a;
     a.own = c;
     a.prefix = prefix_[(size_t)l];
-    a.prefix_len = prefix_len_;
+    a.prefix_len = prefix_lens_[0];
     a.own_len = own_len_;
     a.q = qkv_;
     a.T = 1;
@@ -434,8 +438,9 @@ class Decoder {
   std::vector<KvMap> maps_;  // TMA maps of each layer's K and V caches
   float *x_ = nullptr, *n_ = nullptr, *o_ = nullptr, *ff_ = nullptr, *qkv_ = nullptr, *q_ = nullptr, *attn_ = nullptr;
   int serve_fmt_ = 0;  // a serving decoder's cache format
-  int64_t prefix_max_ = 0, prefix_len_ = 0;
+  int64_t prefix_max_ = 0;
   std::vector<KvCache> own_, prefix_;  // of each layer
+  std::vector<int64_t> prefix_lens_;   // positions set in each; the same in all when a step is taken
   int32_t *own_pos_ = nullptr, *own_len_ = nullptr;
   float *po_ = nullptr, *pm_ = nullptr, *pl_ = nullptr, *logits_ = nullptr;
   int32_t *tokens_ = nullptr, *next_ = nullptr;
