@@ -231,13 +231,14 @@ def _dtype_code(t) -> int:
 
 
 def _rows(t, *shape):
-    """Element strides (batch, token, head) of a [batch, token, head, head_dim] view with a dense last dimension."""
+    """Element strides (batch, token, head) of a [batch, token, head, head_dim] view with a dense last dimension; 0 for a
+    dimension of one, whose stride says nothing."""
     if t.shape != shape:
         raise ValueError(f"expected shape {shape}, got {tuple(t.shape)}")
     sb, st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError("the last dimension must be dense")
-    return sb, st, sh
+    return sb if shape[0] > 1 else 0, st if shape[1] > 1 else 0, sh if shape[2] > 1 else 0
 
 
 def _whole(t, what, *shape):
@@ -424,8 +425,9 @@ class Backend:
         """Write k, v [batch, tokens, n_kv_heads, head_dim] (f32 or f16, any strides with a dense last dimension, the
         same for both) at positions pos[i] + t, for t < n_new[i] (int32) where given."""
         b, t = k.shape[0], k.shape[1]
-        sb, st, sh = _rows(k, cache.batch, t, cache.n_kv_heads, cache.head_dim)
-        if v.shape != k.shape or v.stride() != k.stride() or v.dtype is not k.dtype:
+        shape = (cache.batch, t, cache.n_kv_heads, cache.head_dim)
+        rows = sb, st, sh = _rows(k, *shape)
+        if v.shape != k.shape or v.dtype is not k.dtype or (v.stride() != k.stride() and _rows(v, *shape) != rows):
             raise ValueError("k and v must have the same shape, strides and type")
         i32 = (_T or _torch()).int32
         _check(lib.uaii_moe_kv_append(self._h, byref(cache), k.data_ptr(), v.data_ptr(), _dtype_code(k), t, sb, st, sh,
