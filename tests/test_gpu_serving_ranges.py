@@ -7,9 +7,10 @@ and a split of q to 2^-22), a result may be off by
     sum_j p_j e_j |v_j|  +  (sum_j p_j e_j) sum_j p_j |v_j|          the scores' errors, in weights and denominator
   + ((n / 16 + 64) 2^-23 + 2^-20) sum_j p_j |v_j|                    sums over n positions; exponentials and scales
   + n 2^-32 max_j (p_j max_d |v_jd|)                                 weights that f16's smallest step cuts: at most 2^-25
-                                                                     each, where the largest product of a weight and a
-                                                                     row's scale is 2^7 or more
-f16 results add a rounding of p and of the result: 2^-11 (sum_j p_j |v_j| + |result|) + 2^-25.
+                                                                     in each of two parts, where the largest product of
+                                                                     a weight and a row's scale is 2^8 or more
+f16 results add a rounding of p and of the result: 2^-11 (sum_j p_j |v_j| + |result|) + 2^-25; where the test says so, of
+the result alone: 2^-11 |result| + 2^-25.
 """
 import numpy as np
 import pytest
@@ -88,14 +89,14 @@ def definition(q, own, lens, prefix=None, p_len=0, scale=None):
     return tuple(x.view(b, t, hq, d) for x in (out, tol, mag))
 
 
-def check(um, backend, q, own, lens, prefix=None, p_len=0, scale=0.0):
+def check(um, backend, q, own, lens, prefix=None, p_len=0, scale=0.0, weights=2.0 ** -11):
     out = torch.full_like(q, 9.0)
     backend.prefix_attention(q, own.view, dev(np.array(lens, np.int32)), out, prefix=prefix.view if prefix else None,
                              prefix_len=p_len, scale=scale)
     backend.synchronize()
     want, tol, mag = definition(q, own, lens, prefix, p_len, scale)
     if q.dtype is torch.float16:
-        tol = tol + 2.0 ** -11 * (mag + want.abs()) + 2.0 ** -25
+        tol = tol + weights * mag + 2.0 ** -11 * want.abs() + 2.0 ** -25
         over = want.abs() - tol >= 65520.0  # beyond the type: an infinity (and near its end, either)
         assert (out[over] == torch.copysign(torch.full_like(want[over], float("inf")), want[over])).all()
         edge = want.abs() + tol >= 65520.0
@@ -307,3 +308,47 @@ def test_long_f32_sums_of_few_rows_do_not_shrink(um, backend, fmt, d):
             off += float((out[i, 0, kh * g:(kh + 1) * g].double() - want).square().sum())
             whole += float(want.square().sum())
     assert (off / whole) ** 0.5 <= 2.5e-6, (off / whole) ** 0.5
+
+
+# ---------------------------------------------------------------- f16 queries
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,g,t,p_len,n", [(3, 4, 1, 0, 300), (3, 4, 3, 0, 300), (3, 4, 4, 200, 70), (3, 7, 4, 200, 70),
+                                           (70, 4, 1, 900, 40), (2, 2, 90, 0, 200)])
+def test_f16_results_are_rounded_once(um, backend, fmt, d, b, g, t, p_len, n):
+    """Whatever the rows of an item (4, 12, 16, 28, 280 over a prefix, 180), the weights keep f32's bits and the result is
+    rounded once."""
+    rng = np.random.default_rng(b + g + t)
+    h = 2
+    own = Rows(um, fmt, *(rng.standard_normal((b, h, n, d)).astype(np.float32) for _ in range(2)))
+    prefix = Rows(um, fmt, *(rng.standard_normal((1, h, p_len, d)).astype(np.float32) for _ in range(2))) if p_len else None
+    q = dev(rng.standard_normal((b, t, g * h, d)).astype(np.float16))
+    check(um, backend, q, own, [n - i % 30 for i in range(b)], prefix, p_len, weights=0.0)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("g,t", [(4, 1), (4, 4), (3, 5), (7, 4)])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_infinite_v_that_every_token_sees(um, backend, half, d, g, t, where):
+    """An infinity of V at a position of weight makes an infinity of its sign of that dimension and nothing of the others,
+    whether its weight has a rest beside f16's leading part or none (equal scores: a weight of 2^8)."""
+    rng = np.random.default_rng(g)
+    b, h, n, p_len = 2, 2, 80, 90
+    for k_gain in (0.0, 0.5):
+        (k, v), (pk, pv) = random_rows(rng, b, h, n, d), random_rows(rng, 1, h, p_len, d)
+        k, pk = k_gain * k, k_gain * pk
+        clean = definition(q := queries(b, t, g * h, d, half, rng), Rows(um, "f16", k, v), [n] * b, Rows(um, "f16", pk, pv), p_len)
+        y = pv if where == "prefix" else v
+        y[:, :, 20, 3], y[:, :, 41, 17] = np.inf, -np.inf
+        out = torch.empty_like(q)
+        backend.prefix_attention(q, Rows(um, "f16", k, v).view, dev(np.array([n] * b, np.int32)), out,
+                                 prefix=Rows(um, "f16", pk, pv).view, prefix_len=p_len)
+        backend.synchronize()
+        assert (out[..., 3] == np.inf).all() and (out[..., 17] == -np.inf).all()
+        rest = [x for x in range(d) if x not in (3, 17)]
+        want, tol, _ = (x[..., rest] for x in clean)
+        tol = tol + (2.0 ** -11 * want.abs() + 2.0 ** -25 if half else 0)
+        assert ((out[..., rest].double() - want).abs() <= tol).all()

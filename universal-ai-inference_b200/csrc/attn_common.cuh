@@ -18,15 +18,16 @@ constexpr int kWarps = 4;        // narrow: warps of a CTA
 constexpr int kNarrowCtas = 3;   // narrow: CTAs per SM (wide: one)
 constexpr int kMaxScan = 512;    // sequences whose unit counts a CTA sums itself
 constexpr float kLog2e = 1.4426950408889634f;
-// A position's weight is 2^(s - m + 8) in the denominator, and that times V's row scale (1 in an f16 cache) where it meets
+// A position's weight is 2^(s - m + 9) in the denominator, and that times V's row scale (1 in an f16 cache) where it meets
 // V's bytes.  Only the second becomes f16, so a row's reference m is a whole number at or above the largest product 2^s vs
 // so far, not the largest score: a V row much larger than the others does not push them out of f16's range unless its
 // product outweighs theirs.  (A reference made from the scales alone lost 2e-4 of a result beside a row 10^6 times
 // larger whose own weight was 0, and all of it beside one 10^12 times larger.)  m moves only when a product has come to
-// be near f16's end: the sums are then seldom rescaled, and f16 keeps 11 bits of a product down to 2^-22 of the largest.
+// be near f16's end: the sums are then seldom rescaled, and the two f16 parts of a product (split_weights) are off by at most
+// 2^-22 of it or 2^-32 of the largest, whichever is more.
 // The denominator is f32 and may lie far from 1; V rows of scale 0, whose products ask for no reference, are held within
 // it by kOver.
-constexpr float kLift = 8.0f, kSlack = 6.0f, kOver = 96.0f;
+constexpr float kLift = 9.0f, kSlack = 6.0f, kOver = 96.0f;
 constexpr float kMostProduct = 15.f, kMostWeight = 110.f;  // binary orders
 constexpr float kLeastScale = 0x1p-96f;
 
@@ -125,6 +126,22 @@ __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_
 // h, but the smallest half of s's sign rather than 0 unless s is 0.
 __device__ __forceinline__ __half but_zero(__half h, float s) {
   return __hisnan(h) || (__half_as_ushort(h) & 0x7fff) || s == 0.f ? h : __ushort_as_half(s < 0.f ? 0x8001 : 1);
+}
+
+// Two weights as leading parts, cut off after f16's 11 bits, and what that left, rounded: off by at most 2^-22 of the weight
+// or 2^-25, and below 2^-14, where the leading part is rounded again, by 2^-24.  (Rounding the leading part and taking the rest from its value makes a longer chain:
+// 128 sequences behind 32801 positions took 130.8 us against 124.9.)  INFINITE: V may hold infinities and both parts meet
+// it in one accumulator, so the rest is not 0 where there is a leading part (0 * inf is NaN).
+template <bool INFINITE>
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t& lead, uint32_t& rest) {
+  const float u = __uint_as_float(__float_as_uint(x) & 0xffffe000u), v = __uint_as_float(__float_as_uint(y) & 0xffffe000u);
+  lead = half2_bits(__floats2half2_rn(u, v));
+  float c = x - u, d = y - v;
+  if constexpr (INFINITE) {
+    c = fmaxf(c, fminf(x, 0x1p-24f));
+    d = fmaxf(d, fminf(y, 0x1p-24f));
+  }
+  rest = half2_bits(__floats2half2_rn(c, d));
 }
 
 // Two pairs of stored bytes -> two f16 pairs.  i8: a byte u behind 0x64 is the half 1024 + u, less 1152 = u - 128.

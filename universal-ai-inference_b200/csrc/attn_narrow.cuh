@@ -27,7 +27,7 @@ template <int F, int HD, bool FOLD, int KEYS, bool F32>
 struct Rows {
   static constexpr int kPer = FOLD ? 1 : 2;  // logical rows of a lane in one MMA tile
   static constexpr int kPieces = HD * Tile<F, HD, KEYS>::kEsz / 16;  // 16-byte pieces of a row
-  // The two parts of a weight resolve 2^-24, f16's smallest step.  Smaller weights are added in passes of their own,
+  // The two parts of a weight resolve 2^-24, f16's smallest step (2^-33 of the largest).  Smaller weights are added in passes of their own,
   // 20 binary orders at a time, raised to [2^-6, 2^14): only very uneven scores (22 e-foldings) need them.
   static constexpr bool kFar = FOLD;
   static constexpr float kNear = 0x1p-24f;
@@ -178,7 +178,7 @@ struct Rows {
     float low = 1.f;  // the smallest
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
-      uint32_t p[4];
+      uint32_t p[4], rest[4];
       operand(n, [&](int r, int n, int i) {
         if (!seen(r, n, i)) return 0.f;
         float e;
@@ -186,8 +186,11 @@ struct Rows {
         l[r] += e;
         if (kFar) low = fminf(low, w);
         return kFar && w < kNear ? 0.f : w;
-      }, p);
-      products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) { mma16816(o[c], p, b0, b1); });
+      }, p, rest);
+      products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) {
+        mma16816(o[c], p, b0, b1);
+        if constexpr (!FOLD) mma16816(o[c], rest, b0, b1);
+      });
     }
     if constexpr (kFar) {
       if (__any_sync(0xffffffffu, low < kNear)) {
@@ -195,12 +198,12 @@ struct Rows {
         for (float top = kNear, up = 0x1p38f, down = 0x1p-38f; top > 0x1p-110f; top *= 0x1p-20f, up *= 0x1p20f, down *= 0x1p-20f) {
 #pragma unroll
           for (int n = 0; n < NT; n += 2) {
-            uint32_t p[4];
+            uint32_t p[4], rest[4];
             operand(n, [&](int r, int n, int i) {
               float e;
               const float w = weight(r, n, i, e);
               return seen(r, n, i) && w >= top * 0x1p-20f && w < top ? w * up : 0.f;
-            }, p);
+            }, p, rest);
             if (__any_sync(0xffffffffu, (p[0] | p[2]) != 0))
               products(v_base, key + 8 * n, [&](int c, uint32_t b0, uint32_t b1) {
                 float y[4] = {};
@@ -214,20 +217,16 @@ struct Rows {
     }
   }
 
-  // Weights of 16 keys as an operand: weight(r, n, i).
+  // Weights of 16 keys, weight(r, n, i), as an operand: leading parts, and what their rounding left, in rows of its own (FOLD)
+  // or as a second operand.
   template <typename W>
-  __device__ __forceinline__ void operand(int n, W&& weight, uint32_t (&p)[4]) {
+  __device__ __forceinline__ void operand(int n, W&& weight, uint32_t (&p)[4], uint32_t (&rest)[4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < kPer; ++r) {
         const float x = weight(r, n + h, 0), y = weight(r, n + h, 1);
-        const __half2 lead = __floats2half2_rn(x, y);
-        p[2 * h + r] = half2_bits(lead);
-        if constexpr (FOLD) {
-          const float2 z = __half22float2(lead);
-          p[2 * h + 1] = half2_bits(__floats2half2_rn(x - z.x, y - z.y));
-        }
+        split_weights<F == kKvF16 && !FOLD>(x, y, p[2 * h + r], FOLD ? p[2 * h + 1] : rest[2 * h + r]);
       }
   }
 

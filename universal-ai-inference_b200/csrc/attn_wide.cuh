@@ -276,7 +276,7 @@ __device__ void wide_products(const PrefixAttnArgs& a, const Plan& p, const Seqs
         wait(&sh.p_full[r][h], mine & 1);
         if (umma::elect_one()) {
 #pragma unroll
-          for (int part = 0; part < (SPLIT_Q ? 2 : 1); ++part)
+          for (int part = 0; part < 2; ++part)  // leading parts of the weights, then the rests
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks)
               umma::mma_f16_ts(to, ts + 32 * h + 16 * part + 8 * ks, v + 2 * (2 * h + ks), kIdO, summed || h || part || ks);
@@ -342,7 +342,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 constexpr int kHalf = kTile / 2;  // keys of a half
 
 // The largest sum of a half's weights, times the tile's largest V scale, for which every product is surely an f16.  (At or
-// below the reference products are at most 2^8.)
+// below the reference products are at most 2^9.)
 constexpr float kMostSum = 46000.f;
 
 // Operand position -> dimension: K's words hold four consecutive dimensions of a byte row, which lie in two chunks of an
@@ -529,7 +529,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
         const float *kf = &sh.kf[o][kHalf * h], *vf = &sh.vf[o][kHalf * h];
         // Weights against the reference as it is, and the operand made of them; their sum tells whether one is too
         // large.  No maximum is made then.  (cut: columns from `seen` on get no weight, whatever their scale is.)
-        uint32_t pk[kHalf / 2];
+        uint32_t pk[kHalf / 2], rests[kHalf / 2];
         auto weights = [&](auto cut) {
           const float off = kLift - (m == -INFINITY ? 0.f : m);
           float2 sum[2] = {};
@@ -558,13 +558,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
                   if (j + 2 * k + 1 >= seen) w[k].y = 0.f;
                 }
               }
-              const __half2 e = __floats2half2_rn(w[k].x, w[k].y);
-              pk[j / 2 + k] = half2_bits(e);
-              if constexpr (SPLIT_Q) {  // what the rounding left
-                const float2 z = __half22float2(e);
-                s[j + 2 * k] = w[k].x - z.x;
-                s[j + 2 * k + 1] = w[k].y - z.y;
-              }
+              split_weights<F == kKvF16>(w[k].x, w[k].y, pk[j / 2 + k], rests[j / 2 + k]);
             }
           }
           return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
@@ -611,11 +605,7 @@ __device__ void wide_softmax(const PrefixAttnArgs& a, const Plan& p, const Seqs&
         }
         l += sum;
         tmem_st16(tsh, pk);
-        if constexpr (SPLIT_Q) {
-#pragma unroll
-          for (int j = 0; j < kHalf / 2; ++j) pk[j] = half2_bits(__floats2half2_rn(s[2 * j], s[2 * j + 1]));
-          tmem_st16(tsh + kHalf / 2, pk);
-        }
+        tmem_st16(tsh + kHalf / 2, rests);
         umma::tmem_st_wait();
         umma::tc_fence_before();
         __syncwarp();

@@ -20,8 +20,11 @@
 //           the work, and the kernel is near the cache's bytes).
 //   wide    (attn_wide.cuh) 128 or 256 rows on tcgen05, operands made once for all rows (many rows: the products and the
 //           exponentials are the work).
-// f32 queries are split in two f16 parts, and so are the probabilities: rows 0-7 of an MMA hold the leading parts and
-// rows 8-15 the rests ("folded"), which keeps f32 accuracy at no cost while an item has no more than 8 rows.
+// f32 queries are split in two f16 parts, and so are the weights of all queries: rows 0-7 of an MMA hold the leading parts
+// and rows 8-15 the rests ("folded"), which keeps f32 accuracy at no cost while an item has no more than 8 rows; items of
+// more rows add a second product with the rests.  Weights of f16 queries in one part cost less (128 sequences behind 32801
+// positions 117.4 against 122.4 us, 64 behind 8192 47.7 against 49.4, items of 16 rows 70 against 78) but a result's error
+// was 2.9e-4 where its own rounding to f16 makes 2.1e-4, and which of the two a call got went by its rows.
 #include <algorithm>
 
 #include "attn_narrow.cuh"
