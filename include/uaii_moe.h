@@ -466,7 +466,9 @@ UAII_MOE_API int uaii_moe_kv_read(uaii_moe_backend* b, const uaii_moe_kv_cache* 
  * prefix_len 0; same format, head_dim and n_kv_heads as `own`.  q: view [batch, n_tokens, n_heads, head_dim] of f32
  * or f16 with a dense last dimension; n_heads a multiple of n_kv_heads, query head h reading kv head
  * h / (n_heads / n_kv_heads).  scale 0 means 1 / sqrt(head_dim).  out [batch, n_tokens, n_heads, head_dim] of q's
- * type, dense, 16-byte aligned. */
+ * type, dense, 16-byte aligned.  Sums are f32.  A position's weight, times V's row scale in the 8-bit formats, enters its
+ * products off by at most 2^-22 of itself or 2^-32 of the row's largest, whichever is more; f32 queries by 2^-22 of the
+ * row's largest value. */
 UAII_MOE_API int uaii_moe_prefix_attention(uaii_moe_backend* b, const uaii_moe_kv_cache* prefix, int64_t prefix_len,
                                            const uaii_moe_kv_cache* own, const int32_t* own_len, const void* q,
                                            int dtype, int64_t n_heads, int64_t n_tokens, int64_t stride_batch,

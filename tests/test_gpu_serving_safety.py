@@ -137,3 +137,44 @@ def test_sample_from_several_threads_with_other_vocabularies(um):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+def test_calls_captured_in_a_graph(um):
+    """A decode step's operators captured in a CUDA graph on the backend's stream: a replay gives what the calls gave."""
+    st = torch.cuda.Stream()
+    be = um.Backend(0, stream=st.cuda_stream)
+    try:
+        rng = np.random.default_rng(0)
+        b, h, hd = 40, 2, 128
+        own, prefix = Cache(um, "i8", b, h, 400, hd, rng), Cache(um, "i8", 1, h, 600, hd, rng)
+        lens = dev((np.arange(b) * 9 % 400).astype(np.int32))
+        q, drafts = torch.randn((b, 1, 8, hd), device="cuda"), torch.randn((b, 4, 16, hd), device="cuda").half()
+        outs = [torch.empty_like(q), torch.empty_like(drafts), torch.empty(b, dtype=torch.int32, device="cuda")]
+        x, f, i = torch.randn((b, 32000), device="cuda"), torch.ones(b, device="cuda"), torch.zeros(b, dtype=torch.int32, device="cuda")
+        settings = f, i + 40, f * 0.9, f * 0, f * 0.5
+        row, pos = torch.randn((b, 1, h, hd), device="cuda"), i + 399
+        torch.cuda.synchronize()
+
+        def step():
+            be.kv_append(own.view, row, row, pos)
+            be.prefix_attention(q, own.view, lens, outs[0], prefix=prefix.view, prefix_len=600)
+            be.prefix_attention(drafts, own.view, lens, outs[1], prefix=prefix.view, prefix_len=600)
+            be.sample(x, *settings, outs[2])
+
+        with torch.cuda.stream(st):
+            step()
+        be.synchronize()
+        want = [t.clone() for t in outs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            step()
+        for t in outs:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, t) for a, t in zip(want, outs))
+        be.synchronize()
+    finally:
+        be.close()

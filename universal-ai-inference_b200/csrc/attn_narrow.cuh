@@ -8,9 +8,9 @@ namespace attn {
 
 // Narrow: every warp is a worker of its own, with its own copies: kKeys positions at a time, the next ones while it
 // works.  Three CTAs of four warps hold 200 KB of an SM, about half of it in flight.
-// A step of 32 keys of 128 dimensions takes a warp about 800 instructions (bytes to f16 a third of them) and, with twelve
-// warps an SM, 4000 cycles; 32 sequences of 4096 i8 positions (268 MB) take 56 us, 4.8 TB/s, 0.74 of a copy's rate: the
-// instructions and the bytes are close to one another.  A further piece costs a warp about 7000 cycles.
+// A step of 32 keys of 128 dimensions takes a warp about 780 instructions (bytes to f16 a third of them); 32 sequences
+// around 4096 i8 positions (275 MB) take 51.5 us, 5.3 TB/s, 0.83 of a copy's rate, at half the issue rate: a warp's chain
+// from copied bytes over scores and weights to sums is what it waits for.  A further piece costs a warp about 7000 cycles.
 template <int F, int HD>
 struct Narrow {
   static constexpr int kKeys = F == kKvF16 && HD == 128 ? 16 : 32;

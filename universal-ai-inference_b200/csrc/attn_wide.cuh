@@ -10,11 +10,11 @@
 // that held S -> O += P V, P from tensor memory.  Q and P in tensor memory leave shared memory's bandwidth to K and V:
 // with Q there as well, S alone would read 6 KB per 32 cycles of products.  S and P go by halves of 32 keys: while a
 // warpgroup makes one half's weights, the other half's products and the next scores are under way.
-// A key tile of 256 f16 rows takes about 2800 cycles, 1220 of them products (1032 in the exponential unit, 1500 of shared
-// memory): 512 rows a kv head, 8 kv heads, 32801 i8 positions 94 us, 0.73 PFLOP/s (0.44 of a plain bf16 product's measured
-// rate); products, conversions, exponentials and shared memory each make up no more than 20 us of it.  A CTA's first
-// scores come after 12000 cycles; a further piece costs about seven tiles.  Taking the next piece's queries in before a
-// piece's sums go out was no faster (registers at their limit: 125 against 123 us).
+// A key tile of 256 f16 rows takes about 3400 cycles, 1930 of them products (the tensor pipe's active half; the weights'
+// rests are a third of them): 512 rows a kv head, 8 kv heads, 32801 i8 positions 109 us, 0.63 PFLOP/s of the formula's
+// operations, 0.38 of a plain bf16 product's measured rate.  The weights of a half are made by one thread a row at the
+// limit of its registers, and do not hide under the other half's products.  A CTA's first scores come after 12000 cycles;
+// a further piece costs about seven tiles.  Taking the next piece's queries in before a piece's sums go out was no faster.
 // Tensor memory: S and P of tile r, half h at column 64 r + 32 h, Q at 128 + 64 r, O at 256 + 128 r.
 #pragma once
 

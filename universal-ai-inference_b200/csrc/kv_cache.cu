@@ -9,9 +9,10 @@
 // fault shows wherever the row is used instead of turning into finite values.  Every step is one IEEE
 // operation, so the bytes are the same on every run and equal the formula's.
 //
-// Both kernels make one pass and keep nothing between rows.  4 x 4096 tokens of 8 heads of 128 (f16 to e4m3 and back to
-// f16, 100 MB each way): the append 22.8 us (4.4 TB/s: 16 values a thread, since index, maximum and two divisions cost a
-// thread as much as the conversions; with 8 values 29.5 us), the read 13.5 us (the bytes partly still in L2).  16 values
+// Both kernels make one pass and keep nothing between rows.  Prompts of 4096 tokens and fewer, 8 heads of 128, f16 to e4m3
+// and back to f16: the append of 12450 tokens (77 MB) 22.8 us, 3.4 TB/s, 0.52 of a copy's rate (16 values a thread, since
+// index, maximum and two divisions cost a thread as much as the conversions; with 8 values 29.5 us), the read of 4 x 4096
+// (102 MB) 13.5 us, the bytes partly still in L2.  16 values
 // a thread made the read slower (20 against 13.5 us): its stores then lie 32 bytes apart.  A token or two is bound by
 // the launch.
 #include <cuda_fp16.h>

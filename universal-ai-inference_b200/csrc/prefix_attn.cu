@@ -5,7 +5,7 @@
 //
 // with c_j, c'_j the stored K and V values of position j and ks_j, vs_j their row scales (1 for f16).
 // Token t of sequence b sees prefix positions [0, P) and own positions [0, own_len[b] - T + t]; a row that sees
-// none is zero.  Running maximum, sums and outputs are f32.
+// none is zero.  References, sums and outputs are f32.
 //
 // Work.  An item is a tile of query rows that read the same keys: (kv head, rows of the whole batch) over the
 // prefix, (sequence, kv head, rows) over own positions.  Its keys come in units, a few more of them in front of each
@@ -17,13 +17,13 @@
 // Two tilings, one kernel each.  Bytes become exact f16 operands (the row scales act on scores and probabilities);
 // accumulators are f32.
 //   narrow  (attn_narrow.cuh) 8 or 16 rows; every warp takes other keys, from copies of its own (few rows: the keys are
-//           the work, and the kernel is near the cache's bytes).
+//           the work).
 //   wide    (attn_wide.cuh) 128 or 256 rows on tcgen05, operands made once for all rows (many rows: the products and the
 //           exponentials are the work).
 // f32 queries are split in two f16 parts, and so are the weights of all queries: rows 0-7 of an MMA hold the leading parts
 // and rows 8-15 the rests ("folded"), which keeps f32 accuracy at no cost while an item has no more than 8 rows; items of
 // more rows add a second product with the rests.  Weights of f16 queries in one part cost less (128 sequences behind 32801
-// positions 117.4 against 122.4 us, 64 behind 8192 47.7 against 49.4, items of 16 rows 70 against 78) but a result's error
+// positions 117.6 against 132.8 us, 64 behind 8192 47.4 against 49.3, items of 16 rows 70 against 78) but a result's error
 // was 2.9e-4 where its own rounding to f16 makes 2.1e-4, and which of the two a call got went by its rows.
 #include <algorithm>
 
@@ -97,8 +97,8 @@ __device__ __forceinline__ Pieces pieces_of(const PrefixAttnArgs& a, const Plan&
 
 // out = sum over a row's pieces of 2^(m - M) o / sum of 2^(m - M) l.  WARPS warps per row; the pieces are taken in the
 // order of the workers, prefix first, a warp every WARPS-th.  Bound by latency (lengths, then maxima, then sums: 4 to 8 us
-// whatever the rows); inside the narrow kernel, by the worker that comes last, it cost more (67 against 63 us at 64 rows
-// behind 8192 positions).  px, po: the plans of the kernels that took the prefix and
+// whatever the rows); inside the narrow kernel, by the worker that comes last, it cost more (6 % of a call of 64
+// sequences behind 8192 positions).  px, po: the plans of the kernels that took the prefix and
 // the own items.  cum is not __restrict__: it is written while this grid waits, and a load of data declared unchanging may
 // be moved in front of the wait.
 template <int HD, typename Q, int WARPS>
@@ -248,11 +248,11 @@ Layout lay_out(const PrefixAttnArgs& a, char* ws) {
     const int each = wide ? 1 : kWarps, full = kSms * (wide ? 1 : kNarrowCtas);  // workers of a CTA, CTAs
     p.grid = (int)(most < full * each ? (most + each - 1) / each : full);
     p.workers = p.grid * each;
-    // A piece costs more than its keys (sums out, other queries in: 58000 cycles for 7 wide tiles in two pieces, 41000
-    // in one), so every item counts as kWideLead tiles or kNarrowLead steps longer.  64 rows behind 8192 positions, 24 x 4
-    // tokens behind 4101: 62.3 and 66.8 us without, 51.6 and 43.1 with 3 tiles, 49.2 and 41.5 with 7 (45 with f32 sums
-    // taken out); 32 rows of 4096
-    // own positions: 64.1, 62.2, 61.5 and 60.0 us with 0, 1, 2 and 4 steps, 64 rows behind 8192 62.2, 58.2, 57.5, 58.7.
+    // A piece costs more than its keys (sums out, other queries in), so every item counts as kWideLead tiles or
+    // kNarrowLead steps longer.  With 0, 3, 7 and 9 tiles 64 sequences behind 8192 positions take 55.5, 51.6, 49.3 and
+    // 49.4 us, 24 x 4 tokens behind 4101 66.0, 48.5, 44.9 and 46.6, 128 sequences behind 32801 129.1, 125.2, 123.9 and
+    // 123.2; with 0, 1, 2 and 4 steps 32 sequences of 4096 own positions 59.9, 58.3, 58.0 and 58.3, 64 behind 8192 52.7,
+    // 49.4, 49.3 and 49.5.
     p.lead = wide ? kWideLead : kNarrowLead;
     p.prefix_units = tiles ? tiles + p.lead : 0;
     l.most = std::max(l.most, most + p.lead * (p.prefix_items + own_items));
@@ -323,7 +323,7 @@ cudaError_t run_all(const PrefixAttnArgs& a, const Layout& l, const int32_t* giv
   if (l.prefix.grid) e = l.prefix_wide ? wide(l.prefix) : narrow(l.prefix, false);
   if (e == cudaSuccess) e = l.own_wide ? wide(l.own) : narrow(l.own, l.prefix.grid > 0);
   if (e != cudaSuccess) return e;
-  // four warps a row up to what the GPU holds at once (2048 rows 54.4 against 55.6 us with one; 4096 rows 130 against 124)
+  // four warps a row up to what the GPU holds at once (2048 rows 49.3 against 50.8 us with one; 4096 rows 129 against 124)
   const int64_t rows = a.B * a.T * a.H;
   const bool few = rows <= 16 * kSms;
   const auto kern = a.half ? (few ? join_kernel<HD, __half, 4> : join_kernel<HD, __half, 1>)

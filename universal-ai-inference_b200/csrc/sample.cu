@@ -13,10 +13,10 @@
 // A cluster of up to eight CTAs holds a row: every logit is read once and its weight kept in shared memory.  The cut is
 // found with one histogram over the weights' leading bits and a ranking, by logit, of the few tokens of one bin; counts,
 // sums and bins of the CTAs meet through distributed shared memory.
-// 256 rows of 151936 f16 logits take 270 us (77 MB read once, which alone would be 12 us): 127 instructions a logit at
+// 256 rows of 151936 f16 logits take 273 us (77 MB read once, which alone would be 12 us): 127 instructions a logit at
 // 0.55 of the issue rate, with two CTAs an SM; of a CTA's 60000 cycles 10000 go to reading, 7000 to weights, 8000 to the
 // histogram's atomics, 7000 to ranking, 6000 to the kept mass and 15000 to seven cluster barriers.  A single row takes
-// 20 us, 13.5 of which the caller's side of the call.
+// 20 us on the device: passes over a few logits a thread and seven barriers, one after the other.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>
@@ -189,7 +189,7 @@ struct Row {
   static __device__ __forceinline__ int low_at(int bin) { return 2 * bin + (bin >> 4 & 1); }
   // The bin, from the highest down, at which the cluster's bins reach `goal`: sh.bin and sh.above (plus `above`).  Remote
   // shared memory gave 4 to 5 bytes a cycle to an SM, so bins are read in 512-byte pieces and are no more than
-  // 512: 1024 took 4 us more, 256 left longer lists to rank (381 against 341 us at 256 rows of 151936).
+  // 512: 1024 took 4 us more, 256 left longer lists to rank (a tenth more at 256 rows of 151936).
   __device__ __forceinline__ void reach(uint64_t goal, uint64_t above) {
     constexpr int kEach = kMaxCluster / kGroups;
     const int t = threadIdx.x, at = t % (kBins / 2), group = t / (kBins / 2);
