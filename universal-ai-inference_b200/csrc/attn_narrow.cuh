@@ -27,16 +27,16 @@ template <int F, int HD, bool FOLD, int KEYS, bool F32>
 struct Rows {
   static constexpr int kPer = FOLD ? 1 : 2;  // logical rows of a lane in one MMA tile
   static constexpr int kPieces = HD * Tile<F, HD, KEYS>::kEsz / 16;  // 16-byte pieces of a row
-  // The two parts of a weight resolve 2^-24, f16's smallest step (2^-33 of the largest).  Smaller weights are added in passes of their own,
-  // 20 binary orders at a time, raised to [2^-6, 2^14): only very uneven scores (22 e-foldings) need them.
+  // The two parts of a weight resolve 2^-24, f16's smallest step (2^-33 of the largest).  Smaller weights are added in passes
+  // of their own, 20 binary orders at a time, raised to [2^-6, 2^14): only very uneven scores (22 e-foldings) need them.
   static constexpr bool kFar = FOLD;
   static constexpr float kNear = 0x1p-24f;
   float o[HD / 8][4];
   float m[kPer], l[kPer];  // the reference (attn_common.cuh), the denominator
   float f[kPer];           // score factor: scale * log2(e), and the power of two taken out of a folded row of q
   int lim[kPer];           // positions the row sees
-  // The tensor cores cut sums off where they should round (half of f32's last place at each addition, 1e-5 of a sum after
-  // the 1500 of a warp's 750 steps), so f32 sums are taken out after 32 additions and added up in f32.
+  // The tensor cores cut sums off where they should round (half of f32's last place at each addition: 1e-5 of a sum was
+  // measured after the 650 of 320 steps), so f32 sums are taken out after 32 additions and added up in f32.
   static constexpr bool kTake = FOLD && F32;
   static constexpr int kTakeSteps = 32 / (KEYS / 16);
   float taken_m;           // their reference
@@ -57,6 +57,7 @@ struct Rows {
       m[r] = -INFINITY;
       l[r] = 0.f;
     }
+    taken_m = -INFINITY;
   }
 
   // Keys [key, key + 8 NT) of the tile at k_base / v_base, which starts at position pos0; masked says that some row may not

@@ -15,8 +15,8 @@
 // sums and bins of the CTAs meet through distributed shared memory.
 // 256 rows of 151936 f16 logits take 273 us (77 MB read once, which alone would be 12 us): 127 instructions a logit at
 // 0.55 of the issue rate, with two CTAs an SM; of a CTA's 60000 cycles 10000 go to reading, 7000 to weights, 8000 to the
-// histogram's atomics, 7000 to ranking, 6000 to the kept mass and 15000 to seven cluster barriers.  A single row takes
-// 20 us on the device: passes over a few logits a thread and seven barriers, one after the other.
+// histogram's atomics, 7000 to ranking, 6000 to the kept mass and 15000 to cluster barriers.  A single row takes
+// 20 us on the device: passes over a few logits a thread and cluster barriers, one after the other.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <type_traits>
